@@ -41,6 +41,36 @@ class QdEpi(C.Structure):
                 ("res_ws", i64)]
 
 
+class Norm(C.Structure):
+    """bnh_norm: one norm over a row (kind 0 none, 1 RMS, 2 layer)."""
+    _fields_ = [("kind", i32), ("eps", C.c_float), ("w", vp), ("b", vp)]
+
+
+class BlockNorm(C.Structure):
+    """bnh_bnorm: the norms around a block with its gate and residual."""
+    _fields_ = [("f", vp), ("f_ws", i64), ("ldf", i32), ("f16", i32),
+                ("post", Norm), ("gate", vp), ("g_ws", i64), ("ldg", i32),
+                ("gate_act", i32), ("scale", vp), ("rs", C.c_float),
+                ("x", vp), ("x_ws", i64), ("ldx", i32), ("x16", i32),
+                ("y", vp), ("y_ws", i64), ("ldy", i32), ("pre", Norm),
+                ("n", vp), ("n_ws", i64), ("ldn", i32)]
+
+
+class Lora(C.Structure):
+    """bnh_lora: low-rank adapters of one projection (device pointers)."""
+    _fields_ = [("n", i32), ("r", i32), ("a", vp), ("b", vp), ("scale", vp)]
+
+
+class LinAttn(C.Structure):
+    """bnh_la: linear attention with a decay for each head."""
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("o", vp), ("f16", i32),
+                ("ldq", i32), ("ldk", i32), ("ldv", i32), ("ldo", i32),
+                ("H", i32), ("Hq", i32), ("Hk", i32), ("Hv", i32),
+                ("dk", i32), ("dv", i32), ("g", vp), ("ldg", i32),
+                ("scale", C.c_float), ("s0", vp), ("s1", vp), ("slots", i32),
+                ("slot", vp)]
+
+
 _SIGS = {
     "bnh_last_error": (C.c_char_p, []),
     "bnh_device_count": (i32, []),
@@ -151,6 +181,12 @@ _SIGS = {
     "bnh_fproto_free": (None, [vp]),
     "bnh_l2norm_cells": (i32, [vp, i64, i32, i32, i32, C.c_float, i32, vp, i64, i32, vp]),
     "bnh_fproto_colmax": (i32, [vp, i64, i32, vp, vp, i64, i32, vp]),
+    "bnh_block_norm": (i32, [C.POINTER(BlockNorm), i32, i32, i32, vp]),
+    "bnh_pw_lora_work_bytes": (C.c_size_t, [i32, i32, i32, i32, i32]),
+    "bnh_pw_lora": (i32, [vp, i64, i32, i32, i32, vp, i32, i32, i32, vp, C.POINTER(Lora), vp, C.POINTER(Epi16), vp,
+                          C.c_size_t, vp]),
+    "bnh_linattn_work_bytes": (C.c_size_t, [C.POINTER(LinAttn), i32, i32]),
+    "bnh_linattn": (i32, [C.POINTER(LinAttn), i32, i32, i32, vp, vp, vp, C.c_size_t, vp]),
 }
 
 

@@ -32,6 +32,9 @@ SOURCES = [
     "kern_qdot.hip",
     "kern_fe.hip",
     "kern_f32.hip",
+    "kern_bnorm.hip",
+    "kern_lora.hip",
+    "kern_linattn.hip",
     "pkg_file.cpp",
     "rt_contract.cpp",
     "rt_pkg.cpp",

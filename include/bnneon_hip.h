@@ -428,6 +428,98 @@ int bnh_gem_a(const float *F, long long f_ws, int M, int C, float eps, float p, 
 /* test hook: the family's scalar functions elementwise (f 0 exp2_p5, 1 silu_f32_a, 2 log2_f32, 3 the SE sigmoid) */
 int bnh_eval_qd(int f, const float *x, float *y, long long n, void *stream);
 
+/* ------------------------------------------------------------------ temporal context over windows
+ * What looks from one window of a recording to the next, over embeddings: no counterpart in the reference, which scores every
+ * window by itself. The rows of a station (one a window, in time order) go through blocks of
+ *   n = norm(x), projections with the station's adapter, linear attention with a decay, x += scale gate norm(f),
+ * an archive with all its rows at once, a live station with one row a call and its state kept between calls. Values are
+ * fp32 or fp16 (bit patterns); statistics, sums and states are fp32. Outputs share no memory with inputs but where said. */
+/* one norm over a row u of C values: kind 0: u, 1 (RMS): u / sqrt(mean(u^2) + eps) w + b, 2 (layer):
+ * (u - mean(u)) / sqrt(var(u) + eps) w + b; w, b fp32 [C] on the device, NULL: 1 and 0 */
+typedef struct {
+  int kind;
+  float eps;
+  const float *w, *b;
+} bnh_norm;
+/* y = x + rs scale[c] act(gate) post(f), n = pre(y): the exit of a block with its norm, gate and residual scale and the
+ * entry of the next in one pass. f NULL: y = x (the entry alone); x NULL: y without the residual (f's norm and gate alone);
+ * gate or scale NULL: 1; y or n NULL: not stored. pre's statistics are those of y before it is rounded. Strides in
+ * elements, the _ws between windows; ldg 0: one gate row [C] for a window's rows. y may lie over x, n over f or over a
+ * gate of rows (ldg != 0), each with its input's type, rows and strides. C <= 16384. */
+typedef struct {
+  const void *f;
+  long long f_ws;
+  int ldf;
+  int f16;            /* type of f, gate and n: 0 fp32, 1 fp16 */
+  bnh_norm post;
+  const void *gate;
+  long long g_ws;
+  int ldg;
+  int gate_act;       /* of the gate: 0 none, 1 SiLU, 2 ReLU, 3 sigmoid */
+  const float *scale; /* fp32 [C] */
+  float rs;
+  const void *x;
+  long long x_ws;
+  int ldx;
+  int x16;            /* type of x and y: 0 fp32, 1 fp16 (with f16 1 only) */
+  void *y;
+  long long y_ws;
+  int ldy;
+  bnh_norm pre;
+  void *n;
+  long long n_ws;
+  int ldn;
+} bnh_bnorm;
+int bnh_block_norm(const bnh_bnorm *p, int M, int C, int B, void *stream);
+
+/* low-rank adapters of one projection, fp16 on the device: a [n][r][K], b [n][N][r], scale fp32 [n] (NULL: 1); r <= 256 */
+typedef struct {
+  int n, r;
+  const uint16_t *a, *b;
+  const float *scale;
+} bnh_lora;
+/* A shared fp16 projection with the adapters of many requests beside it: every row x of window i gives
+ * out = act(w x + bias + scale[j] b[j] (a[j] x)) (+ res), j = idx[i]; no adapter for a j outside [0, L->n).
+ * w fp16 rows [N][ldw >= K], bias fp32 [N] (NULL: 0), idx int32 [B] on the device; L NULL: no adapters. The epilogue is
+ * e's with rows only (opad 0; act 1 is the fp32 SiLU x / (1 + e^-x)): fp16 MFMA with fp32 sums over all of K and r, a
+ * and x's product rounded to fp16 in between, one rounding at the end. A row depends on its own window's adapter alone,
+ * whatever the others hold. Windows of one adapter side by side are fastest. work: device scratch of at least
+ * bnh_pw_lora_work_bytes bytes, 16-byte aligned. */
+size_t bnh_pw_lora_work_bytes(int M, int B, int N, int K, int r);
+int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const uint16_t *w, int ldw, int N, int K,
+                const float *bias, const bnh_lora *L, const int32_t *idx, const bnh_epi16 *e, void *work,
+                size_t work_bytes, void *stream);
+
+/* Linear attention with a decay for each head. Per sequence and head, over the sequence's rows t in order:
+ *   S = exp(g_t) S + k_t v_t^T,  o_t = scale q_t^T S
+ * with S [dk][dv] from s0 (NULL: zeros) and left in s1 (NULL: not stored; s1 may be s0). Row r of q holds Hq heads of dk
+ * at r ldq, k Hk of dk, v Hv of dv, o H of dv, g H log decays (ldg 0: the same for every row); head h reads q head
+ * h Hq / H and so on (Hq, Hk, Hv divide H). g may be -inf (the state starts anew), and is meant to be <= 0. States are fp32
+ * [slots][H][dk][dv]; sequence i's is slot[i] (NULL: i), and a slot outside [0, slots) starts from zeros and stores
+ * nothing; no two sequences of a call share one that is stored. dk, dv <= 256. */
+typedef struct {
+  const void *q, *k, *v;
+  void *o;
+  int f16;            /* type of q, k, v and o: 0 fp32, 1 fp16 */
+  int ldq, ldk, ldv, ldo;
+  int H, Hq, Hk, Hv, dk, dv;
+  const float *g;
+  int ldg;
+  float scale;
+  const float *s0;
+  float *s1;
+  int slots;
+  const int32_t *slot;
+} bnh_la;
+/* B sequences of at most T rows among `rows` rows: sequence i has the len[i] rows from start[i] (int32 [B] on the device;
+ * NULL: T rows each, from i T), cut to T and to [0, rows); one of no rows leaves its state as it is. Sequences share no
+ * rows. T = 1 (a live station's new window) runs the recurrence, long sequences a chunked form of it with matrix products.
+ * work: device scratch of at least bnh_linattn_work_bytes bytes, 16-byte aligned (0 bytes for some shapes: NULL is
+ * allowed then). */
+size_t bnh_linattn_work_bytes(const bnh_la *p, int T, int B);
+int bnh_linattn(const bnh_la *p, int T, int B, int rows, const int32_t *start, const int32_t *len, void *work,
+                size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
