@@ -135,6 +135,539 @@ int step_run(const LaDev &d, int B, hipStream_t s) {
   return 0;
 }
 
+// The chunked form, for sequences of many rows. Over a chunk of C rows with the running sums c_i of g within it:
+//   o_i = scale (e^{c_i} q_i^T S + sum_{j <= i} e^{c_i - c_j} (q_i . k_j) v_j^T),
+//   S <- e^{c_C} S + sum_j e^{c_C - c_j} k_j v_j^T,
+// four matrix products on MFMA. Every exponent is a sum of g over the rows in between, at most 0 where g is, so nothing is
+// divided by a small decay; c is kept in 64 bits because differences of its values matter where c itself has grown
+// large, and g below -1e4 (whose e^g is 0) counts as -1e4, so that a reset's infinity does not cancel another's.
+//
+// A block of four waves owns 64 NC columns of one state over one piece of one sequence. The state stays in the accumulators of
+// the waves (16 NC columns each, all of dk): their layout is, for pairs of 16-row tiles, that of the first operand of the
+// product with q's rows, so it never passes through LDS. q, k and v of the next chunk are loaded into registers while this
+// one's are multiplied out of LDS; k's and v's transposes come out of LDS through ds_read_b64_tr_b16.
+//
+// fp16 rows: the factors of a product have to be fp16, its sums are fp32. Scores are scaled row by row and the state
+// column by column by powers of two before they are rounded (their largest to 2^12..2^13), so neither overflows and both
+// keep 11 bits, as the rounded output does. The state itself is not rounded: its update takes v_j e^{c_C - c_j}, scaled
+// the same way, in two fp16 parts of 11 bits each (the second, times 2^11, in a product of its own) against the exact k. fp32 rows run
+// on the fp32 MFMA, unscaled and unsplit.
+//
+// A row's v that is not finite would reach earlier rows of its chunk as 0 x inf; it is taken out of the product and added to
+// the rows that see it one by one (a wave that finds none skips this).
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v8f __attribute__((ext_vector_type(8)));
+typedef h16 v8h __attribute__((ext_vector_type(8)));
+typedef h16 v4h __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+// A fragment: 8 of the 32 steps of a product for row (or column) lane & 15, the same 8 of both operands in a lane
+template <typename T>
+struct Frag;
+template <>
+struct Frag<h16> {
+  typedef v8h V;   // a fragment
+  typedef v4h H;   // four values
+};
+template <>
+struct Frag<float> {
+  typedef v8f V;
+  typedef v4f H;
+};
+__device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v4f mma(v8f a, v8f b, v4f c) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+// steps 8 q + e (q = lane >> 4) of a row at p = its step 8 q
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::V row8(const T *p) {
+  return *(const typename Frag<T>::V *)p;
+}
+// steps 4 q + e and 16 + 4 q + e of a row at p = its step 4 q
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::V row44(const T *p) {
+  const typename Frag<T>::H a = *(const typename Frag<T>::H *)p, b = *(const typename Frag<T>::H *)(p + 16);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// steps 8 q + e of column lane & 15 of a matrix at p whose rows (a step each) are `ld` apart
+__device__ __forceinline__ v8h col8(const h16 *p, int ld, int lane) {
+  const h16 *a = p + (8 * (lane >> 4) + ((lane & 15) >> 2)) * ld + 4 * (lane & 3);
+  typedef __attribute__((address_space(3))) v4s L;
+  const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(a + 4 * ld));
+  typedef short v8s __attribute__((ext_vector_type(8)));
+  const v8s z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(v8h, z);
+}
+__device__ __forceinline__ v8f col8(const float *p, int ld, int lane) {
+  v8f r;
+#pragma unroll
+  for (int e = 0; e < 8; e++) r[e] = p[(8 * (lane >> 4) + e) * ld + (lane & 15)];
+  return r;
+}
+// 2^-e that takes a largest value m to 2^12..2^13: 0 and infinities are left as they are, and nothing grows past 2^24
+__device__ __forceinline__ int scale_exp(float m) {
+  const int e = (int)(__float_as_uint(m) >> 23 & 255) - 127 - 12;
+  return m == 0.f || e > 127 - 12 ? 0 : e < -24 ? -24 : e;
+}
+
+// 16 bytes of a row of `cols` values from its value c, zeros past the end; V: all of them are in or out, 16-byte aligned
+template <typename T, bool V>
+__device__ __forceinline__ uint4 row16(const T *p, int c, int cols) {
+  constexpr int VE = 16 / sizeof(T);
+  uint4 r = make_uint4(0, 0, 0, 0);
+  if (V) {
+    if (c < cols) r = *(const uint4 *)(p + c);
+  } else if (c + VE <= cols) {
+    __builtin_memcpy(&r, p + c, 16);
+  } else if (c < cols) {
+    T t[VE] = {};
+#pragma unroll
+    for (int i = 0; i < VE; i++)
+      if (c + i < cols) t[i] = p[c + i];
+    __builtin_memcpy(&r, t, 16);
+  }
+  return r;
+}
+
+// One piece of one sequence. OUT: the outputs, from the state before the piece, and s1 from the sequence's last; else the
+// state that every piece but the last adds (the first one's includes s0), into part, and its whole decay.
+template <typename T, int DKT, int NC, int C, bool V, bool OUT>
+__global__ __launch_bounds__(256) void k_la_chunk(LaDev p, int nsl, int npc, int pcr, float *part, float *pdec) {
+  constexpr bool F16 = sizeof(T) == 2;
+  constexpr int VE = 16 / sizeof(T), KD = 32 * DKT, DV = 64 * NC, SK = KD + VE, SV = DV + VE, SP = C + VE;
+  constexpr int NK = C * KD / VE / 256, NV = C * DV / VE / 256, RK = 256 * VE / KD, RV = 256 * VE / DV;
+  typedef typename Frag<T>::V FV;
+  typedef typename Frag<T>::H FH;
+  __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SK : 1], s_k[C * SK], s_v[C * SV], s_p[OUT ? C * SP : 1];
+  __shared__ double s_c[2][64];                    // c_i
+  __shared__ __attribute__((aligned(16))) float s_w[2][64];  // e^{c_C - c_j}
+  __shared__ float s_e[2][64], s_d[2];             // e^{c_i}; e^{c_C}
+  __shared__ int s_x[64];                          // the scores' scale by row
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q4 = lane >> 4;
+  unsigned lb = bnh_xcd_block(blockIdx.x, gridDim.x);
+  const int sl = (int)(lb % nsl), h = (int)(lb / nsl % p.H);
+  lb /= nsl * p.H;
+  const int pc = (int)(lb % (OUT ? npc : npc - 1)), b = (int)(lb / (OUT ? npc : npc - 1));
+  int first;
+  const int n = la_rows(p, b, &first), slot = la_slot(p, b);
+  const int r0 = pc * pcr;
+  if (OUT ? pc > 0 && r0 >= n : r0 + pcr >= n) return;  // no such piece, or a last one, whose state nobody takes
+  const int rows = n - r0 < pcr ? n - r0 : pcr;        // of this piece; 0: only a state to copy
+  const int c0 = sl * DV + wave * 16 * NC;             // this wave's columns
+  const long long pst = ((((long long)b * p.H + h) * nsl + sl) * (npc - 1)) * (KD * DV);  // this state's pieces
+  const long long at = ((long long)slot * p.H + h) * p.dk * p.dv;
+
+  v4f S[2 * DKT][NC];  // rows 16 t + 4 q4 + r, column c0 + 16 nc + lr
+  bool some = false;   // whether the state may be other than zero
+#pragma unroll
+  for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+    for (int c = 0; c < NC; c++) S[t][c] = (v4f){0.f, 0.f, 0.f, 0.f};
+  if (OUT && pc > 0) {
+    some = true;
+    const float *w = part + pst + (long long)(pc - 1) * (KD * DV) + wave * (KD * 16 * NC) + 4 * lane;
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+      for (int c = 0; c < NC; c++) S[t][c] = *(const v4f *)(w + 256 * (t * NC + c));
+  } else if (pc == 0 && p.s0 && slot >= 0) {
+    some = true;
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int kk = 16 * t + 4 * q4 + r, col = c0 + 16 * c + lr;
+          if (kk < p.dk && col < p.dv) S[t][c][r] = p.s0[at + (long long)kk * p.dv + col];
+        }
+  }
+  if (OUT) {  // the blocks right of the diagonal that a step of 32 reads
+    for (int i = tid; i < C / 32 * 256; i += 256) s_p[(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] = (T)0.f;
+  }
+
+  const int kr = tid / (KD / VE), kc = tid % (KD / VE) * VE, vr = tid / (DV / VE), vc = tid % (DV / VE) * VE;
+  const T *qp = (const T *)p.q + ((long long)first + r0 + kr) * p.ldq + h / p.rq * p.dk;
+  const T *kp = (const T *)p.k + ((long long)first + r0 + kr) * p.ldk + h / p.rk * p.dk;
+  const T *vp = (const T *)p.v + ((long long)first + r0 + vr) * p.ldv + h / p.rv * p.dv + sl * DV;
+  uint4 qn[OUT ? NK : 1], kn[NK], vn[NV];
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      const bool in = t0 + kr + RK * i < rows;
+      if (OUT) qn[i] = in ? row16<T, V>(qp + (long long)(t0 + RK * i) * p.ldq, kc, p.dk) : make_uint4(0, 0, 0, 0);
+      kn[i] = in ? row16<T, V>(kp + (long long)(t0 + RK * i) * p.ldk, kc, p.dk) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      vn[i] = t0 + vr + RV * i < rows ? row16<T, V>(vp + (long long)(t0 + RV * i) * p.ldv, vc, p.dv - sl * DV)
+                                      : make_uint4(0, 0, 0, 0);
+  };
+  // c of the chunk from row t0 and what follows from it, by one wave; rows past the end count as g = 0
+  double ctot = 0;
+  auto sums = [&](int t0, int u) {
+    float g = 0.f;
+    if (lane < C && t0 + lane < rows) g = p.g[((long long)first + r0 + t0 + lane) * p.ldg + h];
+    g = g < -1e4f ? -1e4f : g;
+    double c = g;
+#pragma unroll
+    for (int d = 1; d < C; d *= 2) {
+      const double o = __shfl_up(c, d);
+      c = lane >= d ? c + o : c;
+    }
+    const double last = __shfl(c, C - 1);
+    if (lane < C) {
+      s_c[u][lane] = c;
+      s_e[u][lane] = expf((float)c);
+      s_w[u][lane] = expf((float)(last - c));
+      if (lane == C - 1) s_d[u] = expf((float)c);
+    }
+    ctot += last;
+  };
+
+  load(0);
+  if (wave == 0) sums(0, 0);
+  int u = 0;
+  for (int t0 = 0; t0 < rows; t0 += C, u ^= 1) {
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      if (OUT) *(uint4 *)(s_q + (kr + RK * i) * SK + kc) = qn[i];
+      *(uint4 *)(s_k + (kr + RK * i) * SK + kc) = kn[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) *(uint4 *)(s_v + (vr + RV * i) * SV + vc) = vn[i];
+    __syncthreads();
+    load(t0 + C);
+
+    if (OUT && wave < C / 16) {  // scores of rows 16 wave + lr, four columns a lane in each block of 16
+      const int i = 16 * wave + lr;
+      const double ci = s_c[u][i];
+      v4f a[C / 16];
+      float m = 0.f;
+#pragma unroll
+      for (int jb = 0; jb < C / 16; jb++) a[jb] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < DKT; d++) {
+        const FV x = row8<T>(s_q + i * SK + 32 * d + 8 * q4);
+#pragma unroll
+        for (int jb = 0; jb < C / 16; jb++)
+          if (jb <= wave) a[jb] = mma(row8<T>(s_k + (16 * jb + lr) * SK + 32 * d + 8 * q4), x, a[jb]);
+      }
+#pragma unroll
+      for (int jb = 0; jb < C / 16; jb++)
+        if (jb <= wave)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int j = 16 * jb + 4 * q4 + r;
+            a[jb][r] = j <= i ? a[jb][r] * __expf((float)(ci - s_c[u][j])) : 0.f;
+            m = fmaxf(m, fabsf(a[jb][r]));
+          }
+      int x = 0;
+      if (F16) {
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        x = scale_exp(m);
+        if (q4 == 0) s_x[i] = x;
+      }
+#pragma unroll
+      for (int jb = 0; jb < C / 16; jb++)
+        if (jb <= wave) {
+          FH y;
+#pragma unroll
+          for (int r = 0; r < 4; r++) y[r] = (T)(F16 ? ldexpf(a[jb][r], -x) : a[jb][r]);
+          *(FH *)(s_p + i * SP + 16 * jb + 4 * q4) = y;
+        }
+    }
+    if (wave == 0 && t0 + C < rows) sums(t0 + C, u ^ 1);
+    FV vf[C / 32][NC];
+    bool odd = false;  // whether a value of v is not finite
+#pragma unroll
+    for (int j = 0; j < C / 32; j++)
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        vf[j][c] = col8(s_v + 32 * j * SV + wave * 16 * NC + 16 * c, SV, lane);
+        T z = (T)0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) z += vf[j][c][e] * (T)0.f;
+        odd = odd || z != z;
+      }
+    if (OUT) {
+      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+      FV sf[DKT][NC];
+      int sx[NC];
+      float xs[NC][4];  // 2^x of the accumulators' columns 4 q4 + r
+      if (some) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          sx[c] = 0;
+          if (F16) {
+            float m = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(S[t][c][r]));
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            sx[c] = scale_exp(m);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; r++) xs[c][r] = F16 ? ldexpf(1.f, __shfl(sx[c], 4 * q4 + r)) : 1.f;
+          const float dn = ldexpf(1.f, -sx[c]);
+#pragma unroll
+          for (int d = 0; d < DKT; d++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) sf[d][c][e] = (T)(F16 ? S[2 * d + e / 4][c][e % 4] * dn : S[2 * d + e / 4][c][e % 4]);
+        }
+      }
+      FV vz[C / 32][NC];
+#pragma unroll
+      for (int j = 0; j < C / 32; j++)
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          vz[j][c] = vf[j][c];
+          if (odd)
+#pragma unroll
+            for (int e = 0; e < 8; e++) vz[j][c][e] = vf[j][c][e] - vf[j][c][e] == (T)0.f ? vf[j][c][e] : (T)0.f;
+        }
+      __syncthreads();
+#pragma unroll
+      for (int ib = 0; ib < C / 16; ib++) {
+        if (t0 + 16 * ib >= rows) break;
+        const int i = 16 * ib + lr;
+        v4f a[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) a[c] = (v4f){0.f, 0.f, 0.f, 0.f};
+        const float ec = s_e[u][i], dn = F16 ? ldexpf(ec, -s_x[i]) : ec, up = F16 ? ldexpf(p.scale, s_x[i]) : p.scale;
+        if (some) {
+#pragma unroll
+          for (int d = 0; d < DKT; d++) {
+            const FV x = row44<T>(s_q + i * SK + 32 * d + 4 * q4);
+#pragma unroll
+            for (int c = 0; c < NC; c++) a[c] = mma(sf[d][c], x, a[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) a[c][r] *= xs[c][r] * dn;
+        }
+#pragma unroll
+        for (int j = 0; j <= ib / 2; j++) {
+          const FV x = row8<T>(s_p + i * SP + 32 * j + 8 * q4);
+#pragma unroll
+          for (int c = 0; c < NC; c++) a[c] = mma(vz[j][c], x, a[c]);
+        }
+        if (odd) {
+          for (int j = 0; j < 16 * ib + 16; j++) {
+            if (j > i) continue;
+            const float x = (float)s_p[i * SP + j];
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                const float y = (float)s_v[j * SV + wave * 16 * NC + 16 * c + 4 * q4 + r];
+                if (y - y != 0.f) a[c][r] += x * y;
+              }
+          }
+        }
+        if (t0 + i < rows) {
+          T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv;
+#pragma unroll
+          for (int c = 0; c < NC; c++) {
+            const int col = c0 + 16 * c + 4 * q4;
+            FH y;
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] = (T)(up * a[c][r]);
+            if (V) {
+              if (col < p.dv) *(FH *)(o + col) = y;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; r++)
+                if (col + r < p.dv) o[col + r] = y[r];
+            }
+          }
+        }
+      }
+    } else {
+      __syncthreads();
+    }
+    // the state's update
+    const float dec = s_d[u];
+    FV hi[C / 32][NC], lo[C / 32][NC];
+    float up[NC];  // what the products are multiplied by, a power of two a column
+    {
+      float w[C / 32][8];
+#pragma unroll
+      for (int j = 0; j < C / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[j][e] = s_w[u][32 * j + 8 * q4 + e];
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        float dn = 1.f;
+        up[c] = 1.f;
+        if (F16) {
+          float m = 0.f;
+#pragma unroll
+          for (int j = 0; j < C / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf((float)vf[j][c][e] * w[j][e]));
+          m = fmaxf(m, __shfl_xor(m, 16));
+          m = fmaxf(m, __shfl_xor(m, 32));
+          const int x = scale_exp(m);
+          up[c] = ldexpf(1.f, x);
+          dn = ldexpf(1.f, -x);
+        }
+#pragma unroll
+        for (int j = 0; j < C / 32; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float y = (float)vf[j][c][e] * w[j][e] * dn;
+            hi[j][c][e] = (T)y;
+            if (F16) {
+              const float d = y - (float)hi[j][c][e];
+              lo[j][c][e] = (T)(d - d == 0.f ? 2048.f * d : 0.f);
+            }
+          }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++) {
+      FV kf[C / 32];
+#pragma unroll
+      for (int j = 0; j < C / 32; j++) kf[j] = col8(s_k + 32 * j * SK + 16 * t, SK, lane);
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        if (some)
+#pragma unroll
+          for (int r = 0; r < 4; r++) S[t][c][r] *= dec;
+        if (F16) {
+          v4f l = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < C / 32; j++) l = mma(kf[j], lo[j][c], l);
+#pragma unroll
+          for (int r = 0; r < 4; r++) l[r] *= 1.f / 2048;
+#pragma unroll
+          for (int j = 0; j < C / 32; j++) l = mma(kf[j], hi[j][c], l);
+#pragma unroll
+          for (int r = 0; r < 4; r++) S[t][c][r] = __builtin_fmaf(l[r], up[c], S[t][c][r]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < C / 32; j++) S[t][c] = mma(kf[j], hi[j][c], S[t][c]);
+        }
+      }
+    }
+    some = true;
+    __syncthreads();
+  }
+  if (!OUT) {
+    float *w = part + pst + (long long)pc * (KD * DV) + wave * (KD * 16 * NC) + 4 * lane;
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+      for (int c = 0; c < NC; c++) *(v4f *)(w + 256 * (t * NC + c)) = S[t][c];
+    if (tid == 0) pdec[(((long long)b * p.H + h) * nsl + sl) * (npc - 1) + pc] = expf((float)ctot);
+  } else if (p.s1 && slot >= 0 && r0 + pcr >= n) {
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int kk = 16 * t + 4 * q4 + r, col = c0 + 16 * c + lr;
+          if (kk < p.dk && col < p.dv) p.s1[at + (long long)kk * p.dv + col] = S[t][c][r];
+        }
+  }
+}
+
+// The states before each piece from what the pieces add: part[i] <- part[i] + pdec[i] part[i - 1], in order, four values
+// a thread
+__global__ __launch_bounds__(256) void k_la_scan(LaDev p, int npc, int pcr, int quads, int nsl, float *part,
+                                                 const float *pdec) {
+  const int st = (int)(blockIdx.y), b = st / (nsl * p.H);
+  int first;
+  const int n = la_rows(p, b, &first);
+  const int np = (n + pcr - 1) / pcr - 1;  // pieces whose state a later one takes
+  const int i = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (i >= quads || np < 2) return;
+  float4 *w = (float4 *)(part + (long long)st * (npc - 1) * 4 * quads) + i;
+  const float *d = pdec + (long long)st * (npc - 1);
+  float4 s = w[0];
+  for (int k = 1; k < np; k++) {
+    const float4 x = w[(long long)k * quads];
+    const float y = d[k];
+    s = make_float4(__builtin_fmaf(y, s.x, x.x), __builtin_fmaf(y, s.y, x.y), __builtin_fmaf(y, s.z, x.z),
+                    __builtin_fmaf(y, s.w, x.w));
+    w[(long long)k * quads] = s;
+  }
+}
+
+// How a call is cut: dk and dv in tiles, and rows in pieces
+struct Plan {
+  bool chunk;
+  int dkt, nc, c, nsl, npc, pcr;
+  long long states, floats;  // of a state
+};
+Plan plan(const bnh_la *p, int T, int B) {
+  Plan r;
+  r.chunk = T > 8;
+  r.dkt = p->dk <= 32 ? 1 : p->dk <= 64 ? 2 : p->dk <= 128 ? 4 : 8;
+  r.nc = p->f16 && r.dkt <= 4 && p->dv > 64 ? 2 : 1;
+  r.c = p->f16 ? 64 : 32;
+  r.nsl = (int)bnh_ceil_div(p->dv, 64 * r.nc);
+  r.states = (long long)B * p->H * r.nsl;
+  r.floats = 32LL * r.dkt * 64 * r.nc;
+  r.npc = 1;
+  r.pcr = T;
+  if (r.chunk) {
+    long long want = bnh_ceil_div(512, r.states);
+    const long long most = bnh_ceil_div(T, 4 * r.c);
+    if (want > most) want = most;
+    r.pcr = (int)bnh_round_up(bnh_ceil_div(T, want), r.c);
+    r.npc = (int)bnh_ceil_div(T, r.pcr);
+  }
+  return r;
+}
+size_t plan_bytes(const Plan &r) {
+  if (r.npc < 2) return 0;
+  return (size_t)(bnh_round_up(4 * r.states * (r.npc - 1) * r.floats, 256) + bnh_round_up(4 * r.states * (r.npc - 1), 256));
+}
+
+template <typename T, int DKT, int NC, int C, bool V>
+int chunk_run(const LaDev &d, const Plan &r, int B, void *work, hipStream_t s) {
+  float *part = (float *)work, *pdec = part ? (float *)((char *)work + bnh_round_up(4 * r.states * (r.npc - 1) * r.floats, 256)) : nullptr;
+  if (r.npc > 1) {
+    hipLaunchKernelGGL((k_la_chunk<T, DKT, NC, C, V, false>), dim3((unsigned)(r.states * (r.npc - 1))), dim3(256), 0, s, d,
+                       r.nsl, r.npc, r.pcr, part, pdec);
+    BNH_HIP(hipGetLastError());
+    const int quads = (int)(r.floats / 4);
+    if (r.npc > 2) {
+      hipLaunchKernelGGL(k_la_scan, dim3((unsigned)bnh_ceil_div(quads, 256), (unsigned)r.states), dim3(256), 0, s, d, r.npc,
+                         r.pcr, quads, r.nsl, part, pdec);
+      BNH_HIP(hipGetLastError());
+    }
+  }
+  hipLaunchKernelGGL((k_la_chunk<T, DKT, NC, C, V, true>), dim3((unsigned)(r.states * r.npc)), dim3(256), 0, s, d, r.nsl,
+                     r.npc, r.pcr, part, pdec);
+  BNH_HIP(hipGetLastError());
+  return 0;
+}
+template <typename T, int C, bool V>
+int chunk_go(const LaDev &d, const Plan &r, int B, void *work, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (r.nc == 2) {
+      if (r.dkt == 1) return chunk_run<T, 1, 2, C, V>(d, r, B, work, s);
+      if (r.dkt == 2) return chunk_run<T, 2, 2, C, V>(d, r, B, work, s);
+      return chunk_run<T, 4, 2, C, V>(d, r, B, work, s);
+    }
+  }
+  if (r.dkt == 1) return chunk_run<T, 1, 1, C, V>(d, r, B, work, s);
+  if (r.dkt == 2) return chunk_run<T, 2, 1, C, V>(d, r, B, work, s);
+  if (r.dkt == 4) return chunk_run<T, 4, 1, C, V>(d, r, B, work, s);
+  return chunk_run<T, 8, 1, C, V>(d, r, B, work, s);
+}
+
 int la_check(const bnh_la *p, int T, int B) {
   BNH_REQ(p && T > 0 && B > 0 && p->H > 0 && p->Hq > 0 && p->Hk > 0 && p->Hv > 0);
   BNH_REQ(p->H % p->Hq == 0 && p->H % p->Hk == 0 && p->H % p->Hv == 0);
@@ -149,7 +682,7 @@ extern "C" {
 
 size_t bnh_linattn_work_bytes(const bnh_la *p, int T, int B) {
   if (la_check(p, T, B)) return 0;
-  return 0;
+  return plan_bytes(plan(p, T, B));
 }
 
 int bnh_linattn(const bnh_la *p, int T, int B, int rows, const int32_t *start, const int32_t *len, void *work,
@@ -168,6 +701,17 @@ int bnh_linattn(const bnh_la *p, int T, int B, int rows, const int32_t *start, c
              p->H, p->H / p->Hq, p->H / p->Hk, p->H / p->Hv, p->dk, p->dv, p->slots, T, rows, p->scale};
   const bool vs = p->dv % 4 == 0 && on(p->s0, 16) && on(p->s1, 16);
   hipStream_t s = bnh_stream(stream);
+  const Plan r = plan(p, T, B);
+  if (r.chunk) {
+    const size_t need = plan_bytes(r);
+    BNH_REQ(need == 0 || (work && on(work, 16) && work_bytes >= need));
+    BNH_REQ(r.states * r.npc < (1LL << 31) && (r.npc < 3 || r.states < 65536));
+    const int ve = 16 / (int)es;
+    const bool v = on(p->q, 16) && on(p->k, 16) && on(p->v, 16) && on(p->o, 16) && p->ldq % ve == 0 && p->ldk % ve == 0 &&
+                   p->ldv % ve == 0 && p->ldo % ve == 0 && p->dk % ve == 0 && p->dv % ve == 0;
+    if (p->f16) return v ? chunk_go<h16, 64, true>(d, r, B, work, s) : chunk_go<h16, 64, false>(d, r, B, work, s);
+    return v ? chunk_go<float, 32, true>(d, r, B, work, s) : chunk_go<float, 32, false>(d, r, B, work, s);
+  }
   if (p->f16) return vs ? step_run<h16, 32, true>(d, B, s) : step_run<h16, 32, false>(d, B, s);
   return vs ? step_run<float, 32, true>(d, B, s) : step_run<float, 32, false>(d, B, s);
 }
