@@ -7,6 +7,8 @@
 // over the output. Rows of one matrix instruction are independent of each other, so a block of 16 rows whose adapters
 // differ multiplies all of them by each of the adapters in it and every row keeps its own: nothing of another request's
 // adapter, not even an infinity or a NaN, reaches it.
+#include <type_traits>
+
 #include "bnh_internal.h"
 #include "bnh_f16.h"
 #include "bnh_lds_dma.h"
@@ -33,6 +35,15 @@ __device__ __forceinline__ v8h ld8(const uint16_t *p, int n) {
 }
 __device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// f(0) ... f(N - 1), each with its index as a constant: accumulators indexed by it stay in registers
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
 struct LoraDev {
   const uint16_t *x, *w, *a, *b;
   const float *bias, *scale;
@@ -49,16 +60,15 @@ __device__ __forceinline__ int lora_id(const LoraDev &p, int win) {  // -1: none
   return j >= 0 && j < p.n ? j : -1;
 }
 
-// t of 16 rows for the blockIdx.y-th different adapter among them; the block's four waves take every fourth step of 32
-// of K. RT: 16-column tiles of r32.
+// t of the 16 rows from 16 tile for the which-th different adapter among them; the block's four waves take every fourth
+// step of 32 of K. RT: 16-column tiles of r32; s: 768 RT floats of LDS
 template <int RT, bool V>
-__global__ __launch_bounds__(256) void k_lora_down(LoraDev p) {
-  __shared__ float s_t[3][RT][256];
+__device__ __forceinline__ void lora_down(const LoraDev &p, long long tile, unsigned which, float *s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, kc = (lane >> 4) * 8;
-  const long long row = (long long)blockIdx.x * 16 + lr < p.rows ? (long long)blockIdx.x * 16 + lr : p.rows - 1;
+  const long long row = tile * 16 + lr < p.rows ? tile * 16 + lr : p.rows - 1;
   const int win = bnh_div(row, p.M, p.rM);
   const int id = lora_id(p, win);
-  // the first rows of the different adapters, and of those the one that is this block's
+  // the first rows of the different adapters, and of those the one that is asked for
   bool dup = false;
 #pragma unroll
   for (int j = 0; j < 15; j++) {
@@ -66,41 +76,55 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraDev p) {
     dup = dup || (j < lr && o == id);
   }
   uint32_t lead = (uint32_t)(__builtin_amdgcn_ballot_w64(lane < 16 && !dup && id >= 0));
-  for (unsigned i = 0; i < blockIdx.y; i++) lead &= lead - 1;
+  for (unsigned i = 0; i < which; i++) lead &= lead - 1;
   if (!lead) return;
   const int j = __builtin_amdgcn_readlane(id, __builtin_ctz(lead));
   const uint16_t *xp = p.x + win * p.x_ws + (long long)(row - (long long)win * p.M) * p.lda + kc;
-  const uint16_t *ap = p.a + (long long)j * p.r * p.K + kc;
+  const uint16_t *ap[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++)  // past the last rank: any row, whose results are not kept
+    ap[t] = p.a + ((long long)j * p.r + (16 * t + lr < p.r ? 16 * t + lr : p.r - 1)) * p.K + kc;
   v4f acc[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) acc[t] = (v4f){0.f, 0.f, 0.f, 0.f};
-  for (int k = 32 * wave; k < p.K; k += 128) {
+  int k = 32 * wave;
+#pragma unroll 4
+  for (; k + 32 <= p.K; k += 128) {
+    const v8h x = ld8<V>(xp + k, 8);
+#pragma unroll
+    for (int t = 0; t < RT; t++) acc[t] = mma(x, ld8<V>(ap[t] + k, 8), acc[t]);
+  }
+  if (k < p.K) {
     const v8h x = ld8<V>(xp + k, p.K - k - kc);
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-      const int c = 16 * t + lr;
-      const v8h a = c < p.r ? ld8<V>(ap + (long long)c * p.K + k, p.K - k - kc) : (v8h){};
-      acc[t] = mma(x, a, acc[t]);
-    }
+    for (int t = 0; t < RT; t++) acc[t] = mma(x, ld8<V>(ap[t] + k, p.K - k - kc), acc[t]);
   }
   if (wave) {
 #pragma unroll
-    for (int t = 0; t < RT; t++) *(v4f *)&s_t[wave - 1][t][4 * lane] = acc[t];
+    for (int t = 0; t < RT; t++) *(v4f *)(s + ((wave - 1) * RT + t) * 256 + 4 * lane) = acc[t];
   }
   __syncthreads();
   if (wave) return;
   const float sc = p.scale ? p.scale[j] : 1.f;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    acc[t] += *(v4f *)&s_t[0][t][4 * lane] + (*(v4f *)&s_t[1][t][4 * lane] + *(v4f *)&s_t[2][t][4 * lane]);
+    const float *q = s + t * 256 + 4 * lane;
+    acc[t] += *(const v4f *)q + (*(const v4f *)(q + RT * 256) + *(const v4f *)(q + 2 * RT * 256));
+    const int c = 16 * t + lr;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int m = 4 * (lane >> 4) + e;
-      const long long r = (long long)blockIdx.x * 16 + m;
       const int rid = __shfl(id, m);
-      if (r < p.rows && rid == j && 16 * t + lr < p.r32) p.t[r * p.r32 + 16 * t + lr] = 16 * t + lr < p.r ? hbits((h16)(sc * acc[t][e])) : 0;
+      if (tile * 16 + m < p.rows && rid == j && c < p.r32)
+        p.t[(tile * 16 + m) * p.r32 + c] = c < p.r ? hbits((h16)(sc * acc[t][e])) : 0;
+      if (RT == 1 && tile * 16 + m < p.rows && rid == j) p.t[(tile * 16 + m) * p.r32 + 16 + lr] = 0;
     }
   }
+}
+template <int RT, bool V>
+__global__ __launch_bounds__(256) void k_lora_down(LoraDev p) {
+  __shared__ __attribute__((aligned(16))) float s[768 * RT];
+  lora_down<RT, V>(p, blockIdx.x, blockIdx.y, s);
 }
 
 __device__ __forceinline__ float lora_act(float y, int act) {
@@ -114,6 +138,108 @@ struct EpiDev {
   const uint16_t *res;
   long long out_ws, res_ws;
 };
+
+// Up to 64 rows: bound by reading w. The first nd blocks compute t (as k_lora_down), the others the shared product of all
+// rows with 32 channels over one of `ks` slices of K, into part [ks][rows][Np]; k_lora_few_out adds the slices and the
+// adapters' products. RW: 16-row tiles.
+template <int RT, int RW, bool V>
+__global__ __launch_bounds__(256) void k_lora_few(LoraDev p, int nd, int dy, int nn, int ks, int Np, float *part) {
+  constexpr int LF = RT > 2 * RW ? 768 * RT : 768 * 2 * RW;
+  __shared__ __attribute__((aligned(16))) float s[LF];
+  if ((int)blockIdx.x < nd) {
+    lora_down<RT, V>(p, blockIdx.x / dy, blockIdx.x % dy, s);
+    return;
+  }
+  const int blk = (int)blockIdx.x - nd, sl = blk / nn, n0 = blk % nn * 32;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, kc = (lane >> 4) * 8;
+  const uint16_t *xp[RW], *wp[2];
+#pragma unroll
+  for (int i = 0; i < RW; i++) {
+    const int row = 16 * i + lr < p.rows ? 16 * i + lr : (int)p.rows - 1;
+    const int w = row / p.M;
+    xp[i] = p.x + w * p.x_ws + (long long)(row - w * p.M) * p.lda + kc;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; j++) wp[j] = p.w + (long long)(n0 + 16 * j + lr < p.N ? n0 + 16 * j + lr : p.N - 1) * p.ldw + kc;
+  v4f acc[2][RW];
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+#pragma unroll
+    for (int i = 0; i < RW; i++) acc[j][i] = (v4f){0.f, 0.f, 0.f, 0.f};
+  int k = 32 * (4 * sl + wave);
+#pragma unroll 4
+  for (; k + 32 <= p.K; k += 128 * ks) {
+    const v8h w0 = ld8<V>(wp[0] + k, 8), w1 = ld8<V>(wp[1] + k, 8);
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+      const v8h x = ld8<V>(xp[i] + k, 8);
+      acc[0][i] = mma(w0, x, acc[0][i]);
+      acc[1][i] = mma(w1, x, acc[1][i]);
+    }
+  }
+  if (k < p.K) {
+    const v8h w0 = ld8<V>(wp[0] + k, p.K - k - kc), w1 = ld8<V>(wp[1] + k, p.K - k - kc);
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+      const v8h x = ld8<V>(xp[i] + k, p.K - k - kc);
+      acc[0][i] = mma(w0, x, acc[0][i]);
+      acc[1][i] = mma(w1, x, acc[1][i]);
+    }
+  }
+  if (wave) {
+#pragma unroll
+    for (int i = 0; i < 2 * RW; i++) *(v4f *)(s + ((wave - 1) * 2 * RW + i) * 256 + 4 * lane) = acc[i / RW][i % RW];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int i = 0; i < 2 * RW; i++) {
+    const float *q = s + i * 256 + 4 * lane;
+    const v4f y = acc[i / RW][i % RW] + (*(const v4f *)q + (*(const v4f *)(q + 512 * RW) + *(const v4f *)(q + 1024 * RW)));
+    const int row = 16 * (i % RW) + lr, n = n0 + 16 * (i / RW) + (lane >> 4) * 4;
+    if (row < p.rows && n < p.N) *(v4f *)(part + ((long long)sl * p.rows + row) * Np + n) = y;  // Np: N rounded up to 4
+  }
+}
+// four channels of one row a thread
+template <bool VR, bool VO>
+__global__ __launch_bounds__(256) void k_lora_few_out(LoraDev p, EpiDev e, int ks, int Np, const float *part) {
+  const int i = (int)(blockIdx.x * 256 + threadIdx.x), nq = Np / 4;
+  const int row = i / nq, n = i % nq * 4;
+  if (row >= p.rows) return;
+  const int w = row / p.M, m = row - w * p.M;
+  const int id = p.idx ? lora_id(p, w) : -1;
+  v4f y = (v4f){0.f, 0.f, 0.f, 0.f}, u = y;
+#pragma unroll 4
+  for (int k = 0; k < ks; k++) y += *(const v4f *)(part + ((long long)k * p.rows + row) * Np + n);
+  if (id >= 0) {
+    const uint16_t *t = p.t + (long long)row * p.r32, *b = p.b + ((long long)id * p.N + n) * p.r;
+    for (int k = 0; k < p.r; k += 8) {
+      const v8h x = *(const v8h *)(t + k);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        if (n + c >= p.N) continue;
+        const v8h z = ld8<VR>(b + (long long)c * p.r + k, p.r - k);
+#pragma unroll
+        for (int l = 0; l < 8; l++) u[c] = __builtin_fmaf((float)x[l], (float)z[l], u[c]);
+      }
+    }
+    y += u;
+  }
+  uint16_t *o = e.out + w * e.out_ws + (long long)m * e.ldo + n;
+  const uint16_t *rs = e.res ? e.res + w * e.res_ws + (long long)m * e.ldr + n : nullptr;
+  typedef h16 v4h __attribute__((ext_vector_type(4)));
+  v4h z = {}, q;
+  if (VO && rs) z = *(const v4h *)rs;
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    if (!VO && n + c >= p.N) continue;
+    if (!VO && rs) z[c] = hfrom(rs[c]);
+    const float v = lora_act(y[c] + (p.bias ? p.bias[n + c] : 0.f), e.act);
+    q[c] = (h16)(rs ? v + (float)z[c] : v);
+    if (!VO) o[c] = hbits(q[c]);
+  }
+  if (VO) *(v4h *)o = q;
+}
 
 // The tile of rows [r0, ...) x channels [n0, ...) of logical block lb: blocks that follow each other (and so run under one
 // XCD's L2) form groups of 8 row tiles that share their channels' weights
@@ -130,10 +256,10 @@ __device__ __forceinline__ void lora_tile(unsigned lb, int nm, int nn, int *tm, 
 // fragment's read fall on different banks (the loads write 16 bytes a lane in lane order, so the lane's chunk of the
 // row is permuted instead). The first operand of the matrix instruction is the weights': a lane's accumulators are
 // four channels of one row.
-template <int BM, int BN, int WM, int WN, int BK, bool DMA, bool VR, bool VO>
+template <int BM, int BN, int WM, int WN, int BK, int RING, bool DMA, bool VR, bool VO>
 __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e, int nm, int nn) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, CH = BK / 8, RPI = 64 / CH;
-  constexpr int NL = (BM + BN) * CH / 64 / NW, ST = DMA ? 4 : 2, SH = (BM + BN) * BK;  // loads a wave; stages, their halves
+  constexpr int NL = (BM + BN) * CH / 64 / NW, ST = DMA ? RING : 2, SH = (BM + BN) * BK;  // loads a wave; stages, their halves
   constexpr int XS = 16 * TN + 4;                                                   // an exchange row, floats
   static_assert((BM + BN) * CH % (64 * NW) == 0 && BM % RPI == 0, "");
   constexpr int LDS = ST * SH * 2 > NW * 16 * XS * 4 ? ST * SH * 2 : NW * 16 * XS * 4;
@@ -189,25 +315,25 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
   };
   const int full = p.K / BK;
   if constexpr (DMA) {
-    auto issue = [&](int t) {
+    auto issue = [&](int t, int stage) {
 #pragma unroll
       for (int i = 0; i < NL; i++)
-        rq_dma16((const int8_t *)(gp[i] + (long long)t * BK), (const lds_i8 *)(s + (t & 3) * SH + (i * NW + wave) * 512));
+        rq_dma16((const int8_t *)(gp[i] + (long long)t * BK), (const lds_i8 *)(s + stage * SH + (i * NW + wave) * 512));
     };
-    for (int t = 0; t < 3 && t < full; t++) issue(t);
+    static_assert((ST == 2 || ST == 3) && (ST - 2) * NL <= 8, "the waits below");
+    for (int t = 0; t < ST - 1 && t < full; t++) issue(t, t);
+    int at = 0;
     for (int t = 0; t < full; t++) {
-      if (t + 2 < full) {
-        if constexpr (NL == 2) RQ_WAIT_VM(4);
-        else if constexpr (NL == 4) RQ_WAIT_VM(8);
-        else RQ_WAIT_VM(0);
-      } else {
-        RQ_WAIT_VM(0);
-      }
-      // every read of step t - 1's stage is done, which step t + 3 takes
+      if (ST == 2 || t + 1 >= full) RQ_WAIT_VM(0);
+      else if (NL == 4) RQ_WAIT_VM(4);
+      else RQ_WAIT_VM(8);
+      // step t's stage is full, and every read of step t - 1's, which the next loads take, is done
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       RQ_BARRIER();
-      if (t + 3 < full) issue(t + 3);
-      step(s + (t & 3) * SH);
+      const int next = at + ST - 1 < ST ? at + ST - 1 : at - 1;
+      if (t + ST - 1 < full) issue(t + ST - 1, next);
+      step(s + at * SH);
+      at = at + 1 < ST ? at + 1 : 0;
     }
   } else {
     v8h v[NL];
@@ -234,36 +360,64 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
   }
   __syncthreads();
 
-  float *xch = (float *)s_raw + wave * 16 * XS;
+  // The adapters: one of those among the wave's rows a turn, its b read once for all of them. A tile of 16 rows that all
+  // have it adds to its sums directly; of others every row takes the product or keeps what it has, so that one
+  // request's infinities stay its own.
+  if (p.idx) {
+    int id[TM];
+    const uint16_t *tp[TM];
+    each<TM>([&](auto tile) {
+      constexpr int i = decltype(tile)::value;
+      const long long row = r0 + wm + 16 * i + lr < p.rows ? r0 + wm + 16 * i + lr : p.rows - 1;
+      id[i] = lora_id(p, bnh_div(row, p.M, p.rM));
+      tp[i] = p.t + row * p.r32 + 8 * q4;
+    });
+    const uint16_t *bp[TN];
 #pragma unroll
-  for (int i = 0; i < TM; i++) {
-    const long long rb = r0 + wm + 16 * i;
-    if (rb >= p.rows) break;
-    const long long row = rb + lr < p.rows ? rb + lr : p.rows - 1;
-    if (p.idx) {
-      const int id = lora_id(p, bnh_div(row, p.M, p.rM));
-      const uint16_t *tp = p.t + row * p.r32 + 8 * q4;
-      uint32_t left = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && id >= 0);
-      while (left) {  // one adapter of the 16 rows a turn
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-        left &= ~(uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && id == a);
-        v4f u[TN];
+    for (int j = 0; j < TN; j++)
+      bp[j] = p.b + (long long)(n0 + wn + 16 * j + lr < p.N ? n0 + wn + 16 * j + lr : p.N - 1) * p.r + 8 * q4;
+    uint32_t todo[TM];
+    each<TM>([&](auto tile) {
+      constexpr int i = decltype(tile)::value;
+      todo[i] = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && id[i] >= 0);
+    });
+    for (;;) {
+      int a = -1;
+      each<TM>([&](auto tile) {
+        constexpr int i = decltype(tile)::value;
+        if (a < 0 && todo[i]) a = __builtin_amdgcn_readlane(id[i], __builtin_ctz(todo[i]));
+      });
+      if (a < 0) break;
+      for (int k = 0; k < p.r32; k += 32) {
+        v8h b[TN];
 #pragma unroll
-        for (int j = 0; j < TN; j++) u[j] = (v4f){0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < p.r32; k += 32) {
-          const v8h x = *(const v8h *)(tp + k);
+        for (int j = 0; j < TN; j++) b[j] = ld8<VR>(bp[j] + (long long)a * p.N * p.r + k, p.r - k - 8 * q4);
+        each<TM>([&](auto tile) {
+          constexpr int i = decltype(tile)::value;
+          const uint32_t mine = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && id[i] == a);
+          if (mine == 0xffff) {
+            const v8h x = *(const v8h *)(tp[i] + k);
 #pragma unroll
-          for (int j = 0; j < TN; j++) {
-            const int n = n0 + wn + 16 * j + lr < p.N ? n0 + wn + 16 * j + lr : p.N - 1;
-            u[j] = mma(ld8<VR>(p.b + ((long long)a * p.N + n) * p.r + k + 8 * q4, p.r - k - 8 * q4), x, u[j]);
+            for (int j = 0; j < TN; j++) acc[j][i] = mma(b[j], x, acc[j][i]);
+          } else if (mine) {
+            const v8h x = *(const v8h *)(tp[i] + k);
+#pragma unroll
+            for (int j = 0; j < TN; j++) {
+              const v4f u = mma(b[j], x, (v4f){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+              for (int q = 0; q < 4; q++) acc[j][i][q] = id[i] == a ? acc[j][i][q] + u[q] : acc[j][i][q];
+            }
           }
-        }
-        if (id == a) {
-#pragma unroll
-          for (int j = 0; j < TN; j++) acc[j][i] += u[j];
-        }
+          if (k + 32 >= p.r32) todo[i] &= ~mine;
+        });
       }
     }
+  }
+  float *xch = (float *)s_raw + wave * 16 * XS;
+  each<TM>([&](auto tile) {
+    constexpr int i = decltype(tile)::value;
+    const long long rb = r0 + wm + 16 * i;
+    if (rb >= p.rows) return;
 #pragma unroll
     for (int j = 0; j < TN; j++) {
       const int n = n0 + wn + 16 * j + 4 * q4;
@@ -302,16 +456,16 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
+  });
 }
 
-template <int BM, int BN, int WM, int WN, int BK>
+template <int BM, int BN, int WM, int WN, int BK, int RING>
 int lora_tiles(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipStream_t s) {
   const long long nm = bnh_ceil_div(p.rows, BM), nn = bnh_ceil_div(p.N, BN);
   if (nm * nn >= (1LL << 31)) return bnh_fail("bnh_pw_lora: %lld x %d outputs are too many tiles", p.rows, p.N);
   const dim3 grid((unsigned)(nm * nn)), block(64 * WM * WN);
 #define GO(V, VR, VO) \
-  hipLaunchKernelGGL((k_lora_gemm<BM, BN, WM, WN, BK, V, VR, VO>), grid, block, 0, s, p, d, (int)nm, (int)nn)
+  hipLaunchKernelGGL((k_lora_gemm<BM, BN, WM, WN, BK, RING, V, VR, VO>), grid, block, 0, s, p, d, (int)nm, (int)nn)
   if (v && vr && vo) GO(true, true, true);
   else if (v && vo) GO(true, false, true);
   else if (v) GO(true, false, false);
@@ -321,11 +475,49 @@ int lora_tiles(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipS
   BNH_HIP(hipGetLastError());
   return 0;
 }
+constexpr long long few = 64;  // rows up to which w's bytes bound the product
+// slices of K of the few-row form: two blocks a compute unit, and a step of 32 a wave at least
+long long few_slices(int N, int K) {
+  const long long want = bnh_ceil_div(512, bnh_ceil_div(N, 32)), most = bnh_ceil_div(K, 128);
+  return want < most ? want : most;
+}
+long long lora_t_bytes(long long rows, int r) { return bnh_round_up(rows * bnh_round_up(r, 32) * 2, 256); }
+
+int lora_few(const LoraDev &p, const EpiDev &d, int dy, bool v, bool vr, bool vo, void *work, hipStream_t s) {
+  const int Np = (int)bnh_round_up(p.N, 4), nn = (int)bnh_ceil_div(p.N, 32), ks = (int)few_slices(p.N, p.K);
+  const int nd = dy * (int)bnh_ceil_div(p.rows, 16);
+  float *part = (float *)((char *)work + lora_t_bytes(p.rows, p.r));
+  const dim3 grid((unsigned)(nd + nn * ks)), block(256);
+#define GO2(RT, RW)                                                                                            \
+  do {                                                                                                         \
+    if (v) hipLaunchKernelGGL((k_lora_few<RT, RW, true>), grid, block, 0, s, p, nd, dy, nn, ks, Np, part);     \
+    else hipLaunchKernelGGL((k_lora_few<RT, RW, false>), grid, block, 0, s, p, nd, dy, nn, ks, Np, part);      \
+  } while (0)
+#define GO(RW)                       \
+  do {                               \
+    if (p.r <= 16) GO2(1, RW);       \
+    else if (p.r <= 64) GO2(4, RW);  \
+    else GO2(16, RW);                \
+  } while (0)
+  if (p.rows <= 16) GO(1);
+  else if (p.rows <= 32) GO(2);
+  else GO(4);
+#undef GO
+#undef GO2
+  BNH_HIP(hipGetLastError());
+  const dim3 og((unsigned)bnh_ceil_div(p.rows * (Np / 4), 256));
+  if (vr && vo) hipLaunchKernelGGL((k_lora_few_out<true, true>), og, block, 0, s, p, d, ks, Np, part);
+  else if (vr) hipLaunchKernelGGL((k_lora_few_out<true, false>), og, block, 0, s, p, d, ks, Np, part);
+  else if (vo) hipLaunchKernelGGL((k_lora_few_out<false, true>), og, block, 0, s, p, d, ks, Np, part);
+  else hipLaunchKernelGGL((k_lora_few_out<false, false>), og, block, 0, s, p, d, ks, Np, part);
+  BNH_HIP(hipGetLastError());
+  return 0;
+}
 // The largest tile that still gives every compute unit one: a large tile reads its operands from L2 less often
 int lora_gemm(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipStream_t s) {
-  if (bnh_ceil_div(p.rows, 256) * bnh_ceil_div(p.N, 256) >= 256) return lora_tiles<256, 256, 2, 4, 32>(p, d, v, vr, vo, s);
-  if (bnh_ceil_div(p.rows, 128) * bnh_ceil_div(p.N, 128) >= 256) return lora_tiles<128, 128, 2, 2, 32>(p, d, v, vr, vo, s);
-  return lora_tiles<64, 64, 2, 2, 64>(p, d, v, vr, vo, s);
+  if (bnh_ceil_div(p.rows, 256) * bnh_ceil_div(p.N, 256) >= 256) return lora_tiles<256, 256, 2, 4, 64, 2>(p, d, v, vr, vo, s);
+  if (bnh_ceil_div(p.rows, 128) * bnh_ceil_div(p.N, 128) >= 256) return lora_tiles<128, 128, 2, 2, 64, 2>(p, d, v, vr, vo, s);
+  return lora_tiles<64, 64, 2, 2, 64, 3>(p, d, v, vr, vo, s);
 }
 
 }  // namespace
@@ -333,11 +525,12 @@ int lora_gemm(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipSt
 extern "C" {
 
 size_t bnh_pw_lora_work_bytes(int M, int B, int N, int K, int r) {
-  if (M <= 0 || B <= 0 || N <= 0 || K <= 0 || r < 0 || r > 256) {
+  if (M <= 0 || B <= 0 || N <= 0 || K <= 0 || r < 0 || r > 256 || (long long)M * B >= (1LL << 31) || N >= (1 << 24)) {
     bnh_fail("bnh_pw_lora_work_bytes: parameter check failed");
     return 0;
   }
-  return (size_t)bnh_round_up((long long)M * B * bnh_round_up(r, 32) * 2, 256);
+  const long long rows = (long long)M * B;
+  return (size_t)(lora_t_bytes(rows, r) + (rows <= few ? 4 * few_slices(N, K) * rows * bnh_round_up(N, 4) : 0));
 }
 
 int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const uint16_t *w, int ldw, int N, int K,
@@ -350,10 +543,9 @@ int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const 
   auto on = [](const void *q, size_t a) { return (uintptr_t)q % a == 0; };
   BNH_REQ(on(x, 2) && on(w, 2) && on(bias, 4) && on(idx, 4) && on(e->out, 2) && on(e->res, 2));
   const bool ad = L && L->n > 0;
-  if (ad) {
-    BNH_REQ(on(L->a, 2) && on(L->b, 2) && on(L->scale, 4) && work && on(work, 16));
-    BNH_REQ(work_bytes >= bnh_pw_lora_work_bytes(M, B, N, K, L->r));
-  }
+  if (ad) BNH_REQ(on(L->a, 2) && on(L->b, 2) && on(L->scale, 4));
+  const size_t need = bnh_pw_lora_work_bytes(M, B, N, K, ad ? L->r : 0);
+  BNH_REQ(need == 0 || (work && on(work, 16) && work_bytes >= need));
   LoraDev p = {x, w, ad ? L->a : nullptr, ad ? L->b : nullptr, bias, ad ? L->scale : nullptr, ad ? idx : nullptr,
                (uint16_t *)work, x_ws, lda, ldw, M, N, K, ad ? L->n : 0, ad ? L->r : 0,
                ad ? (int)bnh_round_up(L->r, 32) : 0, (long long)M * B, 1.0 / M};
@@ -361,21 +553,24 @@ int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const 
   hipStream_t s = bnh_stream(stream);
   const bool vx = K % 8 == 0 && lda % 8 == 0 && on(x, 16) && (B == 1 || x_ws % 8 == 0);
   const bool v = vx && ldw % 8 == 0 && on(w, 16), va = ad && vx && on(L->a, 16), vr = ad && L->r % 8 == 0 && on(L->b, 16);
+  // different adapters among 16 rows in a line: at most the windows that they touch
+  const int dy = M >= 15 ? 2 : (14 + M) / M + 1 < 16 ? (14 + M) / M + 1 : 16;
+  const bool vo = N % 8 == 0 && e->ldo % 8 == 0 && on(e->out, 16) && (B == 1 || e->out_ws % 8 == 0) &&
+                  (!e->res || (e->ldr % 8 == 0 && on(e->res, 16) && (B == 1 || e->res_ws % 8 == 0)));
+  if (p.rows <= few) return lora_few(p, d, ad ? dy : 0, v && (!ad || va), vr || !ad, vo, work, s);
   if (ad) {
-    // different adapters among 16 rows in a line: at most the windows that they touch
-    const dim3 grid((unsigned)bnh_ceil_div(p.rows, 16), (unsigned)(M >= 15 ? 2 : (14 + M) / M + 1 < 16 ? (14 + M) / M + 1 : 16));
-#define GO(RT)                                                                         \
-  if (va) hipLaunchKernelGGL((k_lora_down<RT, true>), grid, dim3(256), 0, s, p);       \
+    const dim3 grid((unsigned)bnh_ceil_div(p.rows, 16), (unsigned)dy);
+#define GO(RT)                                                                   \
+  if (va) hipLaunchKernelGGL((k_lora_down<RT, true>), grid, dim3(256), 0, s, p); \
   else hipLaunchKernelGGL((k_lora_down<RT, false>), grid, dim3(256), 0, s, p)
-    if (p.r32 <= 32) GO(2);
-    else if (p.r32 <= 64) GO(4);
-    else if (p.r32 <= 128) GO(8);
+    if (p.r <= 16) GO(1);
+    else if (p.r <= 32) GO(2);
+    else if (p.r <= 64) GO(4);
+    else if (p.r <= 128) GO(8);
     else GO(16);
 #undef GO
     BNH_HIP(hipGetLastError());
   }
-  const bool vo = N % 8 == 0 && e->ldo % 8 == 0 && on(e->out, 16) && (B == 1 || e->out_ws % 8 == 0) &&
-                  (!e->res || (e->ldr % 8 == 0 && on(e->res, 16) && (B == 1 || e->res_ws % 8 == 0)));
   return lora_gemm(p, d, v, vr, vo, s);
 }
 
