@@ -142,15 +142,15 @@ int step_run(const LaDev &d, int B, hipStream_t s) {
 // divided by a small decay; c is kept in 64 bits because differences of its values matter where c itself has grown
 // large, and g below -1e4 (whose e^g is 0) counts as -1e4, so that a reset's infinity does not cancel another's.
 //
-// A block of four waves owns 64 NC columns of one state over one piece of one sequence. The state stays in the accumulators of
-// the waves (16 NC columns each, all of dk): their layout is, for pairs of 16-row tiles, that of the first operand of the
+// A block of four or eight waves owns 64 or 128 columns of one state over one piece of one sequence. The state stays in the
+// accumulators of the waves (16 columns each, all of dk): their layout is, for pairs of 16-row tiles, that of the first operand of the
 // product with q's rows, so it never passes through LDS. q, k and v of the next chunk are loaded into registers while this
 // one's are multiplied out of LDS; k's and v's transposes come out of LDS through ds_read_b64_tr_b16.
 //
 // fp16 rows: the factors of a product have to be fp16, its sums are fp32. Scores are scaled row by row and the state
 // column by column by powers of two before they are rounded (their largest to 2^12..2^13), so neither overflows and both
 // keep 11 bits, as the rounded output does. The state itself is not rounded: its update takes v_j e^{c_C - c_j}, scaled
-// the same way, in two fp16 parts of 11 bits each (the second, times 2^11, in a product of its own) against the exact k. fp32 rows run
+// by column to 2^14..2^15 (the state's own unit from then on), in two fp16 parts, 22 bits, against the exact k. fp32 rows run
 // on the fp32 MFMA, unscaled and unsplit.
 //
 // A row's v that is not finite would reach earlier rows of its chunk as 0 x inf; it is taken out of the product and added to
@@ -232,20 +232,22 @@ __device__ __forceinline__ uint4 row16(const T *p, int c, int cols) {
   return r;
 }
 
-// One piece of one sequence. OUT: the outputs, from the state before the piece, and s1 from the sequence's last; else the
-// state that every piece but the last adds (the first one's includes s0), into part, and its whole decay.
-template <typename T, int DKT, int NC, int C, bool V, bool OUT>
-__global__ __launch_bounds__(256) void k_la_chunk(LaDev p, int nsl, int npc, int pcr, float *part, float *pdec) {
+// One piece of one sequence by NW waves, 16 of the state's columns each. OUT: the outputs, from the state before the piece,
+// and s1 from the sequence's last; else the state that every piece but the last adds (the first one's includes s0), into
+// part, and its whole decay.
+template <typename T, int DKT, int NW, int C, bool V, bool OUT>
+__global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc, int pcr, float *part, float *pdec) {
   constexpr bool F16 = sizeof(T) == 2;
-  constexpr int VE = 16 / sizeof(T), KD = 32 * DKT, DV = 64 * NC, SK = KD + VE, SV = DV + VE, SP = C + VE;
-  constexpr int NK = C * KD / VE / 256, NV = C * DV / VE / 256, RK = 256 * VE / KD, RV = 256 * VE / DV;
+  constexpr int VE = 16 / sizeof(T), KD = 32 * DKT, DV = 16 * NW, NT = 64 * NW, SK = KD + VE, SV = DV + VE, SP = C + VE;
+  constexpr int RK = NT * VE / KD, RV = NT * VE / DV;                          // rows that one load of all threads covers
+  constexpr int NK = C / RK > 0 ? C / RK : 1, NV = C / RV > 0 ? C / RV : 1;
   typedef typename Frag<T>::V FV;
   typedef typename Frag<T>::H FH;
   __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SK : 1], s_k[C * SK], s_v[C * SV], s_p[OUT ? C * SP : 1];
-  __shared__ double s_c[2][64];                    // c_i
+  __shared__ double s_c[2][64];                              // c_i
   __shared__ __attribute__((aligned(16))) float s_w[2][64];  // e^{c_C - c_j}
-  __shared__ float s_e[2][64], s_d[2];             // e^{c_i}; e^{c_C}
-  __shared__ int s_x[64];                          // the scores' scale by row
+  __shared__ float s_e[2][64], s_d[2], s_m[2];               // e^{c_i}; e^{c_C}; the largest of s_w
+  __shared__ int s_x[64];                                    // the scores' scale by row
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q4 = lane >> 4;
   unsigned lb = bnh_xcd_block(blockIdx.x, gridDim.x);
   const int sl = (int)(lb % nsl), h = (int)(lb / nsl % p.H);
@@ -255,92 +257,127 @@ __global__ __launch_bounds__(256) void k_la_chunk(LaDev p, int nsl, int npc, int
   const int n = la_rows(p, b, &first), slot = la_slot(p, b);
   const int r0 = pc * pcr;
   if (OUT ? pc > 0 && r0 >= n : r0 + pcr >= n) return;  // no such piece, or a last one, whose state nobody takes
-  const int rows = n - r0 < pcr ? n - r0 : pcr;        // of this piece; 0: only a state to copy
-  const int c0 = sl * DV + wave * 16 * NC;             // this wave's columns
+  const int rows = n - r0 < pcr ? n - r0 : pcr;         // of this piece; 0: only a state to copy
+  const int c0 = sl * DV + wave * 16;                   // this wave's columns
   const long long pst = ((((long long)b * p.H + h) * nsl + sl) * (npc - 1)) * (KD * DV);  // this state's pieces
   const long long at = ((long long)slot * p.H + h) * p.dk * p.dv;
 
-  v4f S[2 * DKT][NC];  // rows 16 t + 4 q4 + r, column c0 + 16 nc + lr
-  bool some = false;   // whether the state may be other than zero
+  v4f S[2 * DKT];     // times 2^ux: rows 16 t + 4 q4 + r, column c0 + lr
+  int ux = 0;
+  bool some = false;  // whether the state may be other than zero
 #pragma unroll
-  for (int t = 0; t < 2 * DKT; t++)
-#pragma unroll
-    for (int c = 0; c < NC; c++) S[t][c] = (v4f){0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < 2 * DKT; t++) S[t] = (v4f){0.f, 0.f, 0.f, 0.f};
   if (OUT && pc > 0) {
     some = true;
-    const float *w = part + pst + (long long)(pc - 1) * (KD * DV) + wave * (KD * 16 * NC) + 4 * lane;
+    const float *w = part + pst + (long long)(pc - 1) * (KD * DV) + wave * (KD * 16) + 4 * lane;
 #pragma unroll
-    for (int t = 0; t < 2 * DKT; t++)
-#pragma unroll
-      for (int c = 0; c < NC; c++) S[t][c] = *(const v4f *)(w + 256 * (t * NC + c));
+    for (int t = 0; t < 2 * DKT; t++) S[t] = *(const v4f *)(w + 256 * t);
   } else if (pc == 0 && p.s0 && slot >= 0) {
     some = true;
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++)
 #pragma unroll
-      for (int c = 0; c < NC; c++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int kk = 16 * t + 4 * q4 + r, col = c0 + 16 * c + lr;
-          if (kk < p.dk && col < p.dv) S[t][c][r] = p.s0[at + (long long)kk * p.dv + col];
-        }
+      for (int r = 0; r < 4; r++) {
+        const int kk = 16 * t + 4 * q4 + r, col = c0 + lr;
+        if (kk < p.dk && col < p.dv) S[t][r] = p.s0[at + (long long)kk * p.dv + col];
+      }
   }
   if (OUT) {  // the blocks right of the diagonal that a step of 32 reads
-    for (int i = tid; i < C / 32 * 256; i += 256) s_p[(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] = (T)0.f;
+    for (int i = tid; i < C / 32 * 256; i += NT) s_p[(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] = (T)0.f;
   }
 
   const int kr = tid / (KD / VE), kc = tid % (KD / VE) * VE, vr = tid / (DV / VE), vc = tid % (DV / VE) * VE;
-  const T *qp = (const T *)p.q + ((long long)first + r0 + kr) * p.ldq + h / p.rq * p.dk;
-  const T *kp = (const T *)p.k + ((long long)first + r0 + kr) * p.ldk + h / p.rk * p.dk;
-  const T *vp = (const T *)p.v + ((long long)first + r0 + vr) * p.ldv + h / p.rv * p.dv + sl * DV;
+  const int vcols = p.dv - sl * DV;
+  const T *qp = (const T *)p.q + ((long long)first + r0) * p.ldq + h / p.rq * p.dk;
+  const T *kp = (const T *)p.k + ((long long)first + r0) * p.ldk + h / p.rk * p.dk;
+  const T *vp = (const T *)p.v + ((long long)first + r0) * p.ldv + h / p.rv * p.dv + sl * DV;
   uint4 qn[OUT ? NK : 1], kn[NK], vn[NV];
+  // the chunk from row t0 into registers. V: rows and columns outside come from a row and a column inside, and put() has
+  // zeros for them; no load waits on a branch
   auto load = [&](int t0) {
+    if (t0 >= rows) return;
 #pragma unroll
     for (int i = 0; i < NK; i++) {
-      const bool in = t0 + kr + RK * i < rows;
-      if (OUT) qn[i] = in ? row16<T, V>(qp + (long long)(t0 + RK * i) * p.ldq, kc, p.dk) : make_uint4(0, 0, 0, 0);
-      kn[i] = in ? row16<T, V>(kp + (long long)(t0 + RK * i) * p.ldk, kc, p.dk) : make_uint4(0, 0, 0, 0);
+      const int r = t0 + kr + RK * i;
+      if (V) {
+        const int rc = r < rows ? r : rows - 1, cc = kc < p.dk ? kc : 0;
+        if (OUT) qn[i] = *(const uint4 *)(qp + (long long)rc * p.ldq + cc);
+        kn[i] = *(const uint4 *)(kp + (long long)rc * p.ldk + cc);
+      } else {
+        if (OUT) qn[i] = r < rows ? row16<T, false>(qp + (long long)r * p.ldq, kc, p.dk) : make_uint4(0, 0, 0, 0);
+        kn[i] = r < rows ? row16<T, false>(kp + (long long)r * p.ldk, kc, p.dk) : make_uint4(0, 0, 0, 0);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++)
-      vn[i] = t0 + vr + RV * i < rows ? row16<T, V>(vp + (long long)(t0 + RV * i) * p.ldv, vc, p.dv - sl * DV)
-                                      : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < NV; i++) {
+      const int r = t0 + vr + RV * i;
+      if (V) vn[i] = *(const uint4 *)(vp + (long long)(r < rows ? r : rows - 1) * p.ldv + (vc < vcols ? vc : 0));
+      else vn[i] = r < rows ? row16<T, false>(vp + (long long)r * p.ldv, vc, vcols) : make_uint4(0, 0, 0, 0);
+    }
   };
-  // c of the chunk from row t0 and what follows from it, by one wave; rows past the end count as g = 0
+  auto put = [&](int t0) {
+    if (V && (t0 + C > rows || p.dk < KD || vcols < DV)) {
+#pragma unroll
+      for (int i = 0; i < NK; i++) {
+        const bool in = t0 + kr + RK * i < rows && kc < p.dk;
+        if (OUT && !in) qn[i] = make_uint4(0, 0, 0, 0);
+        if (!in) kn[i] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if (t0 + vr + RV * i >= rows || vc >= vcols) vn[i] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      if (RK > C && kr >= C) break;
+      if (OUT) *(uint4 *)(s_q + (kr + RK * i) * SK + kc) = qn[i];
+      *(uint4 *)(s_k + (kr + RK * i) * SK + kc) = kn[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      if (RV > C && vr >= C) break;
+      *(uint4 *)(s_v + (vr + RV * i) * SV + vc) = vn[i];
+    }
+  };
+  // c of the chunk from row t0 and what follows from it, by the last wave; rows past the end count as g = 0
   double ctot = 0;
-  auto sums = [&](int t0, int u) {
-    float g = 0.f;
-    if (lane < C && t0 + lane < rows) g = p.g[((long long)first + r0 + t0 + lane) * p.ldg + h];
-    g = g < -1e4f ? -1e4f : g;
-    double c = g;
+  float gn = 0.f;
+  auto gload = [&](int t0) {
+    gn = 0.f;
+    if (lane < C && t0 + lane < rows) gn = p.g[((long long)first + r0 + t0 + lane) * p.ldg + h];
+  };
+  auto sums = [&](int u) {
+    double c = gn < -1e4f ? -1e4f : gn;
 #pragma unroll
     for (int d = 1; d < C; d *= 2) {
       const double o = __shfl_up(c, d);
       c = lane >= d ? c + o : c;
     }
     const double last = __shfl(c, C - 1);
+    const float w = expf((float)(last - c));
+    float m = lane < C ? w : 0.f;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
     if (lane < C) {
       s_c[u][lane] = c;
       s_e[u][lane] = expf((float)c);
-      s_w[u][lane] = expf((float)(last - c));
-      if (lane == C - 1) s_d[u] = expf((float)c);
+      s_w[u][lane] = w;
+      if (lane == C - 1) s_d[u] = expf((float)c), s_m[u] = m;
     }
     ctot += last;
   };
 
   load(0);
-  if (wave == 0) sums(0, 0);
+  if (wave == NW - 1) {
+    gload(0);
+    sums(0);
+  }
   int u = 0;
   for (int t0 = 0; t0 < rows; t0 += C, u ^= 1) {
-#pragma unroll
-    for (int i = 0; i < NK; i++) {
-      if (OUT) *(uint4 *)(s_q + (kr + RK * i) * SK + kc) = qn[i];
-      *(uint4 *)(s_k + (kr + RK * i) * SK + kc) = kn[i];
-    }
-#pragma unroll
-    for (int i = 0; i < NV; i++) *(uint4 *)(s_v + (vr + RV * i) * SV + vc) = vn[i];
+    put(t0);
     __syncthreads();
     load(t0 + C);
+    if (wave == NW - 1) gload(t0 + C);
 
     if (OUT && wave < C / 16) {  // scores of rows 16 wave + lr, four columns a lane in each block of 16
       const int i = 16 * wave + lr;
@@ -363,13 +400,14 @@ __global__ __launch_bounds__(256) void k_la_chunk(LaDev p, int nsl, int npc, int
           for (int r = 0; r < 4; r++) {
             const int j = 16 * jb + 4 * q4 + r;
             a[jb][r] = j <= i ? a[jb][r] * __expf((float)(ci - s_c[u][j])) : 0.f;
-            m = fmaxf(m, fabsf(a[jb][r]));
+            if (F16) m = fmaxf(m, fabsf(a[jb][r]));
           }
-      int x = 0;
+      float dn = 1.f;
       if (F16) {
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        x = scale_exp(m);
+        const int x = scale_exp(m);
+        dn = ldexpf(1.f, -x);
         if (q4 == 0) s_x[i] = x;
       }
 #pragma unroll
@@ -377,116 +415,107 @@ __global__ __launch_bounds__(256) void k_la_chunk(LaDev p, int nsl, int npc, int
         if (jb <= wave) {
           FH y;
 #pragma unroll
-          for (int r = 0; r < 4; r++) y[r] = (T)(F16 ? ldexpf(a[jb][r], -x) : a[jb][r]);
+          for (int r = 0; r < 4; r++) y[r] = (T)(F16 ? a[jb][r] * dn : a[jb][r]);
           *(FH *)(s_p + i * SP + 16 * jb + 4 * q4) = y;
         }
     }
-    if (wave == 0 && t0 + C < rows) sums(t0 + C, u ^ 1);
-    FV vf[C / 32][NC];
-    bool odd = false;  // whether a value of v is not finite
+    if (wave == NW - 1 && t0 + C < rows) sums(u ^ 1);
+    FV vf[C / 32];
 #pragma unroll
-    for (int j = 0; j < C / 32; j++)
-#pragma unroll
-      for (int c = 0; c < NC; c++) {
-        vf[j][c] = col8(s_v + 32 * j * SV + wave * 16 * NC + 16 * c, SV, lane);
-        T z = (T)0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) z += vf[j][c][e] * (T)0.f;
-        odd = odd || z != z;
-      }
-    if (OUT) {
-      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-      FV sf[DKT][NC];
-      int sx[NC];
-      float xs[NC][4];  // 2^x of the accumulators' columns 4 q4 + r
-      if (some) {
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-          sx[c] = 0;
-          if (F16) {
-            float m = 0.f;
-#pragma unroll
-            for (int t = 0; t < 2 * DKT; t++)
-#pragma unroll
-              for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(S[t][c][r]));
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            sx[c] = scale_exp(m);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; r++) xs[c][r] = F16 ? ldexpf(1.f, __shfl(sx[c], 4 * q4 + r)) : 1.f;
-          const float dn = ldexpf(1.f, -sx[c]);
-#pragma unroll
-          for (int d = 0; d < DKT; d++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) sf[d][c][e] = (T)(F16 ? S[2 * d + e / 4][c][e % 4] * dn : S[2 * d + e / 4][c][e % 4]);
-        }
-      }
-      FV vz[C / 32][NC];
+    for (int j = 0; j < C / 32; j++) vf[j] = col8(s_v + 32 * j * SV + wave * 16, SV, lane);
+    // the largest |v| of the lane's, and whether a value of v is not finite
+    float vm = 0.f;
+    bool odd = false;
+    if constexpr (F16) {
+      typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+      u2 m = {0, 0};
 #pragma unroll
       for (int j = 0; j < C / 32; j++)
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-          vz[j][c] = vf[j][c];
-          if (odd)
-#pragma unroll
-            for (int e = 0; e < 8; e++) vz[j][c][e] = vf[j][c][e] - vf[j][c][e] == (T)0.f ? vf[j][c][e] : (T)0.f;
+        for (int e = 0; e < 8; e += 2) {
+          const u2 x = {(unsigned short)(hbits(vf[j][e]) & 0x7fff), (unsigned short)(hbits(vf[j][e + 1]) & 0x7fff)};
+          m = __builtin_elementwise_max(m, x);
         }
+      const unsigned short mm = m[0] > m[1] ? m[0] : m[1];
+      odd = mm >= 0x7c00;
+      vm = (float)hfrom(mm);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) odd = odd || vf[j][e] - vf[j][e] != 0.f;
+    }
+    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    if (OUT) {
+      FV sf[DKT];
+      float xs[4];  // 2^x of the accumulators' columns 4 q4 + r
+      if (some) {
+        float dn = 1.f;
+        if (F16) {
+          float m = 0.f;
+#pragma unroll
+          for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(S[t][r]));
+          m = fmaxf(m, __shfl_xor(m, 16));
+          m = fmaxf(m, __shfl_xor(m, 32));
+          const int x = scale_exp(m);
+          const float up = ldexpf(1.f, x + ux);
+          dn = ldexpf(1.f, -x);
+#pragma unroll
+          for (int r = 0; r < 4; r++) xs[r] = __shfl(up, 4 * q4 + r);
+        }
+#pragma unroll
+        for (int d = 0; d < DKT; d++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) sf[d][e] = (T)(F16 ? S[2 * d + e / 4][e % 4] * dn : S[2 * d + e / 4][e % 4]);
+      }
+      FV vz[C / 32];
+#pragma unroll
+      for (int j = 0; j < C / 32; j++) {
+        vz[j] = vf[j];
+        if (odd)
+#pragma unroll
+          for (int e = 0; e < 8; e++) vz[j][e] = vf[j][e] - vf[j][e] == (T)0.f ? vf[j][e] : (T)0.f;
+      }
       __syncthreads();
 #pragma unroll
       for (int ib = 0; ib < C / 16; ib++) {
         if (t0 + 16 * ib >= rows) break;
         const int i = 16 * ib + lr;
-        v4f a[NC];
-#pragma unroll
-        for (int c = 0; c < NC; c++) a[c] = (v4f){0.f, 0.f, 0.f, 0.f};
+        v4f a = (v4f){0.f, 0.f, 0.f, 0.f};
         const float ec = s_e[u][i], dn = F16 ? ldexpf(ec, -s_x[i]) : ec, up = F16 ? ldexpf(p.scale, s_x[i]) : p.scale;
         if (some) {
 #pragma unroll
-          for (int d = 0; d < DKT; d++) {
-            const FV x = row44<T>(s_q + i * SK + 32 * d + 4 * q4);
+          for (int d = 0; d < DKT; d++) a = mma(sf[d], row44<T>(s_q + i * SK + 32 * d + 4 * q4), a);
 #pragma unroll
-            for (int c = 0; c < NC; c++) a[c] = mma(sf[d][c], x, a[c]);
-          }
-#pragma unroll
-          for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) a[c][r] *= xs[c][r] * dn;
+          for (int r = 0; r < 4; r++) a[r] *= F16 ? xs[r] * dn : dn;
         }
 #pragma unroll
-        for (int j = 0; j <= ib / 2; j++) {
-          const FV x = row8<T>(s_p + i * SP + 32 * j + 8 * q4);
-#pragma unroll
-          for (int c = 0; c < NC; c++) a[c] = mma(vz[j][c], x, a[c]);
-        }
+        for (int j = 0; j <= ib / 2; j++) a = mma(vz[j], row8<T>(s_p + i * SP + 32 * j + 8 * q4), a);
         if (odd) {
-          for (int j = 0; j < 16 * ib + 16; j++) {
-            if (j > i) continue;
+#pragma unroll 1
+          for (int j = 0; j <= i; j++) {
             const float x = (float)s_p[i * SP + j];
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const float y = (float)s_v[j * SV + wave * 16 * NC + 16 * c + 4 * q4 + r];
-                if (y - y != 0.f) a[c][r] += x * y;
-              }
+            for (int r = 0; r < 4; r++) {
+              const float y = (float)s_v[j * SV + wave * 16 + 4 * q4 + r];
+              if (y - y != 0.f) a[r] += x * y;
+            }
           }
         }
         if (t0 + i < rows) {
-          T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv;
+          const int col = c0 + 4 * q4;
+          T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv + col;
+          FH y;
 #pragma unroll
-          for (int c = 0; c < NC; c++) {
-            const int col = c0 + 16 * c + 4 * q4;
-            FH y;
+          for (int r = 0; r < 4; r++) y[r] = (T)(up * a[r]);
+          if (V) {
+            if (col < p.dv) *(FH *)o = y;
+          } else {
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = (T)(up * a[c][r]);
-            if (V) {
-              if (col < p.dv) *(FH *)(o + col) = y;
-            } else {
-#pragma unroll
-              for (int r = 0; r < 4; r++)
-                if (col + r < p.dv) o[col + r] = y[r];
-            }
+            for (int r = 0; r < 4; r++)
+              if (col + r < p.dv) o[r] = y[r];
           }
         }
       }
@@ -494,90 +523,73 @@ __global__ __launch_bounds__(256) void k_la_chunk(LaDev p, int nsl, int npc, int
       __syncthreads();
     }
     // the state's update
-    const float dec = s_d[u];
-    FV hi[C / 32][NC], lo[C / 32][NC];
-    float up[NC];  // what the products are multiplied by, a power of two a column
-    {
-      float w[C / 32][8];
+    FV hi[C / 32], lo[C / 32];
+    float dec = s_d[u], dn = 1.f;
+    if (F16) {
+      float m = fmaxf(vm, __shfl_xor(vm, 16));
+      m = fmaxf(m, __shfl_xor(m, 32)) * s_m[u];
+      const int e = (int)(__float_as_uint(m) >> 23 & 255) - 127;
+      const int x = m == 0.f ? ux : e > 127 ? 0 : e - 14;  // the largest to 2^14..2^15
+      dn = ldexpf(1.f, -x);
+      dec = ldexpf(dec, ux - x);
+      ux = x;
+    }
+#pragma unroll
+    for (int j = 0; j < C / 32; j++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float w = s_w[u][32 * j + 8 * q4 + e];
+        if (F16) {
+          const float y = __builtin_fmaf((float)vf[j][e], w * dn, 0.f);
+          hi[j][e] = (T)y;
+          lo[j][e] = (T)(y - (float)hi[j][e]);
+        } else {
+          hi[j][e] = (T)((float)vf[j][e] * w);
+        }
+      }
+    if (F16 && odd) {  // an infinity has no second part
 #pragma unroll
       for (int j = 0; j < C / 32; j++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[j][e] = s_w[u][32 * j + 8 * q4 + e];
-#pragma unroll
-      for (int c = 0; c < NC; c++) {
-        float dn = 1.f;
-        up[c] = 1.f;
-        if (F16) {
-          float m = 0.f;
-#pragma unroll
-          for (int j = 0; j < C / 32; j++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf((float)vf[j][c][e] * w[j][e]));
-          m = fmaxf(m, __shfl_xor(m, 16));
-          m = fmaxf(m, __shfl_xor(m, 32));
-          const int x = scale_exp(m);
-          up[c] = ldexpf(1.f, x);
-          dn = ldexpf(1.f, -x);
-        }
-#pragma unroll
-        for (int j = 0; j < C / 32; j++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float y = (float)vf[j][c][e] * w[j][e] * dn;
-            hi[j][c][e] = (T)y;
-            if (F16) {
-              const float d = y - (float)hi[j][c][e];
-              lo[j][c][e] = (T)(d - d == 0.f ? 2048.f * d : 0.f);
-            }
-          }
-      }
+        for (int e = 0; e < 8; e++) lo[j][e] = hi[j][e] - hi[j][e] == (T)0.f ? lo[j][e] : (T)0.f;
     }
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++) {
       FV kf[C / 32];
 #pragma unroll
       for (int j = 0; j < C / 32; j++) kf[j] = col8(s_k + 32 * j * SK + 16 * t, SK, lane);
+      if (some)
 #pragma unroll
-      for (int c = 0; c < NC; c++) {
-        if (some)
+        for (int r = 0; r < 4; r++) S[t][r] *= dec;
+      if (F16)
 #pragma unroll
-          for (int r = 0; r < 4; r++) S[t][c][r] *= dec;
-        if (F16) {
-          v4f l = (v4f){0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < C / 32; j++) S[t] = mma(kf[j], lo[j], S[t]);
 #pragma unroll
-          for (int j = 0; j < C / 32; j++) l = mma(kf[j], lo[j][c], l);
-#pragma unroll
-          for (int r = 0; r < 4; r++) l[r] *= 1.f / 2048;
-#pragma unroll
-          for (int j = 0; j < C / 32; j++) l = mma(kf[j], hi[j][c], l);
-#pragma unroll
-          for (int r = 0; r < 4; r++) S[t][c][r] = __builtin_fmaf(l[r], up[c], S[t][c][r]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < C / 32; j++) S[t][c] = mma(kf[j], hi[j][c], S[t][c]);
-        }
-      }
+      for (int j = 0; j < C / 32; j++) S[t] = mma(kf[j], hi[j], S[t]);
     }
     some = true;
     __syncthreads();
   }
-  if (!OUT) {
-    float *w = part + pst + (long long)pc * (KD * DV) + wave * (KD * 16 * NC) + 4 * lane;
+  if (F16) {
+    const float up = ldexpf(1.f, ux);
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++)
 #pragma unroll
-      for (int c = 0; c < NC; c++) *(v4f *)(w + 256 * (t * NC + c)) = S[t][c];
-    if (tid == 0) pdec[(((long long)b * p.H + h) * nsl + sl) * (npc - 1) + pc] = expf((float)ctot);
+      for (int r = 0; r < 4; r++) S[t][r] *= up;
+  }
+  if (!OUT) {
+    float *w = part + pst + (long long)pc * (KD * DV) + wave * (KD * 16) + 4 * lane;
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++) *(v4f *)(w + 256 * t) = S[t];
+    if (wave == NW - 1 && lane == 0) pdec[(((long long)b * p.H + h) * nsl + sl) * (npc - 1) + pc] = expf((float)ctot);
   } else if (p.s1 && slot >= 0 && r0 + pcr >= n) {
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++)
 #pragma unroll
-      for (int c = 0; c < NC; c++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int kk = 16 * t + 4 * q4 + r, col = c0 + 16 * c + lr;
-          if (kk < p.dk && col < p.dv) p.s1[at + (long long)kk * p.dv + col] = S[t][c][r];
-        }
+      for (int r = 0; r < 4; r++) {
+        const int kk = 16 * t + 4 * q4 + r, col = c0 + lr;
+        if (kk < p.dk && col < p.dv) p.s1[at + (long long)kk * p.dv + col] = S[t][r];
+      }
   }
 }
 
@@ -606,18 +618,18 @@ __global__ __launch_bounds__(256) void k_la_scan(LaDev p, int npc, int pcr, int 
 // How a call is cut: dk and dv in tiles, and rows in pieces
 struct Plan {
   bool chunk;
-  int dkt, nc, c, nsl, npc, pcr;
+  int dkt, nw, c, nsl, npc, pcr;
   long long states, floats;  // of a state
 };
 Plan plan(const bnh_la *p, int T, int B) {
   Plan r;
   r.chunk = T > 8;
   r.dkt = p->dk <= 32 ? 1 : p->dk <= 64 ? 2 : p->dk <= 128 ? 4 : 8;
-  r.nc = p->f16 && r.dkt <= 4 && p->dv > 64 ? 2 : 1;
+  r.nw = p->dv > 64 ? 8 : 4;
   r.c = p->f16 ? 64 : 32;
-  r.nsl = (int)bnh_ceil_div(p->dv, 64 * r.nc);
+  r.nsl = (int)bnh_ceil_div(p->dv, 16 * r.nw);
   r.states = (long long)B * p->H * r.nsl;
-  r.floats = 32LL * r.dkt * 64 * r.nc;
+  r.floats = 32LL * r.dkt * 16 * r.nw;
   r.npc = 1;
   r.pcr = T;
   if (r.chunk) {
@@ -634,38 +646,37 @@ size_t plan_bytes(const Plan &r) {
   return (size_t)(bnh_round_up(4 * r.states * (r.npc - 1) * r.floats, 256) + bnh_round_up(4 * r.states * (r.npc - 1), 256));
 }
 
-template <typename T, int DKT, int NC, int C, bool V>
-int chunk_run(const LaDev &d, const Plan &r, int B, void *work, hipStream_t s) {
+template <typename T, int DKT, int NW, int C, bool V>
+int chunk_run(const LaDev &d, const Plan &r, void *work, hipStream_t s) {
   float *part = (float *)work, *pdec = part ? (float *)((char *)work + bnh_round_up(4 * r.states * (r.npc - 1) * r.floats, 256)) : nullptr;
+  const dim3 block(64 * NW);
   if (r.npc > 1) {
-    hipLaunchKernelGGL((k_la_chunk<T, DKT, NC, C, V, false>), dim3((unsigned)(r.states * (r.npc - 1))), dim3(256), 0, s, d,
-                       r.nsl, r.npc, r.pcr, part, pdec);
+    hipLaunchKernelGGL((k_la_chunk<T, DKT, NW, C, V, false>), dim3((unsigned)(r.states * (r.npc - 1))), block, 0, s, d, r.nsl,
+                       r.npc, r.pcr, part, pdec);
     BNH_HIP(hipGetLastError());
-    const int quads = (int)(r.floats / 4);
     if (r.npc > 2) {
+      const int quads = (int)(r.floats / 4);
       hipLaunchKernelGGL(k_la_scan, dim3((unsigned)bnh_ceil_div(quads, 256), (unsigned)r.states), dim3(256), 0, s, d, r.npc,
                          r.pcr, quads, r.nsl, part, pdec);
       BNH_HIP(hipGetLastError());
     }
   }
-  hipLaunchKernelGGL((k_la_chunk<T, DKT, NC, C, V, true>), dim3((unsigned)(r.states * r.npc)), dim3(256), 0, s, d, r.nsl,
-                     r.npc, r.pcr, part, pdec);
+  hipLaunchKernelGGL((k_la_chunk<T, DKT, NW, C, V, true>), dim3((unsigned)(r.states * r.npc)), block, 0, s, d, r.nsl, r.npc,
+                     r.pcr, part, pdec);
   BNH_HIP(hipGetLastError());
   return 0;
 }
-template <typename T, int C, bool V>
-int chunk_go(const LaDev &d, const Plan &r, int B, void *work, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    if (r.nc == 2) {
-      if (r.dkt == 1) return chunk_run<T, 1, 2, C, V>(d, r, B, work, s);
-      if (r.dkt == 2) return chunk_run<T, 2, 2, C, V>(d, r, B, work, s);
-      return chunk_run<T, 4, 2, C, V>(d, r, B, work, s);
-    }
-  }
-  if (r.dkt == 1) return chunk_run<T, 1, 1, C, V>(d, r, B, work, s);
-  if (r.dkt == 2) return chunk_run<T, 2, 1, C, V>(d, r, B, work, s);
-  if (r.dkt == 4) return chunk_run<T, 4, 1, C, V>(d, r, B, work, s);
-  return chunk_run<T, 8, 1, C, V>(d, r, B, work, s);
+template <typename T, int NW, int C, bool V>
+int chunk_dk(const LaDev &d, const Plan &r, void *work, hipStream_t s) {
+  if (r.dkt == 1) return chunk_run<T, 1, NW, C, V>(d, r, work, s);
+  if (r.dkt == 2) return chunk_run<T, 2, NW, C, V>(d, r, work, s);
+  if (r.dkt == 4) return chunk_run<T, 4, NW, C, V>(d, r, work, s);
+  return chunk_run<T, 8, NW, C, V>(d, r, work, s);
+}
+template <typename T, int C>
+int chunk_go(const LaDev &d, const Plan &r, bool v, void *work, hipStream_t s) {
+  if (r.nw == 8) return v ? chunk_dk<T, 8, C, true>(d, r, work, s) : chunk_dk<T, 8, C, false>(d, r, work, s);
+  return v ? chunk_dk<T, 4, C, true>(d, r, work, s) : chunk_dk<T, 4, C, false>(d, r, work, s);
 }
 
 int la_check(const bnh_la *p, int T, int B) {
@@ -709,8 +720,7 @@ int bnh_linattn(const bnh_la *p, int T, int B, int rows, const int32_t *start, c
     const int ve = 16 / (int)es;
     const bool v = on(p->q, 16) && on(p->k, 16) && on(p->v, 16) && on(p->o, 16) && p->ldq % ve == 0 && p->ldk % ve == 0 &&
                    p->ldv % ve == 0 && p->ldo % ve == 0 && p->dk % ve == 0 && p->dv % ve == 0;
-    if (p->f16) return v ? chunk_go<h16, 64, true>(d, r, B, work, s) : chunk_go<h16, 64, false>(d, r, B, work, s);
-    return v ? chunk_go<float, 32, true>(d, r, B, work, s) : chunk_go<float, 32, false>(d, r, B, work, s);
+    return p->f16 ? chunk_go<h16, 64>(d, r, v, work, s) : chunk_go<float, 32>(d, r, v, work, s);
   }
   if (p->f16) return vs ? step_run<h16, 32, true>(d, B, s) : step_run<h16, 32, false>(d, B, s);
   return vs ? step_run<float, 32, true>(d, B, s) : step_run<float, 32, false>(d, B, s);
