@@ -192,19 +192,20 @@ __device__ __forceinline__ typename Frag<T>::V row44(const T *p) {
   const typename Frag<T>::H a = *(const typename Frag<T>::H *)p, b = *(const typename Frag<T>::H *)(p + 16);
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// steps 8 q + e of column lane & 15 of a matrix at p whose rows (a step each) are `ld` apart
-__device__ __forceinline__ v8h col8(const h16 *p, int ld, int lane) {
-  const h16 *a = p + (8 * (lane >> 4) + ((lane & 15) >> 2)) * ld + 4 * (lane & 3);
+// the same steps of column lane & 15 of a matrix at p whose rows (a step each) are `ld` apart: a group of 16 lanes reads 4
+// rows of 16 values and gets them by column; rows an odd number of 32 bytes apart fall on different banks
+__device__ __forceinline__ v8h col44(const h16 *p, int ld, int lane) {
+  const h16 *a = p + (4 * (lane >> 4) + ((lane & 15) >> 2)) * ld + 4 * (lane & 3);
   typedef __attribute__((address_space(3))) v4s L;
-  const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(a + 4 * ld));
+  const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(a + 16 * ld));
   typedef short v8s __attribute__((ext_vector_type(8)));
   const v8s z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_bit_cast(v8h, z);
 }
-__device__ __forceinline__ v8f col8(const float *p, int ld, int lane) {
+__device__ __forceinline__ v8f col44(const float *p, int ld, int lane) {
   v8f r;
 #pragma unroll
-  for (int e = 0; e < 8; e++) r[e] = p[(8 * (lane >> 4) + e) * ld + (lane & 15)];
+  for (int e = 0; e < 8; e++) r[e] = p[(4 * (lane >> 4) + e + (e < 4 ? 0 : 12)) * ld + (lane & 15)];
   return r;
 }
 // 2^-e that takes a largest value m to 2^12..2^13: 0 and infinities are left as they are, and nothing grows past 2^24
@@ -238,16 +239,17 @@ __device__ __forceinline__ uint4 row16(const T *p, int c, int cols) {
 template <typename T, int DKT, int NW, int C, bool V, bool OUT>
 __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc, int pcr, float *part, float *pdec) {
   constexpr bool F16 = sizeof(T) == 2;
-  constexpr int VE = 16 / sizeof(T), KD = 32 * DKT, DV = 16 * NW, NT = 64 * NW, SK = KD + VE, SV = DV + VE, SP = C + VE;
+  constexpr int VE = 16 / sizeof(T), KD = 32 * DKT, DV = 16 * NW, NT = 64 * NW, SQ = KD + VE, SP = C + VE;
+  constexpr int SK = KD + (F16 ? 16 : 4), SV = DV + (F16 ? 16 : 4);
   constexpr int RK = NT * VE / KD, RV = NT * VE / DV;                          // rows that one load of all threads covers
   constexpr int NK = C / RK > 0 ? C / RK : 1, NV = C / RV > 0 ? C / RV : 1;
   typedef typename Frag<T>::V FV;
   typedef typename Frag<T>::H FH;
-  __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SK : 1], s_k[C * SK], s_v[C * SV], s_p[OUT ? C * SP : 1];
+  __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SQ : 1], s_k[C * SK], s_v[C * SV], s_p[OUT ? C * SP : 1];
   __shared__ double s_c[2][64];                              // c_i
   __shared__ __attribute__((aligned(16))) float s_w[2][64];  // e^{c_C - c_j}
   __shared__ float s_e[2][64], s_d[2], s_m[2];               // e^{c_i}; e^{c_C}; the largest of s_w
-  __shared__ int s_x[64];                                    // the scores' scale by row
+  __shared__ int s_x[2][64];                                 // the scores' scale by row and by step of 32 columns
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q4 = lane >> 4;
   unsigned lb = bnh_xcd_block(blockIdx.x, gridDim.x);
   const int sl = (int)(lb % nsl), h = (int)(lb / nsl % p.H);
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
 #pragma unroll
     for (int i = 0; i < NK; i++) {
       if (RK > C && kr >= C) break;
-      if (OUT) *(uint4 *)(s_q + (kr + RK * i) * SK + kc) = qn[i];
+      if (OUT) *(uint4 *)(s_q + (kr + RK * i) * SQ + kc) = qn[i];
       *(uint4 *)(s_k + (kr + RK * i) * SK + kc) = kn[i];
     }
 #pragma unroll
@@ -379,50 +381,51 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
     load(t0 + C);
     if (wave == NW - 1) gload(t0 + C);
 
-    if (OUT && wave < C / 16) {  // scores of rows 16 wave + lr, four columns a lane in each block of 16
-      const int i = 16 * wave + lr;
-      const double ci = s_c[u][i];
-      v4f a[C / 16];
-      float m = 0.f;
+    if constexpr (OUT) {  // scores of 16 rows and 32 columns a unit, a row a lane and four columns in each block of 16
+      constexpr int UN = C == 64 ? 6 : 2;
+#pragma unroll 1
+      for (int un = wave; un < UN; un += NW) {
+        const int ib = C == 64 ? 0x021233 >> 4 * un & 15 : 1 - un, jj = C == 64 ? 0x010010 >> 4 * un & 15 : 0;
+        const int i = 16 * ib + lr;
+        const bool two = 2 * jj + 1 <= ib;  // the second block is not all right of the diagonal
+        const double ci = s_c[u][i];
+        v4f a[2] = {(v4f){0.f, 0.f, 0.f, 0.f}, (v4f){0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int jb = 0; jb < C / 16; jb++) a[jb] = (v4f){0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < DKT; d++) {
+          const FV x = row8<T>(s_q + i * SQ + 32 * d + 8 * q4);
+          a[0] = mma(row8<T>(s_k + (32 * jj + lr) * SK + 32 * d + 8 * q4), x, a[0]);
+          a[1] = mma(row8<T>(s_k + (32 * jj + 16 + lr) * SK + 32 * d + 8 * q4), x, a[1]);
+        }
+        float m = 0.f;
 #pragma unroll
-      for (int d = 0; d < DKT; d++) {
-        const FV x = row8<T>(s_q + i * SK + 32 * d + 8 * q4);
-#pragma unroll
-        for (int jb = 0; jb < C / 16; jb++)
-          if (jb <= wave) a[jb] = mma(row8<T>(s_k + (16 * jb + lr) * SK + 32 * d + 8 * q4), x, a[jb]);
-      }
-#pragma unroll
-      for (int jb = 0; jb < C / 16; jb++)
-        if (jb <= wave)
+        for (int c = 0; c < 2; c++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const int j = 16 * jb + 4 * q4 + r;
-            a[jb][r] = j <= i ? a[jb][r] * __expf((float)(ci - s_c[u][j])) : 0.f;
-            if (F16) m = fmaxf(m, fabsf(a[jb][r]));
+            const int j = 32 * jj + 16 * c + 4 * q4 + r;
+            a[c][r] = j <= i ? a[c][r] * __expf((float)(ci - s_c[u][j])) : 0.f;
+            m = fmaxf(m, fabsf(a[c][r]));
           }
-      float dn = 1.f;
-      if (F16) {
-        m = fmaxf(m, __shfl_xor(m, 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        const int x = scale_exp(m);
-        dn = ldexpf(1.f, -x);
-        if (q4 == 0) s_x[i] = x;
-      }
+        float dn = 1.f;
+        if (F16) {
+          m = fmaxf(m, __shfl_xor(m, 16));
+          m = fmaxf(m, __shfl_xor(m, 32));
+          const int x = scale_exp(m);
+          dn = ldexpf(1.f, -x);
+          if (q4 == 0) s_x[jj][i] = x;
+        }
 #pragma unroll
-      for (int jb = 0; jb < C / 16; jb++)
-        if (jb <= wave) {
+        for (int c = 0; c < 2; c++) {
           FH y;
 #pragma unroll
-          for (int r = 0; r < 4; r++) y[r] = (T)(F16 ? a[jb][r] * dn : a[jb][r]);
-          *(FH *)(s_p + i * SP + 16 * jb + 4 * q4) = y;
+          for (int r = 0; r < 4; r++) y[r] = (T)(F16 ? a[c][r] * dn : a[c][r]);
+          if (c == 0 || two) *(FH *)(s_p + i * SP + 32 * jj + 16 * c + 4 * q4) = y;
         }
+      }
     }
     if (wave == NW - 1 && t0 + C < rows) sums(u ^ 1);
     FV vf[C / 32];
 #pragma unroll
-    for (int j = 0; j < C / 32; j++) vf[j] = col8(s_v + 32 * j * SV + wave * 16, SV, lane);
+    for (int j = 0; j < C / 32; j++) vf[j] = col44(s_v + 32 * j * SV + wave * 16, SV, lane);
     // the largest |v| of the lane's, and whether a value of v is not finite
     float vm = 0.f;
     bool odd = false;
@@ -479,44 +482,64 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
           for (int e = 0; e < 8; e++) vz[j][e] = vf[j][e] - vf[j][e] == (T)0.f ? vf[j][e] : (T)0.f;
       }
       __syncthreads();
+      v4f a[C / 16];
 #pragma unroll
-      for (int ib = 0; ib < C / 16; ib++) {
-        if (t0 + 16 * ib >= rows) break;
-        const int i = 16 * ib + lr;
-        v4f a = (v4f){0.f, 0.f, 0.f, 0.f};
-        const float ec = s_e[u][i], dn = F16 ? ldexpf(ec, -s_x[i]) : ec, up = F16 ? ldexpf(p.scale, s_x[i]) : p.scale;
-        if (some) {
+      for (int ib = 0; ib < C / 16; ib++) a[ib] = (v4f){0.f, 0.f, 0.f, 0.f};
+      if (some) {
 #pragma unroll
-          for (int d = 0; d < DKT; d++) a = mma(sf[d], row44<T>(s_q + i * SK + 32 * d + 4 * q4), a);
+        for (int d = 0; d < DKT; d++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) a[r] *= F16 ? xs[r] * dn : dn;
+          for (int ib = 0; ib < C / 16; ib++) a[ib] = mma(sf[d], row44<T>(s_q + (16 * ib + lr) * SQ + 32 * d + 4 * q4), a[ib]);
+      }
+#pragma unroll
+      for (int ib = 0; ib < C / 16; ib++) {  // each step of 32 columns in its own unit
+        const int i = 16 * ib + lr, x0 = F16 ? s_x[0][i] : 0, x1 = F16 && ib >= 2 ? s_x[1][i] : 0;
+        const float ec = F16 ? ldexpf(s_e[u][i], -x0) : s_e[u][i];
+        if (some)
+#pragma unroll
+          for (int r = 0; r < 4; r++) a[ib][r] *= F16 ? xs[r] * ec : ec;
+        a[ib] = mma(vz[0], row44<T>(s_p + i * SP + 4 * q4), a[ib]);
+        if constexpr (C == 64) {
+          if (ib >= 2) {
+            if (F16)
+#pragma unroll
+              for (int r = 0; r < 4; r++) a[ib][r] = ldexpf(a[ib][r], x0 - x1);
+            a[ib] = mma(vz[1], row44<T>(s_p + i * SP + 32 + 4 * q4), a[ib]);
+          }
         }
+        const float up = F16 ? ldexpf(p.scale, ib >= 2 ? x1 : x0) : p.scale;
 #pragma unroll
-        for (int j = 0; j <= ib / 2; j++) a = mma(vz[j], row8<T>(s_p + i * SP + 32 * j + 8 * q4), a);
-        if (odd) {
+        for (int r = 0; r < 4; r++) a[ib][r] *= up;
+      }
+      if (odd) {
+#pragma unroll
+        for (int ib = 0; ib < C / 16; ib++) {
+          const int i = 16 * ib + lr;
 #pragma unroll 1
           for (int j = 0; j <= i; j++) {
-            const float x = (float)s_p[i * SP + j];
+            const float x = p.scale * ldexpf((float)s_p[i * SP + j], F16 ? s_x[j / 32][i] : 0);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
               const float y = (float)s_v[j * SV + wave * 16 + 4 * q4 + r];
-              if (y - y != 0.f) a[r] += x * y;
+              if (y - y != 0.f) a[ib][r] += x * y;
             }
           }
         }
-        if (t0 + i < rows) {
-          const int col = c0 + 4 * q4;
-          T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv + col;
-          FH y;
+      }
 #pragma unroll
-          for (int r = 0; r < 4; r++) y[r] = (T)(up * a[r]);
-          if (V) {
-            if (col < p.dv) *(FH *)o = y;
-          } else {
+      for (int ib = 0; ib < C / 16; ib++) {
+        const int i = 16 * ib + lr, col = c0 + 4 * q4;
+        if (t0 + i >= rows) continue;
+        T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv + col;
+        FH y;
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-              if (col + r < p.dv) o[r] = y[r];
-          }
+        for (int r = 0; r < 4; r++) y[r] = (T)a[ib][r];
+        if (V) {
+          if (col < p.dv) *(FH *)o = y;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (col + r < p.dv) o[r] = y[r];
         }
       }
     } else {
@@ -538,7 +561,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
     for (int j = 0; j < C / 32; j++)
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float w = s_w[u][32 * j + 8 * q4 + e];
+        const float w = s_w[u][32 * j + 4 * q4 + e + (e < 4 ? 0 : 12)];
         if (F16) {
           const float y = __builtin_fmaf((float)vf[j][e], w * dn, 0.f);
           hi[j][e] = (T)y;
@@ -557,7 +580,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
     for (int t = 0; t < 2 * DKT; t++) {
       FV kf[C / 32];
 #pragma unroll
-      for (int j = 0; j < C / 32; j++) kf[j] = col8(s_k + 32 * j * SK + 16 * t, SK, lane);
+      for (int j = 0; j < C / 32; j++) kf[j] = col44(s_k + 32 * j * SK + 16 * t, SK, lane);
       if (some)
 #pragma unroll
         for (int r = 0; r < 4; r++) S[t][r] *= dec;
