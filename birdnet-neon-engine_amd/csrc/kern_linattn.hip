@@ -245,11 +245,11 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
   constexpr int NK = C / RK > 0 ? C / RK : 1, NV = C / RV > 0 ? C / RV : 1;
   typedef typename Frag<T>::V FV;
   typedef typename Frag<T>::H FH;
-  __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SQ : 1], s_k[C * SK], s_v[C * SV], s_p[OUT ? C * SP : 1];
+  __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SQ : 1], s_k[C * SK], s_v[C * SV], s_p[2][OUT ? C * SP : 1];
   __shared__ double s_c[2][64];                              // c_i
   __shared__ __attribute__((aligned(16))) float s_w[2][64];  // e^{c_C - c_j}
   __shared__ float s_e[2][64], s_d[2], s_m[2];               // e^{c_i}; e^{c_C}; the largest of s_w
-  __shared__ int s_x[2][64];                                 // the scores' scale by row and by step of 32 columns
+  __shared__ int s_x[2][2][64];                              // the scores' scale by step of 32 columns and row
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q4 = lane >> 4;
   unsigned lb = bnh_xcd_block(blockIdx.x, gridDim.x);
   const int sl = (int)(lb % nsl), h = (int)(lb / nsl % p.H);
@@ -266,16 +266,13 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
 
   v4f S[2 * DKT];     // times 2^ux: rows 16 t + 4 q4 + r, column c0 + lr
   int ux = 0;
-  bool some = false;  // whether the state may be other than zero
 #pragma unroll
   for (int t = 0; t < 2 * DKT; t++) S[t] = (v4f){0.f, 0.f, 0.f, 0.f};
   if (OUT && pc > 0) {
-    some = true;
     const float *w = part + pst + (long long)(pc - 1) * (KD * DV) + wave * (KD * 16) + 4 * lane;
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++) S[t] = *(const v4f *)(w + 256 * t);
   } else if (pc == 0 && p.s0 && slot >= 0) {
-    some = true;
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++)
 #pragma unroll
@@ -285,7 +282,9 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
       }
   }
   if (OUT) {  // the blocks right of the diagonal that a step of 32 reads
-    for (int i = tid; i < C / 32 * 256; i += NT) s_p[(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] = (T)0.f;
+    for (int i = tid; i < C / 32 * 256; i += NT)
+      s_p[0][(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] =
+          s_p[1][(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] = (T)0.f;
   }
 
   const int kr = tid / (KD / VE), kc = tid % (KD / VE) * VE, vr = tid / (DV / VE), vc = tid % (DV / VE) * VE;
@@ -411,14 +410,14 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
           m = fmaxf(m, __shfl_xor(m, 32));
           const int x = scale_exp(m);
           dn = ldexpf(1.f, -x);
-          if (q4 == 0) s_x[jj][i] = x;
+          if (q4 == 0) s_x[u][jj][i] = x;
         }
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           FH y;
 #pragma unroll
           for (int r = 0; r < 4; r++) y[r] = (T)(F16 ? a[c][r] * dn : a[c][r]);
-          if (c == 0 || two) *(FH *)(s_p + i * SP + 32 * jj + 16 * c + 4 * q4) = y;
+          if (c == 0 || two) *(FH *)(s_p[u] + i * SP + 32 * jj + 16 * c + 4 * q4) = y;
         }
       }
     }
@@ -449,101 +448,36 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
         for (int e = 0; e < 8; e++) odd = odd || vf[j][e] - vf[j][e] != 0.f;
     }
     odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-    if (OUT) {
+    // the state's part of the outputs, before the state moves on
+    v4f a[C / 16];
+    float xs[4];  // 2^x of the accumulators' columns 4 q4 + r
+    if constexpr (OUT) {
       FV sf[DKT];
-      float xs[4];  // 2^x of the accumulators' columns 4 q4 + r
-      if (some) {
-        float dn = 1.f;
-        if (F16) {
-          float m = 0.f;
+      float dn = 1.f;
+      if (F16) {
+        float m = 0.f;
 #pragma unroll
-          for (int t = 0; t < 2 * DKT; t++)
+        for (int t = 0; t < 2 * DKT; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(S[t][r]));
-          m = fmaxf(m, __shfl_xor(m, 16));
-          m = fmaxf(m, __shfl_xor(m, 32));
-          const int x = scale_exp(m);
-          const float up = ldexpf(1.f, x + ux);
-          dn = ldexpf(1.f, -x);
+          for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(S[t][r]));
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const int x = scale_exp(m);
+        const float up = ldexpf(1.f, x + ux);
+        dn = ldexpf(1.f, -x);
 #pragma unroll
-          for (int r = 0; r < 4; r++) xs[r] = __shfl(up, 4 * q4 + r);
-        }
-#pragma unroll
-        for (int d = 0; d < DKT; d++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) sf[d][e] = (T)(F16 ? S[2 * d + e / 4][e % 4] * dn : S[2 * d + e / 4][e % 4]);
+        for (int r = 0; r < 4; r++) xs[r] = __shfl(up, 4 * q4 + r);
       }
-      FV vz[C / 32];
 #pragma unroll
-      for (int j = 0; j < C / 32; j++) {
-        vz[j] = vf[j];
-        if (odd)
+      for (int d = 0; d < DKT; d++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) vz[j][e] = vf[j][e] - vf[j][e] == (T)0.f ? vf[j][e] : (T)0.f;
-      }
-      __syncthreads();
-      v4f a[C / 16];
+        for (int e = 0; e < 8; e++) sf[d][e] = (T)(F16 ? S[2 * d + e / 4][e % 4] * dn : S[2 * d + e / 4][e % 4]);
 #pragma unroll
       for (int ib = 0; ib < C / 16; ib++) a[ib] = (v4f){0.f, 0.f, 0.f, 0.f};
-      if (some) {
 #pragma unroll
-        for (int d = 0; d < DKT; d++)
+      for (int d = 0; d < DKT; d++)
 #pragma unroll
-          for (int ib = 0; ib < C / 16; ib++) a[ib] = mma(sf[d], row44<T>(s_q + (16 * ib + lr) * SQ + 32 * d + 4 * q4), a[ib]);
-      }
-#pragma unroll
-      for (int ib = 0; ib < C / 16; ib++) {  // each step of 32 columns in its own unit
-        const int i = 16 * ib + lr, x0 = F16 ? s_x[0][i] : 0, x1 = F16 && ib >= 2 ? s_x[1][i] : 0;
-        const float ec = F16 ? ldexpf(s_e[u][i], -x0) : s_e[u][i];
-        if (some)
-#pragma unroll
-          for (int r = 0; r < 4; r++) a[ib][r] *= F16 ? xs[r] * ec : ec;
-        a[ib] = mma(vz[0], row44<T>(s_p + i * SP + 4 * q4), a[ib]);
-        if constexpr (C == 64) {
-          if (ib >= 2) {
-            if (F16)
-#pragma unroll
-              for (int r = 0; r < 4; r++) a[ib][r] = ldexpf(a[ib][r], x0 - x1);
-            a[ib] = mma(vz[1], row44<T>(s_p + i * SP + 32 + 4 * q4), a[ib]);
-          }
-        }
-        const float up = F16 ? ldexpf(p.scale, ib >= 2 ? x1 : x0) : p.scale;
-#pragma unroll
-        for (int r = 0; r < 4; r++) a[ib][r] *= up;
-      }
-      if (odd) {
-#pragma unroll
-        for (int ib = 0; ib < C / 16; ib++) {
-          const int i = 16 * ib + lr;
-#pragma unroll 1
-          for (int j = 0; j <= i; j++) {
-            const float x = p.scale * ldexpf((float)s_p[i * SP + j], F16 ? s_x[j / 32][i] : 0);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const float y = (float)s_v[j * SV + wave * 16 + 4 * q4 + r];
-              if (y - y != 0.f) a[ib][r] += x * y;
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int ib = 0; ib < C / 16; ib++) {
-        const int i = 16 * ib + lr, col = c0 + 4 * q4;
-        if (t0 + i >= rows) continue;
-        T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv + col;
-        FH y;
-#pragma unroll
-        for (int r = 0; r < 4; r++) y[r] = (T)a[ib][r];
-        if (V) {
-          if (col < p.dv) *(FH *)o = y;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-            if (col + r < p.dv) o[r] = y[r];
-        }
-      }
-    } else {
-      __syncthreads();
+        for (int ib = 0; ib < C / 16; ib++) a[ib] = mma(sf[d], row44<T>(s_q + (16 * ib + lr) * SQ + 32 * d + 4 * q4), a[ib]);
     }
     // the state's update
     FV hi[C / 32], lo[C / 32];
@@ -581,17 +515,84 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
       FV kf[C / 32];
 #pragma unroll
       for (int j = 0; j < C / 32; j++) kf[j] = col44(s_k + 32 * j * SK + 16 * t, SK, lane);
-      if (some)
 #pragma unroll
-        for (int r = 0; r < 4; r++) S[t][r] *= dec;
+      for (int r = 0; r < 4; r++) S[t][r] *= dec;
       if (F16)
 #pragma unroll
         for (int j = 0; j < C / 32; j++) S[t] = mma(kf[j], lo[j], S[t]);
 #pragma unroll
       for (int j = 0; j < C / 32; j++) S[t] = mma(kf[j], hi[j], S[t]);
     }
-    some = true;
-    __syncthreads();
+    __syncthreads();  // the scores are there, and this chunk's q, k and v are free
+    if constexpr (OUT) {
+      if (odd) {  // v without what is not finite, which the rows that see it get below
+#pragma unroll
+        for (int j = 0; j < C / 32; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const T y = vf[j][e];
+            vf[j][e] = y - y == (T)0.f ? y : (T)0.f;
+            hi[j][e] = y - y == (T)0.f ? (T)0.f : y;
+          }
+      }
+#pragma unroll
+      for (int ib = 0; ib < C / 16; ib++) {  // each step of 32 columns in its own unit
+        const int i = 16 * ib + lr, x0 = F16 ? s_x[u][0][i] : 0, x1 = F16 && ib >= 2 ? s_x[u][1][i] : 0;
+        const float ec = F16 ? ldexpf(s_e[u][i], -x0) : s_e[u][i];
+#pragma unroll
+        for (int r = 0; r < 4; r++) a[ib][r] *= F16 ? xs[r] * ec : ec;
+        a[ib] = mma(vf[0], row44<T>(s_p[u] + i * SP + 4 * q4), a[ib]);
+        if constexpr (C == 64) {
+          if (ib >= 2) {
+            if (F16)
+#pragma unroll
+              for (int r = 0; r < 4; r++) a[ib][r] = ldexpf(a[ib][r], x0 - x1);
+            a[ib] = mma(vf[1], row44<T>(s_p[u] + i * SP + 32 + 4 * q4), a[ib]);
+          }
+        }
+        const float up = F16 ? ldexpf(p.scale, ib >= 2 ? x1 : x0) : p.scale;
+#pragma unroll
+        for (int r = 0; r < 4; r++) a[ib][r] *= up;
+      }
+      if (odd) {
+#pragma unroll
+        for (int j = 0; j < C / 32; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+#pragma unroll 1
+            for (int q = 0; q < 4; q++) {
+              const int jr = 32 * j + 4 * q + e + (e < 4 ? 0 : 12);
+              float y[4];
+#pragma unroll
+              for (int r = 0; r < 4; r++) y[r] = __shfl((float)hi[j][e], 16 * q + 4 * q4 + r);
+#pragma unroll
+              for (int ib = 2 * j; ib < C / 16; ib++) {
+                const int i = 16 * ib + lr;
+                if (jr > i) continue;
+                const float x = p.scale * ldexpf((float)s_p[u][i * SP + jr], F16 ? s_x[u][j][i] : 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                  if (y[r] != 0.f) a[ib][r] += x * y[r];
+              }
+            }
+      }
+#pragma unroll
+      for (int ib = 0; ib < C / 16; ib++) {
+        const int i = 16 * ib + lr, col = c0 + 4 * q4;
+        if (t0 + i >= rows) continue;
+        T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv + col;
+        FH y;
+#pragma unroll
+        for (int r = 0; r < 4; r++) y[r] = (T)a[ib][r];
+        if (V) {
+          if (col < p.dv) *(FH *)o = y;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (col + r < p.dv) o[r] = y[r];
+        }
+      }
+    }
   }
   if (F16) {
     const float up = ldexpf(1.f, ux);
