@@ -488,16 +488,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    constexpr int LPR = 2 * TN, RPP = 64 / LPR;  // lanes to a row, rows a pass
+    // eight channels a lane where rows are aligned, else one: 64 lanes side by side along the row either way
+    constexpr int VC = VO ? 8 : 1, LPR = 16 * TN / VC;  // lanes to a row
 #pragma unroll
-    for (int h = 0; h < 16; h += RPP) {
-      const int m = h + lane / LPR, c = lane % LPR * 8, n = n0 + wn + c;
+    for (int h = 0; h < 16 * LPR; h += 64) {
+      const int m = (h + lane) / LPR, c = (h + lane) % LPR * VC, n = n0 + wn + c;
       const long long r = rb + m;
       if (m >= 16 || r >= p.rows || n >= p.N) continue;
       const float *y = xch + m * XS + c;
       uint16_t *o = e.out + lora_row(p, e.line, r, e.out_ws, e.ldo) + n;
       const uint16_t *rs = e.res ? e.res + lora_row(p, e.line, r, e.res_ws, e.ldr) + n : nullptr;
-      if (VO) {
+      if constexpr (VO) {
         v8h z = {};
         if (rs) z = *(const v8h *)rs;
         v8h t;
@@ -505,9 +506,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
         for (int k = 0; k < 8; k++) t[k] = (h16)(rs ? y[k] + (float)z[k] : y[k]);
         *(v8h *)o = t;
       } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-          if (n + k < p.N) o[k] = hbits((h16)(rs ? y[k] + (float)hfrom(rs[k]) : y[k]));
+        *o = hbits((h16)(rs ? *y + (float)hfrom(*rs) : *y));
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
