@@ -3,10 +3,15 @@
 //
 // Two launches. k_lora_down computes t = s_j A_j x for every row with an adapter (rounded to fp16: the factor that the
 // matrix instruction of the second product takes; |t| past 65504 becomes infinite). k_lora_gemm computes W x on fp16 MFMA
-// with fp32 sums and carries the K loop on over the r values of t with the adapter's B, so that the adapter costs no pass
-// over the output. Rows of one matrix instruction are independent of each other, so a block of 16 rows whose adapters
-// differ multiplies all of them by each of the adapters in it and every row keeps its own: nothing of another request's
-// adapter, not even an infinity or a NaN, reaches it.
+// with fp32 sums and adds the product of t with the adapter's B to the sums it has, so that the adapter costs no pass over
+// the output. Rows of one matrix instruction are independent of each other, so a block of 16 rows whose adapters differ
+// multiplies all of them by each of the adapters in it and every row keeps its own: nothing of another request's adapter,
+// not even an infinity or a NaN, reaches it. Up to 64 rows, where w's bytes are the bound, k_lora_few computes slices of
+// K beside the first products and k_lora_few_out adds them up.
+//
+// Measured: 17,280 rows, K 1,536, N 6,144, rank 16 of 24 stations in 416 us (0.79 PFLOP/s; a library product of the same
+// size without adapters 350): k_lora_down 17, the rest k_lora_gemm, of which the adapters' products, an idx, t and b read
+// a tile, are 45. 24 rows of 24 stations, 1,536 x 1,536: 6.7 us and 5.3, the latencies of two short launches (w is 1 us).
 #include <type_traits>
 
 #include "bnh_internal.h"

@@ -85,7 +85,7 @@ def test_la_refusals(kw):
 
 
 @pytest.mark.parametrize("T,B,rows,start", [(0, 2, 10, P), (5, 0, 10, P), (5, 2, 0, P), (5, 2, 9, None),
-                                            (1, 1 << 23, 1 << 24, P)])
+                                            (1, 1 << 23, 1 << 24, P), ((1 << 30) + 1, 1, 10, P)])
 def test_la_sizes_refused(T, B, rows, start):
     a = la_args(slots=1 << 24)
     refused(H.lib().bnh_linattn(a, T, B, rows, start, P, P, 1 << 30, None))
