@@ -357,6 +357,25 @@ def test_lora_requests_apart(hip, M):
     assert not np.isfinite(got[~fine]).any()
 
 
+@pytest.mark.parametrize("M,B,N,K,r", [(41, 101, 3080, 136, 16), (1, 4100, 3080, 40, 24), (700, 6, 3080, 64, 40),
+                                       (41, 51, 2048, 136, 16), (41, 51, 2048, 200, 12), (41, 51, 2049, 130, 12),
+                                       (1, 2080, 2048, 130, 33), (700, 3, 2056, 32, 8)])
+def test_lora_large_tiles(hip, M, B, N, K, r):
+    """Outputs enough for each of the larger tiles, whole and ragged, with rows of several adapters in a tile, one of them
+    not finite."""
+    def edit(c):
+        c.b[2, N // 3, 1] = np.nan
+
+    say(f"lora large M {M} B {B} N {N} K {K} r {r}")
+    c = LoraCase(hip, B, M, N, K, r, 9, act=M % 3 % 2, res=M == 41, seed=N + K, edit=edit, idx=(np.arange(B) + 2) % 10)
+    with np.errstate(all="ignore"):
+        want, err = R.lora(c.x, c.w, c.bias, c.a, c.b, c.scale, c.idx, c.act, c.res)
+    got = c.run()
+    fine = np.isfinite(want)
+    assert not fine.all() and not np.isfinite(got[~fine]).any()
+    near(got[fine], want[fine], err[fine], "large", True)
+
+
 def test_lora_residual_in_place(hip):
     for M, N in ((1, 136), (70, 136), (70, 61)):
         say(f"lora in place M {M} N {N}")
@@ -498,6 +517,16 @@ def test_la_dims(hip, f16, dk, dv, T):
     c = LaCase(hip, [T, max(1, T - 3)], 2, 2, 1, 2, dk, dv, f16, seed=dk + dv)
     c.run()
     c.check("dims")
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 128), (128, 128), (100, 77), (256, 136)])
+def test_la_pieces(hip, f16, dk, dv):
+    """Long sequences in pieces that are joined, ends inside and at the end of pieces, with a short one beside them."""
+    say(f"la pieces dk {dk} dv {dv} f16 {f16}")
+    c = LaCase(hip, [1024, 700, 5, 0, 513], 2, 2, 2, 2, dk, dv, f16, gscale=0.1, seed=dk)
+    c.run()
+    c.check("pieces")
 
 
 @pytest.mark.parametrize("hq,hk,hv", [(12, 12, 12), (1, 1, 12), (6, 3, 4), (2, 12, 1)])

@@ -104,3 +104,50 @@ def test_plans_refused(hip):
             net.plan(lens, stations)
     with pytest.raises(ValueError):
         contextnet.ContextNet(dim=65, heads=2)
+
+
+def test_captured_in_a_graph(hip):
+    """A live call captured once and replayed between eager calls and synchronisations gives each time what the eager call
+    gives from the same state and rows."""
+    from bnneon import contextnet
+    hip.lib()
+    rt = ctypes.CDLL("libamdhip64.so.7")  # the runtime that the library has loaded
+    vp = ctypes.c_void_p
+
+    def ok(rc):
+        assert rc == 0, rc
+
+    net = contextnet.ContextNet(dim=128, heads=2, layers=2, stations=5, rank=8, seed=7)
+    rng = np.random.default_rng(8)
+    p = net.plan([1] * 5, range(5))
+    rows = [rng.standard_normal((5, net.dim)).astype(np.float32) for _ in range(4)]
+    want = []
+    for x in rows:
+        p["x"].upload(x)
+        net.run(p)
+        hip.sync()
+        want.append((p["x"].numpy(), p["n"].numpy()))
+    last = [s.numpy() for s in net.state]
+    net.reset()
+    stream, graph, call = hip.lib().bnh_stream_new(), vp(), vp()
+    ok(rt.hipStreamBeginCapture(vp(stream), 0))
+    net.run(p, stream)
+    ok(rt.hipStreamEndCapture(vp(stream), ctypes.byref(graph)))
+    ok(rt.hipGraphInstantiate(ctypes.byref(call), graph, None, None, ctypes.c_size_t(0)))
+    other = net.plan([3], [0])
+    for x, (wx, wn) in zip(rows, want):
+        p["x"].upload(x)
+        ok(rt.hipGraphLaunch(call, vp(stream)))
+        hip.sync(stream)
+        assert np.array_equal(p["x"].numpy(), wx) and np.array_equal(p["n"].numpy(), wn)
+        kept = [z.numpy() for z in net.state]
+        other["x"].upload(x[:3])
+        net.run(other)                               # eager work between the replays
+        hip.sync()
+        for z, k in zip(net.state, kept):
+            z.upload(k)
+    for z, k in zip(net.state, last):
+        assert np.array_equal(z.numpy(), k)
+    ok(rt.hipGraphExecDestroy(call))
+    ok(rt.hipGraphDestroy(graph))
+    hip.check(hip.lib().bnh_stream_free(stream))
