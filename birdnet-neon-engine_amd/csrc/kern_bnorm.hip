@@ -3,7 +3,7 @@
 // post and pre an RMS norm u / sqrt(mean(u^2) + eps) w + b or a layer norm (u - mean) / sqrt(var + eps) w + b.
 //
 // Bound by HBM: f, gate and x are read once and y and n written once, about 20 operations a value. A row lives in the
-// registers of the WPR waves that share it (E values a lane), so that the two statistics and the second pass of the
+// registers of the 16 to 1,024 threads that share it (8 or 16 values each), so that the two statistics and the second pass of the
 // variance read nothing again; the layer norm's variance is the sum of squares about the mean already known, not a
 // difference of sums. Few values a lane and more waves to a row keep more loads in flight: 17,280 rows of 1,536 in fp16
 // take 52.5 us (265 MB, 5.05 TB/s, what a copy reaches) with four waves a row and 8 values a lane, 72 with one wave and 32
@@ -50,33 +50,32 @@ __device__ __forceinline__ void st(T *p, const float *v) {
 // (z >> 0) or where the whole is tiny (z << 0, below 1e-6 relative for |z| < 10)
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
-// the sum over the lanes of the WPR waves of a row, the same in every lane; s: WPR floats of LDS, free on entry
-template <int WPR>
+// the sum over the T threads of a row, the same in every one; s: a float of LDS a wave, free on entry
+template <int T>
 __device__ __forceinline__ float row_sum(float v, float *s) {
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  if constexpr (WPR > 1) {
+  for (int d = 1; d < T && d < 64; d *= 2) v += __shfl_xor(v, d);
+  if constexpr (T > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     v = s[0];
 #pragma unroll
-    for (int w = 1; w < WPR; w++) v += s[w];
+    for (int w = 1; w < T / 64; w++) v += s[w];
   }
   return v;
 }
 
-// u's norm in place: NV chunks of VEC values a lane, chunk i at column (i T + t) VEC (t the thread within the row, T
-// threads), inside the row where below C. Values past C are zero on entry and never stored.
-template <int WPR, int VEC, int NV>
+// u's norm in place: NV chunks of VEC values a lane, chunk i at column (i T + t) VEC (t the thread within the row), inside
+// the row where below C. Values past C are zero on entry and never stored.
+template <int T, int VEC, int NV>
 __device__ __forceinline__ void norm(float (&u)[NV * VEC], int kind, float eps, const float *w, const float *b, int C,
                                      float rC, int t, float *s) {
-  constexpr int T = 64 * WPR;
   if (kind == 2) {
     float a = 0.f;
 #pragma unroll
     for (int i = 0; i < NV * VEC; i++) a += u[i];
-    const float mean = row_sum<WPR>(a, s) * rC;
+    const float mean = row_sum<T>(a, s) * rC;
 #pragma unroll
     for (int i = 0; i < NV; i++)
       if ((i * T + t) * VEC < C)
@@ -86,7 +85,7 @@ __device__ __forceinline__ void norm(float (&u)[NV * VEC], int kind, float eps, 
   float a = 0.f;
 #pragma unroll
   for (int i = 0; i < NV * VEC; i++) a = __builtin_fmaf(u[i], u[i], a);
-  const float r = rsqrtf(__builtin_fmaf(row_sum<WPR>(a, s), rC, eps));
+  const float r = rsqrtf(__builtin_fmaf(row_sum<T>(a, s), rC, eps));
 #pragma unroll
   for (int i = 0; i < NV; i++) {
     const int c = (i * T + t) * VEC;
@@ -107,15 +106,15 @@ __device__ __forceinline__ void norm(float (&u)[NV * VEC], int kind, float eps, 
   }
 }
 
-// A block of max(4, WPR) waves; WPR of them to a row.
-template <typename TF, typename TX, int WPR, int VEC, int NV>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_block_norm(NormDev p, int M, double rM, int C, float rC,
+// T threads to a row, a block of 256 or T
+template <typename TF, typename TX, int T, int VEC, int NV>
+__global__ __launch_bounds__(T > 256 ? T : 256) void k_block_norm(NormDev p, int M, double rM, int C, float rC,
                                                                       int rows) {
-  constexpr int T = 64 * WPR, RPB = WPR == 1 ? 4 : 1;  // threads to a row, rows to a block
-  __shared__ float s[WPR];
+  constexpr int RPB = T < 256 ? 256 / T : 1;  // rows to a block
+  __shared__ float s[T > 64 ? T / 64 : 1];
   const int t = threadIdx.x % T;
   const int row = (int)blockIdx.x * RPB + (int)threadIdx.x / T;
-  if (WPR == 1 && row >= rows) return;  // whole waves, and no barrier in this form
+  if (T <= 64 && row >= rows) return;  // all threads of a row, and no barrier in these forms
   const int w = bnh_div(row, M, rM), m = row - w * M;
   float u[NV * VEC], g[NV * VEC], y[NV * VEC];
   const TF *f = p.f ? (const TF *)p.f + w * p.f_ws + (long long)m * p.ldf : nullptr;
@@ -132,7 +131,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_block_norm(NormDev p
     if (x) ld<TX, VEC>(x + c, y + i * VEC);
   }
   if (f) {
-    if (p.post) norm<WPR, VEC, NV>(u, p.post, p.post_eps, p.post_w, p.post_b, C, rC, t, s);
+    if (p.post) norm<T, VEC, NV>(u, p.post, p.post_eps, p.post_w, p.post_b, C, rC, t, s);
     if (gate && p.act) {
 #pragma unroll
       for (int i = 0; i < NV * VEC; i++) {
@@ -160,7 +159,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_block_norm(NormDev p
       if ((i * T + t) * VEC < C) st<TX, VEC>(o + (i * T + t) * VEC, y + i * VEC);
   }
   if (p.n) {
-    if (p.pre) norm<WPR, VEC, NV>(y, p.pre, p.pre_eps, p.pre_w, p.pre_b, C, rC, t, s);
+    if (p.pre) norm<T, VEC, NV>(y, p.pre, p.pre_eps, p.pre_w, p.pre_b, C, rC, t, s);
     TF *o = (TF *)p.n + w * p.n_ws + (long long)m * p.ldn;
 #pragma unroll
     for (int i = 0; i < NV; i++)
@@ -173,19 +172,23 @@ int run(const NormDev &d, int M, int C, int B, hipStream_t s) {
   const int rows = M * B;
   const double rM = 1.0 / M;
   const float rC = 1.f / (float)C;
-#define GO(WPR, E)                                                                                                      \
+#define GO(T, E)                                                                                                        \
   do {                                                                                                                  \
-    hipLaunchKernelGGL((k_block_norm<TF, TX, WPR, VEC, (E) / VEC>),                                                     \
-                       dim3((unsigned)bnh_ceil_div(rows, WPR == 1 ? 4 : 1)), dim3(WPR == 1 ? 256 : 64 * WPR), 0, s, d,  \
-                       M, rM, C, rC, rows);                                                                             \
+    hipLaunchKernelGGL((k_block_norm<TF, TX, T, VEC, (E) / VEC>), dim3((unsigned)bnh_ceil_div(rows, T < 256 ? 256 / T : 1)), \
+                       dim3(T < 256 ? 256 : T), 0, s, d, M, rM, C, rC, rows);                                           \
     BNH_HIP(hipGetLastError());                                                                                         \
     return 0;                                                                                                           \
   } while (0)
-  if (C <= 512) GO(1, 8);
-  if (C <= 2048) GO(4, 8);
-  if (C <= 4096) GO(4, 16);
-  if (C <= 8192) GO(16, 8);
-  GO(16, 16);
+  // 20 M values with 8 or 16 a lane: C 64 73 us by 16 threads a row and 212 by 64; C 512 55 by 64 and 100 by 256; C 768 68
+  // by 64 (16 values) and 80 by 256 (8); C 1,536 52 by 256 and 72 by 64 (32 values); C 4,096 62 by 256 and 69 by 1,024; C
+  // 8,192 58 by 1,024 and 75 by 256 (32 values)
+  if (C <= 128) GO(16, 8);
+  if (C <= 512) GO(64, 8);
+  if (C <= 1024) GO(64, 16);
+  if (C <= 2048) GO(256, 8);
+  if (C <= 4096) GO(256, 16);
+  if (C <= 8192) GO(1024, 8);
+  GO(1024, 16);
 #undef GO
 }
 

@@ -536,7 +536,9 @@ int lora_tiles(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipS
   BNH_HIP(hipGetLastError());
   return 0;
 }
-constexpr long long few = 64;  // rows up to which w's bytes bound the product
+// Rows up to which w's bytes bound the product: 32 rows, 1,536 x 1,536 12.8 us and 25.8 on the tiles; 64 rows, 1,536 x 6,144
+// 19.9 and 26.2
+constexpr long long few = 64;
 // slices of K of the few-row form: two blocks a compute unit, and a step of 32 a wave at least
 long long few_slices(int N, int K) {
   const long long want = bnh_ceil_div(512, bnh_ceil_div(N, 32)), most = bnh_ceil_div(K, 128);
