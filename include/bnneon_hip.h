@@ -512,8 +512,8 @@ typedef struct {
   const int32_t *slot;
 } bnh_la;
 /* B sequences of at most T rows among `rows` rows: sequence i has the len[i] rows from start[i] (int32 [B] on the device;
- * NULL: T rows each, from i T), cut to T and to [0, rows); one of no rows leaves its state as it is. Sequences share no
- * rows. T = 1 (a live station's new window) runs the recurrence, long sequences a chunked form of it with matrix products.
+ * NULL: T rows each, from i T), cut to T and to [0, rows), and none from a start outside; one of no rows leaves its state as it is. Sequences share no
+ * rows. T up to 8 (1: a live station's new window) runs the recurrence, more rows a chunked form of it with matrix products.
  * work: device scratch of at least bnh_linattn_work_bytes bytes, 16-byte aligned (0 bytes for some shapes: NULL is
  * allowed then). */
 size_t bnh_linattn_work_bytes(const bnh_la *p, int T, int B);
