@@ -250,7 +250,8 @@ __device__ __forceinline__ uint4 row16(const T *p, int c, int cols) {
 
 // One piece of one sequence by NW waves, 16 of the state's columns each. OUT: the outputs, from the state before the piece,
 // and s1 from the sequence's last; else the state that every piece but the last adds (the first one's includes s0), into
-// part, and its whole decay.
+// part, and its whole decay. s1 may lie over s0, and the output launch's blocks run in any order: the launch before it keeps
+// the state before the first piece in part's last place, and a first piece that is not also the last starts from there.
 template <typename T, int DKT, int NW, int C, bool V, bool OUT>
 __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc, int pcr, float *part, float *pdec) {
   constexpr bool F16 = sizeof(T) == 2;
@@ -276,15 +277,16 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
   if (OUT ? pc > 0 && r0 >= n : r0 + pcr >= n) return;  // no such piece, or a last one, whose state nobody takes
   const int rows = n - r0 < pcr ? n - r0 : pcr;         // of this piece; 0: only a state to copy
   const int c0 = sl * DV + wave * 16;                   // this wave's columns
-  const long long pst = ((((long long)b * p.H + h) * nsl + sl) * (npc - 1)) * (KD * DV);  // this state's pieces
+  const long long pst = ((((long long)b * p.H + h) * nsl + sl) * npc) * (KD * DV);  // this state's pieces
   const long long at = ((long long)slot * p.H + h) * p.dk * p.dv;
 
   v4f S[2 * DKT];     // times 2^ux: rows 16 t + 4 q4 + r, column c0 + lr
   int ux = 0;
 #pragma unroll
   for (int t = 0; t < 2 * DKT; t++) S[t] = (v4f){0.f, 0.f, 0.f, 0.f};
-  if (OUT && pc > 0) {
-    const float *w = part + pst + (long long)(pc - 1) * (KD * DV) + wave * (KD * 16) + 4 * lane;
+  const bool keep = p.s0 && p.s1 && slot >= 0 && n > pcr;  // another block than the first piece's stores s1
+  if (OUT && (pc > 0 || keep)) {
+    const float *w = part + pst + (long long)(pc > 0 ? pc - 1 : npc - 1) * (KD * DV) + wave * (KD * 16) + 4 * lane;
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++) S[t] = *(const v4f *)(w + 256 * t);
   } else if (pc == 0 && p.s0 && slot >= 0) {
@@ -295,6 +297,11 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
         const int kk = 16 * t + 4 * q4 + r, col = c0 + lr;
         if (kk < p.dk && col < p.dv) S[t][r] = p.s0[at + (long long)kk * p.dv + col];
       }
+  }
+  if (!OUT && keep && pc == 0) {
+    float *w = part + pst + (long long)(npc - 1) * (KD * DV) + wave * (KD * 16) + 4 * lane;
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++) *(v4f *)(w + 256 * t) = S[t];
   }
   if (OUT) {  // the blocks right of the diagonal that a step of 32 reads
     for (int i = tid; i < C / 32 * 256; i += NT)
@@ -649,7 +656,7 @@ __global__ __launch_bounds__(256) void k_la_scan(LaDev p, int npc, int pcr, int 
   const int np = (n + pcr - 1) / pcr - 1;  // pieces whose state a later one takes
   const int i = (int)(blockIdx.x * 256 + threadIdx.x);
   if (i >= quads || np < 2) return;
-  float4 *w = (float4 *)(part + (long long)st * (npc - 1) * 4 * quads) + i;
+  float4 *w = (float4 *)(part + (long long)st * npc * 4 * quads) + i;
   const float *d = pdec + (long long)st * (npc - 1);
   float4 s = w[0];
   for (int k = 1; k < np; k++) {
@@ -692,12 +699,13 @@ Plan plan(const bnh_la *p, int T, int B) {
 }
 size_t plan_bytes(const Plan &r) {
   if (r.npc < 2) return 0;
-  return (size_t)(bnh_round_up(4 * r.states * (r.npc - 1) * r.floats, 256) + bnh_round_up(4 * r.states * (r.npc - 1), 256));
+  // what each piece but the last adds and the state before the first, then the pieces' decays
+  return (size_t)(bnh_round_up(4 * r.states * r.npc * r.floats, 256) + bnh_round_up(4 * r.states * (r.npc - 1), 256));
 }
 
 template <typename T, int DKT, int NW, int C, bool V>
 int chunk_run(const LaDev &d, const Plan &r, void *work, hipStream_t s) {
-  float *part = (float *)work, *pdec = part ? (float *)((char *)work + bnh_round_up(4 * r.states * (r.npc - 1) * r.floats, 256)) : nullptr;
+  float *part = (float *)work, *pdec = part ? (float *)((char *)work + bnh_round_up(4 * r.states * r.npc * r.floats, 256)) : nullptr;
   const dim3 block(64 * NW);
   if (r.npc > 1) {
     hipLaunchKernelGGL((k_la_chunk<T, DKT, NW, C, V, false>), dim3((unsigned)(r.states * (r.npc - 1))), block, 0, s, d, r.nsl,
