@@ -22,6 +22,10 @@ struct LaDev {
   float scale;
 };
 
+// e^g of this g is 0 in 64 bits too: a row at or below it starts the state anew, whatever it holds (0 times an infinity or a
+// NaN would keep it)
+constexpr float kAnew = -746.f;
+
 // sequence b's first row and its rows, cut to T and to the buffers' rows
 __device__ __forceinline__ int la_rows(const LaDev &p, int b, int *first) {
   const long long s = p.start ? p.start[b] : (long long)b * p.T;
@@ -80,7 +84,13 @@ __global__ __launch_bounds__(256) void k_la_step(LaDev p, int nsl) {
     float v[4], a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = col + j < p.dv ? (float)((const T *)p.v)[r * p.ldv + hv + col + j] : 0.f;
-    const float d = expf(p.g[r * p.ldg + h]);
+    const float g = p.g[r * p.ldg + h], d = expf(g);
+    if (g <= kAnew) {
+#pragma unroll
+      for (int i = 0; i < KR; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[i][j] = 0.f;
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < KR; i++) {
@@ -169,7 +179,9 @@ int step_go(const LaDev &d, int B, bool vs, hipStream_t s) {
 // other, with two waves a SIMD at 219 registers; four waves of 128 registers spill and take 1.5 times as long.
 //
 // A row's v that is not finite would reach earlier rows of its chunk as 0 x inf; it is taken out of the product and added to
-// the rows that see it one by one (a wave that finds none skips this).
+// the rows that see it one by one (a wave that finds none skips this). A row that starts the state anew (e^g is 0) takes
+// what was before it times 0; where the state or a row of such a chunk is not finite, the chunk ends ahead of that row, and
+// the next one begins with it and no state.
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v8f __attribute__((ext_vector_type(8)));
@@ -252,8 +264,11 @@ __device__ __forceinline__ uint4 row16(const T *p, int c, int cols) {
 // and s1 from the sequence's last; else the state that every piece but the last adds (the first one's includes s0), into
 // part, and its whole decay. s1 may lie over s0, and the output launch's blocks run in any order: the launch before it keeps
 // the state before the first piece in part's last place, and a first piece that is not also the last starts from there.
+// fp32 rows of dk up to 64 are held to registers of which two blocks of eight waves fit a compute unit (8 sequences of up to
+// 500 rows, 16 heads of 64 x 97: 73 us, 88 with one).
 template <typename T, int DKT, int NW, int C, bool V, bool OUT>
-__global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc, int pcr, float *part, float *pdec) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k_la_chunk(LaDev p, int nsl, int npc, int pcr,
+                                                                                          float *part, float *pdec) {
   constexpr bool F16 = sizeof(T) == 2;
   constexpr int VE = 16 / sizeof(T), KD = 32 * DKT, DV = 16 * NW, NT = 64 * NW, SQ = KD + VE, SP = C + VE;
   constexpr int SK = KD + (F16 ? 16 : 4), SV = DV + (F16 ? 16 : 4);
@@ -266,6 +281,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
   __shared__ __attribute__((aligned(16))) float s_w[2][64];  // e^{c_C - c_j}
   __shared__ float s_e[2][64], s_d[2], s_m[2];               // e^{c_i}; e^{c_C}; the largest of s_w
   __shared__ int s_x[2][2][64];                              // the scores' scale by step of 32 columns and row
+  __shared__ int s_bad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q4 = lane >> 4;
   unsigned lb = bnh_xcd_block(blockIdx.x, gridDim.x);
   const int sl = (int)(lb % nsl), h = (int)(lb / nsl % p.H);
@@ -362,8 +378,10 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
       *(uint4 *)(s_v + (vr + RV * i) * SV + vc) = vn[i];
     }
   };
-  // c of the chunk from row t0 and what follows from it, by the last wave; rows past the end count as g = 0
-  double ctot = 0;
+  // c of the chunk from row t0 and what follows from it, by the last wave (every wave has g, for the rows that start the state
+  // anew); rows past the end count as g = 0
+  double ctot = 0, cpre = 0;  // with and without the chunk's
+  bool anew = false;          // a row of the piece starts the state anew
   float gn = 0.f;
   auto gload = [&](int t0) {
     gn = 0.f;
@@ -387,20 +405,69 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
       s_w[u][lane] = w;
       if (lane == C - 1) s_d[u] = expf((float)c), s_m[u] = m;
     }
+    cpre = ctot;
     ctot += last;
+  };
+  // The rows to take of the chunk in qn, kn and vn, of which `at` start the state anew: all of it where everything is
+  // finite, else what lies ahead of such a row
+  auto rows_to_new = [&](int t0, int u, uint64_t at) {
+    bool bad = !(gn <= kAnew) && gn - gn != 0.f;
+    auto odd = [&](uint4 x) {
+      T y[VE];
+      __builtin_memcpy(y, &x, 16);
+#pragma unroll
+      for (int e = 0; e < VE; e++) bad = bad || y[e] - y[e] != (T)0.f;
+    };
+#pragma unroll
+    for (int i = 0; i < NK; i++)
+      if (t0 + kr + RK * i < rows && kc < p.dk) odd(kn[i]);
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      if (t0 + vr + RV * i < rows && vc < vcols) odd(vn[i]);
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) bad = bad || S[t][r] - S[t][r] != 0.f;
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    if (bad) s_bad = 1;
+    __syncthreads();
+    if (!s_bad) return C;
+    if (at & 1) {
+#pragma unroll
+      for (int t = 0; t < 2 * DKT; t++) S[t] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+    const uint64_t next = at & ~1ull;
+    const int len = next ? __builtin_ctzll(next) : C;
+#pragma unroll
+    for (int i = 0; i < NK; i++)
+      if (kr + RK * i >= len) kn[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      if (vr + RV * i >= len) vn[i] = make_uint4(0, 0, 0, 0);
+    if (wave == NW - 1) {
+      ctot = at & 1 ? 0 : cpre;
+      if (lane >= len || (lane == 0 && (at & 1))) gn = 0.f;
+      sums(u);
+    }
+    return len;
   };
 
   load(0);
-  if (wave == NW - 1) {
-    gload(0);
-    sums(0);
-  }
-  int u = 0;
-  for (int t0 = 0; t0 < rows; t0 += C, u ^= 1) {
+  gload(0);
+  if (wave == NW - 1) sums(0);
+  int u = 0, end;
+  for (int t0 = 0; t0 < rows; t0 = end, u ^= 1) {
+    const uint64_t at = __builtin_amdgcn_ballot_w64(gn <= kAnew);
+    end = t0 + C;
+    if (at) {
+      anew = true;
+      end = t0 + rows_to_new(t0, u, at);
+    }
     put(t0);
     __syncthreads();
-    load(t0 + C);
-    if (wave == NW - 1) gload(t0 + C);
+    load(end);
+    gload(end);
 
     if constexpr (OUT) {  // scores of 16 rows and 32 columns a unit, a row a lane and four columns in each block of 16
       constexpr int UN = C == 64 ? 6 : 2;
@@ -443,7 +510,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
         }
       }
     }
-    if (wave == NW - 1 && t0 + C < rows) sums(u ^ 1);
+    if (wave == NW - 1 && end < rows) sums(u ^ 1);
     FV vf[C / 32];
 #pragma unroll
     for (int j = 0; j < C / 32; j++) vf[j] = col44(s_v + 32 * j * SV + wave * 16, SV, lane);
@@ -608,7 +675,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
 #pragma unroll
       for (int ib = 0; ib < C / 16; ib++) {
         const int i = 16 * ib + lr, col = c0 + 4 * q4;
-        if (t0 + i >= rows) continue;
+        if (t0 + i >= rows || t0 + i >= end) continue;
         T *o = (T *)p.o + ((long long)first + r0 + t0 + i) * p.ldo + (long long)h * p.dv + col;
         FH y;
 #pragma unroll
@@ -634,7 +701,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
     float *w = part + pst + (long long)pc * (KD * DV) + wave * (KD * 16) + 4 * lane;
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++) *(v4f *)(w + 256 * t) = S[t];
-    if (wave == NW - 1 && lane == 0) pdec[(((long long)b * p.H + h) * nsl + sl) * (npc - 1) + pc] = expf((float)ctot);
+    if (wave == NW - 1 && lane == 0) pdec[(((long long)b * p.H + h) * nsl + sl) * (npc - 1) + pc] = anew ? -1.f : expf((float)ctot);
   } else if (p.s1 && slot >= 0 && r0 + pcr >= n) {
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++)
@@ -647,7 +714,7 @@ __global__ __launch_bounds__(64 * NW) void k_la_chunk(LaDev p, int nsl, int npc,
 }
 
 // The states before each piece from what the pieces add: part[i] <- part[i] + pdec[i] part[i - 1], in order, four values
-// a thread
+// a thread; a pdec below 0 is a piece that starts the state anew
 __global__ __launch_bounds__(256) void k_la_scan(LaDev p, int npc, int pcr, int quads, int nsl, float *part,
                                                  const float *pdec) {
   const int st = (int)(blockIdx.y), b = st / (nsl * p.H);
@@ -662,8 +729,8 @@ __global__ __launch_bounds__(256) void k_la_scan(LaDev p, int npc, int pcr, int 
   for (int k = 1; k < np; k++) {
     const float4 x = w[(long long)k * quads];
     const float y = d[k];
-    s = make_float4(__builtin_fmaf(y, s.x, x.x), __builtin_fmaf(y, s.y, x.y), __builtin_fmaf(y, s.z, x.z),
-                    __builtin_fmaf(y, s.w, x.w));
+    s = y < 0.f ? x : make_float4(__builtin_fmaf(y, s.x, x.x), __builtin_fmaf(y, s.y, x.y), __builtin_fmaf(y, s.z, x.z),
+                                  __builtin_fmaf(y, s.w, x.w));
     w[(long long)k * quads] = s;
   }
 }

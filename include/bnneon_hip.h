@@ -494,7 +494,8 @@ int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const 
  *   S = exp(g_t) S + k_t v_t^T,  o_t = scale q_t^T S
  * with S [dk][dv] from s0 (NULL: zeros) and left in s1 (NULL: not stored; s1 may be s0). Row r of q holds Hq heads of dk
  * at r ldq, k Hk of dk, v Hv of dv, o H of dv, g H log decays (ldg 0: the same for every row); head h reads q head
- * h Hq / H and so on (Hq, Hk, Hv divide H). g may be -inf (the state starts anew), and is meant to be <= 0. States are fp32
+ * h Hq / H and so on (Hq, Hk, Hv divide H). g is meant to be <= 0; a g of -746 or below, whose e^g is 0, -inf among them,
+ * starts the state anew at its row, whatever the state holds, infinities and NaNs too. States are fp32
  * [slots][H][dk][dv]; sequence i's is slot[i] (NULL: i), and a slot outside [0, slots) starts from zeros and stores
  * nothing; no two sequences of a call share one that is stored. dk, dv <= 256. */
 typedef struct {
