@@ -169,9 +169,9 @@ int step_go(const LaDev &d, int B, bool vs, hipStream_t s) {
 //
 // fp16 rows: the factors of a product have to be fp16, its sums are fp32. Scores are scaled row by row and the state
 // column by column by powers of two before they are rounded (their largest to 2^12..2^13), so neither overflows and both
-// keep 11 bits, as the rounded output does. The state itself is not rounded: its update takes v_j e^{c_C - c_j}, scaled
-// by column to 2^14..2^15 (the state's own unit from then on), in two fp16 parts, 22 bits, against the exact k. fp32 rows run
-// on the fp32 MFMA, unscaled and unsplit.
+// keep 11 bits, as the rounded output does. The state itself is not rounded: its update takes v_j e^{c_C - c_j}, the
+// largest of the chunk's by column scaled to 2^14..2^15 (the state's own unit from then on), in two fp16 parts, 22 bits, against
+// the exact k. fp32 rows run on the fp32 MFMA, unscaled and unsplit.
 //
 // 12 heads of 128 x 128 in fp16: 17,280 rows of one sequence 126 us (22 pieces of 13 chunks: what the pieces add 34, the
 // join 9, the outputs 78; 214 MB would take 42), 24 sequences of up to 720 rows 126 us. A chunk takes a block 12,000
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
   __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SQ : 1], s_k[C * SK], s_v[C * SV], s_p[2][OUT ? C * SP : 1];
   __shared__ double s_c[2][64];                              // c_i
   __shared__ __attribute__((aligned(16))) float s_w[2][64];  // e^{c_C - c_j}
-  __shared__ float s_e[2][64], s_d[2], s_m[2];               // e^{c_i}; e^{c_C}; the largest of s_w
+  __shared__ float s_e[2][64], s_d[2];                       // e^{c_i}; e^{c_C}
   __shared__ int s_x[2][2][64];                              // the scores' scale by step of 32 columns and row
   __shared__ int s_bad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q4 = lane >> 4;
@@ -396,14 +396,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     }
     const double last = __shfl(c, C - 1);
     const float w = expf((float)(last - c));
-    float m = lane < C ? w : 0.f;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
     if (lane < C) {
       s_c[u][lane] = c;
       s_e[u][lane] = expf((float)c);
       s_w[u][lane] = w;
-      if (lane == C - 1) s_d[u] = expf((float)c), s_m[u] = m;
+      if (lane == C - 1) s_d[u] = expf((float)c);
     }
     cpre = ctot;
     ctot += last;
@@ -514,8 +511,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     FV vf[C / 32];
 #pragma unroll
     for (int j = 0; j < C / 32; j++) vf[j] = col44(s_v + 32 * j * SV + wave * 16, SV, lane);
-    // the largest |v| of the lane's, and whether a value of v is not finite
-    float vm = 0.f;
+    // whether a value of v is not finite
     bool odd = false;
     if constexpr (F16) {
       typedef unsigned short u2 __attribute__((ext_vector_type(2)));
@@ -527,9 +523,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
           const u2 x = {(unsigned short)(hbits(vf[j][e]) & 0x7fff), (unsigned short)(hbits(vf[j][e + 1]) & 0x7fff)};
           m = __builtin_elementwise_max(m, x);
         }
-      const unsigned short mm = m[0] > m[1] ? m[0] : m[1];
-      odd = mm >= 0x7c00;
-      vm = (float)hfrom(mm);
+      odd = m[0] >= 0x7c00 || m[1] >= 0x7c00;
     } else {
 #pragma unroll
       for (int j = 0; j < C / 32; j++)
@@ -570,29 +564,36 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     }
     // the state's update
     FV hi[C / 32], lo[C / 32];
-    float dec = s_d[u], dn = 1.f;
-    if (F16) {
-      float m = fmaxf(vm, __shfl_xor(vm, 16));
-      m = fmaxf(m, __shfl_xor(m, 32)) * s_m[u];
+    float dec = s_d[u];
+    if constexpr (F16) {
+      float y[C / 32][8], m = 0.f;  // v_j e^{c_C - c_j}; the largest of the column
+#pragma unroll
+      for (int j = 0; j < C / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          y[j][e] = __builtin_fmaf((float)vf[j][e], s_w[u][32 * j + 4 * q4 + e + (e < 4 ? 0 : 12)], 0.f);
+          m = fmaxf(m, fabsf(y[j][e]));
+        }
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
       const int e = (int)(__float_as_uint(m) >> 23 & 255) - 127;
       const int x = m == 0.f ? ux : e > 127 ? 0 : e - 14;  // the largest to 2^14..2^15
-      dn = ldexpf(1.f, -x);
       dec = ldexpf(dec, ux - x);
       ux = x;
-    }
 #pragma unroll
-    for (int j = 0; j < C / 32; j++)
+      for (int j = 0; j < C / 32; j++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float w = s_w[u][32 * j + 4 * q4 + e + (e < 4 ? 0 : 12)];
-        if (F16) {
-          const float y = __builtin_fmaf((float)vf[j][e], w * dn, 0.f);
-          hi[j][e] = (T)y;
-          lo[j][e] = (T)(y - (float)hi[j][e]);
-        } else {
-          hi[j][e] = (T)((float)vf[j][e] * w);
+        for (int e = 0; e < 8; e++) {
+          const float z = ldexpf(y[j][e], -x);
+          hi[j][e] = (T)z;
+          lo[j][e] = (T)(z - (float)hi[j][e]);
         }
-      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) hi[j][e] = (T)((float)vf[j][e] * s_w[u][32 * j + 4 * q4 + e + (e < 4 ? 0 : 12)]);
+    }
     if (F16 && odd) {  // an infinity has no second part
 #pragma unroll
       for (int j = 0; j < C / 32; j++)

@@ -1,0 +1,27 @@
+"""Linear attention over fp16 rows whose values, decays and states are far apart in size."""
+import numpy as np
+import pytest
+
+from test_gpu_context import LaCase, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("T,at", [(64, 1), (64, 40), (64, 63), (200, 66), (700, 600)])
+@pytest.mark.parametrize("g", [-40.0, -np.inf])
+@pytest.mark.parametrize("before,after", [(1e3, 1e-3), (1e4, 1e-3), (6e4, 1e-4)])
+def test_large_values_decayed(hip, f16, T, at, g, before, after):
+    """A v that a decay takes away within its chunk does not coarsen the state of what comes after."""
+    def edit(c):
+        v = slice((c.hq + c.hk) * c.dk, None)
+        # to a sixth of `before` and of `after`
+        for rows, size in ((slice(0, at), before), (slice(at, T), after)):
+            c.qkv[rows, v] = (np.clip(c.qkv[rows, v].astype(np.float32), -6, 6) * (size / 6)).astype(c.qkv.dtype)
+        c.g[at] = g
+
+    say(f"la decayed T {T} at {at} g {g} {before} {after} f16 {f16}")
+    c = LaCase(hip, [T], 2, 2, 2, 2, 64, 48, f16, gscale=0.01, s0=False, seed=T + at, edit=edit)
+    c.scale = 1e-3
+    c.run()
+    c.check("decayed")
