@@ -298,6 +298,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
 
   v4f S[2 * DKT];     // times 2^ux: rows 16 t + 4 q4 + r, column c0 + lr
   int ux = 0;
+  float most = 0.f;   // F16: no finite value of the column is larger
 #pragma unroll
   for (int t = 0; t < 2 * DKT; t++) S[t] = (v4f){0.f, 0.f, 0.f, 0.f};
   const bool keep = p.s0 && p.s1 && slot >= 0 && n > pcr;  // another block than the first piece's stores s1
@@ -318,6 +319,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     float *w = part + pst + (long long)(npc - 1) * (KD * DV) + wave * (KD * 16) + 4 * lane;
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++) *(v4f *)(w + 256 * t) = S[t];
+  }
+  if (F16) {
+#pragma unroll
+    for (int t = 0; t < 2 * DKT; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) most = fmaxf(most, S[t][r] - S[t][r] == 0.f ? fabsf(S[t][r]) : 0.f);
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
   }
   if (OUT) {  // the blocks right of the diagonal that a step of 32 reads
     for (int i = tid; i < C / 32 * 256; i += NT)
@@ -576,8 +585,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
         }
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
-      const int e = (int)(__float_as_uint(m) >> 23 & 255) - 127;
-      const int x = m == 0.f ? ux : e > 127 ? 0 : e - 14;  // the largest to 2^14..2^15
+      // k is below 2^16. The state in its unit stays below 2^126, whatever it came with
+      most = __builtin_fmaf(m, 65536.f * C, fmaxf(most * dec, 0.f));
+      const int e = (int)(__float_as_uint(m) >> 23 & 255) - 127, low = (int)(__float_as_uint(most) >> 23 & 255) - 127 - 125;
+      int x = m == 0.f ? ux : e > 127 ? 0 : e - 14;  // the largest to 2^14..2^15
+      x = x > low ? x : low;
       dec = ldexpf(dec, ux - x);
       ux = x;
 #pragma unroll
@@ -633,23 +645,24 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
           }
       }
 #pragma unroll
-      for (int ib = 0; ib < C / 16; ib++) {  // each step of 32 columns in its own unit
-        const int i = 16 * ib + lr, x0 = F16 ? s_x[u][0][i] : 0, x1 = F16 && ib >= 2 ? s_x[u][1][i] : 0;
-        const float ec = F16 ? ldexpf(s_e[u][i], -x0) : s_e[u][i];
+      for (int ib = 0; ib < C / 16; ib++) {  // the state's part and each step of 32 columns have a unit of their own
+        const int i = 16 * ib + lr;
+        const float ec = s_e[u][i];
+        const v4f z = {0.f, 0.f, 0.f, 0.f}, y0 = mma(vf[0], row44<T>(s_p[u] + i * SP + 4 * q4), z);
+        const float u0 = F16 ? ldexpf(1.f, s_x[u][0][i]) : 1.f;
+        if (C == 64 && ib >= 2) {
+          const v4f y1 = mma(vf[C / 32 - 1], row44<T>(s_p[u] + i * SP + 32 + 4 * q4), z);
+          const float u1 = F16 ? ldexpf(1.f, s_x[u][1][i]) : 1.f;
 #pragma unroll
-        for (int r = 0; r < 4; r++) a[ib][r] *= F16 ? xs[r] * ec : ec;
-        a[ib] = mma(vf[0], row44<T>(s_p[u] + i * SP + 4 * q4), a[ib]);
-        if constexpr (C == 64) {
-          if (ib >= 2) {
-            if (F16)
-#pragma unroll
-              for (int r = 0; r < 4; r++) a[ib][r] = ldexpf(a[ib][r], x0 - x1);
-            a[ib] = mma(vf[1], row44<T>(s_p[u] + i * SP + 32 + 4 * q4), a[ib]);
+          for (int r = 0; r < 4; r++) {
+            const float y = F16 ? __builtin_fmaf(y1[r], u1, y0[r] * u0) : y0[r] + y1[r];
+            a[ib][r] = p.scale * __builtin_fmaf(F16 ? a[ib][r] * xs[r] : a[ib][r], ec, y);
           }
-        }
-        const float up = F16 ? ldexpf(p.scale, ib >= 2 ? x1 : x0) : p.scale;
+        } else {
 #pragma unroll
-        for (int r = 0; r < 4; r++) a[ib][r] *= up;
+          for (int r = 0; r < 4; r++)
+            a[ib][r] = p.scale * __builtin_fmaf(F16 ? a[ib][r] * xs[r] : a[ib][r], ec, F16 ? y0[r] * u0 : y0[r]);
+        }
       }
       if (odd) {
 #pragma unroll

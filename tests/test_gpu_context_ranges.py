@@ -25,3 +25,19 @@ def test_large_values_decayed(hip, f16, T, at, g, before, after):
     c.scale = 1e-3
     c.run()
     c.check("decayed")
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("T", [3, 64, 200, 700])
+@pytest.mark.parametrize("state,v", [(1e30, 1e-7), (1e36, 1e-3), (1e-30, 1e4)])
+def test_state_of_another_size(hip, f16, T, state, v):
+    """A state far larger or smaller than what the rows add to it keeps its own size and precision."""
+    def edit(c):
+        c.s0 *= np.float32(state)
+        d = slice((c.hq + c.hk) * c.dk, None)
+        c.qkv[:, d] = (c.qkv[:, d].astype(np.float32) * v).astype(c.qkv.dtype)
+        c.scale = 0.1 / max(state, 1.0)
+
+    say(f"la state {state} v {v} T {T} f16 {f16}")
+    c = LaCase(hip, [T], 2, 2, 2, 2, 64, 48, f16, gscale=1e-3, seed=T, edit=edit)
+    c.run()
+    c.check("state")
