@@ -235,10 +235,10 @@ __device__ __forceinline__ v8f col44(const float *p, int ld, int lane) {
   for (int e = 0; e < 8; e++) r[e] = p[(4 * (lane >> 4) + e + (e < 4 ? 0 : 12)) * ld + (lane & 15)];
   return r;
 }
-// 2^-e that takes a largest value m to 2^12..2^13: 0 and infinities are left as they are, and nothing grows past 2^24
+// 2^-e that takes a largest value m to 2^12..2^13: 0 and infinities are left as they are, and nothing grows past 2^126
 __device__ __forceinline__ int scale_exp(float m) {
   const int e = (int)(__float_as_uint(m) >> 23 & 255) - 127 - 12;
-  return m == 0.f || e > 127 - 12 ? 0 : e < -24 ? -24 : e;
+  return m == 0.f || e > 127 - 12 ? 0 : e < -126 ? -126 : e;
 }
 
 // 16 bytes of a row of `cols` values from its value c, zeros past the end; V: all of them are in or out, 16-byte aligned

@@ -41,3 +41,35 @@ def test_state_of_another_size(hip, f16, T, state, v):
     c = LaCase(hip, [T], 2, 2, 2, 2, 64, 48, f16, gscale=1e-3, seed=T, edit=edit)
     c.run()
     c.check("state")
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("T", [130, 300])
+def test_decayed_state_alone(hip, f16, T):
+    """Outputs of a state that has decayed to 2^-58 with no v since, which the caller's scale brings back into range (those
+    before are infinite in fp16)."""
+    def edit(c):
+        c.qkv[:, (c.hq + c.hk) * c.dk:] = 0
+        c.g[:] = -1e-3
+        c.g[20] = -40.0
+        c.scale = 1e17
+
+    say(f"la decayed state T {T} f16 {f16}")
+    c = LaCase(hip, [T], 2, 2, 2, 2, 64, 48, f16, seed=T, edit=edit)
+    c.run()
+    c.check("decayed state")
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("T", [20, 130])
+def test_small_scores(hip, f16, T):
+    """Scores below 2^-38 of queries and keys of 1e-6, with large values and a scale to match."""
+    def edit(c):
+        d = (c.hq + c.hk) * c.dk
+        c.qkv[:, :d] = (np.sign(c.qkv[:, :d].astype(np.float32)) * 9.5e-7).astype(c.qkv.dtype)
+        c.scale = 1e9
+
+    say(f"la small scores T {T} f16 {f16}")
+    c = LaCase(hip, [T], 2, 2, 2, 2, 16, 48, f16, gscale=0.1, s0=False, seed=T, edit=edit)
+    c.run()
+    c.check("small scores")
