@@ -1,8 +1,9 @@
 // A shared fp16 projection with low-rank adapters of many requests beside it (bnh_pw_lora):
 //   out = act(W x + bias + s_j B_j (A_j x)) (+ res), j the adapter of the row's window.
 //
-// Two launches. k_lora_down computes t = s_j A_j x for every row with an adapter (rounded to fp16: the factor that the
-// matrix instruction of the second product takes; |t| past 65504 becomes infinite). k_lora_gemm computes W x on fp16 MFMA
+// Two launches. k_lora_down computes t = s_j A_j x for every row with an adapter, rounded to fp16: the factor that the
+// matrix instruction of the second product takes. A row's t is scaled by a power of two first (its largest to 2^14..2^15), so
+// that it keeps 11 bits whatever its size; the row's product takes the unit back in fp32. k_lora_gemm computes W x on fp16 MFMA
 // with fp32 sums and adds the product of t with the adapter's B to the sums it has, so that the adapter costs no pass over
 // the output. Rows of one matrix instruction are independent of each other, so a block of 16 rows whose adapters differ
 // multiplies all of them by each of the adapters in it and every row keeps its own: nothing of another request's adapter,
@@ -54,6 +55,7 @@ struct LoraDev {
   const float *bias, *scale;
   const int32_t *idx;
   uint16_t *t;
+  float *u;  // the unit of each row of t
   long long x_ws;
   int lda, ldw, M, N, K, n, r, r32;  // r32: r rounded up to 32, t's row
   bool line;                         // x's windows follow each other: rows lda apart throughout
@@ -112,19 +114,32 @@ __device__ __forceinline__ void lora_down(const LoraDev &p, long long tile, unsi
   __syncthreads();
   if (wave) return;
   const float sc = p.scale ? p.scale[j] : 1.f;
+  v4f most = {0.f, 0.f, 0.f, 0.f};  // of each of the lane's four rows
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const float *q = s + t * 256 + 4 * lane;
     acc[t] += *(const v4f *)q + (*(const v4f *)(q + RT * 256) + *(const v4f *)(q + 2 * RT * 256));
-    const int c = 16 * t + lr;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const int m = 4 * (lane >> 4) + e;
-      const int rid = __shfl(id, m);
-      if (tile * 16 + m < p.rows && rid == j && c < p.r32)
-        p.t[(tile * 16 + m) * p.r32 + c] = c < p.r ? hbits((h16)(sc * acc[t][e])) : 0;
-      if (RT == 1 && tile * 16 + m < p.rows && rid == j) p.t[(tile * 16 + m) * p.r32 + 16 + lr] = 0;
+      acc[t][e] *= sc;
+      if (16 * t + lr < p.r) most[e] = fmaxf(most[e], fabsf(acc[t][e]));
     }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) most[e] = fmaxf(most[e], __shfl_xor(most[e], d));
+    const int m = 4 * (lane >> 4) + e, rid = __shfl(id, m);
+    const long long r = tile * 16 + m;
+    if (r >= p.rows || rid != j) continue;
+    const int x = most[e] == 0.f || most[e] - most[e] != 0.f ? 0 : (int)(__float_as_uint(most[e]) >> 23) - 127 - 14;
+    if (lr == 0) p.u[r] = ldexpf(1.f, x);
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      const int c = 16 * t + lr;
+      if (c < p.r32) p.t[r * p.r32 + c] = c < p.r ? hbits((h16)ldexpf(acc[t][e], -x)) : 0;
+    }
+    if (RT == 1) p.t[r * p.r32 + 16 + lr] = 0;
   }
 }
 template <int RT, bool V>
@@ -236,7 +251,9 @@ __global__ __launch_bounds__(256) void k_lora_few_out(LoraDev p, EpiDev e, int k
         for (int l = 0; l < 8; l++) u[c] = __builtin_fmaf((float)x[l], (float)z[l], u[c]);
       }
     }
-    y += u;
+    const float un = p.u[row];
+#pragma unroll
+    for (int c = 0; c < 4; c++) y[c] = __builtin_fmaf(u[c], un, y[c]);
   }
   uint16_t *o = e.out + w * e.out_ws + (long long)m * e.ldo + n;
   const uint16_t *rs = e.res ? e.res + w * e.res_ws + (long long)m * e.ldr + n : nullptr;
@@ -319,6 +336,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
   for (int j = 0; j < TN; j++)
     bp[j] = p.b + (long long)(n0 + wn + 16 * j + lr < p.N ? n0 + wn + 16 * j + lr : p.N - 1) * p.r + 8 * q4;
   v8h ax[TM], bn[TN];
+  float un[TM];
   uint32_t todo[TM];
   int next = -1;
   auto pick = [&](int k) {  // the next adapter of a row that has not had its own, -1 when all have; its b on the way
@@ -343,6 +361,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
       todo[i] = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && id[i] >= 0);
       const long long row = r0 + wm + 16 * i + lr < p.rows ? r0 + wm + 16 * i + lr : p.rows - 1;
       ax[i] = *(const v8h *)(p.t + row * p.r32 + 8 * q4 + k);
+      un[i] = p.u[row];
     });
     pick(k);
   };
@@ -443,8 +462,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
   __syncthreads();
 
   // The adapters: one of those among the wave's rows a turn, its b read once for all of them while the one before is
-  // multiplied. A tile of 16 rows that all have it adds to its sums directly; of others every row takes the product or
-  // keeps what it has, so that one request's infinities stay its own.
+  // multiplied. Every row takes the product in its unit or keeps what it has, so that one request's infinities stay its own.
   for (int k = 0; k < p.r32; k += 32) {
     if (k || !DMA || full == 0) ahead(k);
     while (next >= 0) {
@@ -455,16 +473,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
       pick(k);
       each<TM>([&](auto tile) {
         constexpr int i = decltype(tile)::value;
-        const uint32_t mine = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && id[i] == a);
-        if (mine == 0xffff) {
-#pragma unroll
-          for (int j = 0; j < TN; j++) acc[j][i] = mma(b[j], ax[i], acc[j][i]);
-        } else if (mine) {
+        if (__builtin_amdgcn_ballot_w64(lane < 16 && id[i] == a)) {
 #pragma unroll
           for (int j = 0; j < TN; j++) {
             const v4f u = mma(b[j], ax[i], (v4f){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int q = 0; q < 4; q++) acc[j][i][q] = id[i] == a ? acc[j][i][q] + u[q] : acc[j][i][q];
+            for (int q = 0; q < 4; q++) acc[j][i][q] = id[i] == a ? __builtin_fmaf(u[q], un[i], acc[j][i][q]) : acc[j][i][q];
           }
         }
       });
@@ -545,11 +559,12 @@ long long few_slices(int N, int K) {
   return want < most ? want : most;
 }
 long long lora_t_bytes(long long rows, int r) { return bnh_round_up(rows * bnh_round_up(r, 32) * 2, 256); }
+long long lora_tu_bytes(long long rows, int r) { return lora_t_bytes(rows, r) + (r ? bnh_round_up(rows * 4, 256) : 0); }
 
 int lora_few(const LoraDev &p, const EpiDev &d, int dy, bool v, bool vr, bool vo, void *work, hipStream_t s) {
   const int Np = (int)bnh_round_up(p.N, 4), nn = (int)bnh_ceil_div(p.N, 32), ks = (int)few_slices(p.N, p.K);
   const int nd = dy * (int)bnh_ceil_div(p.rows, 16);
-  float *part = (float *)((char *)work + lora_t_bytes(p.rows, p.r));
+  float *part = (float *)((char *)work + lora_tu_bytes(p.rows, p.r));
   const dim3 grid((unsigned)(nd + nn * ks)), block(256);
 #define GO2(RT, RW)                                                                                            \
   do {                                                                                                         \
@@ -597,7 +612,7 @@ size_t bnh_pw_lora_work_bytes(int M, int B, int N, int K, int r) {
     return 0;
   }
   const long long rows = (long long)M * B;
-  return (size_t)(lora_t_bytes(rows, r) + (rows <= few ? 4 * few_slices(N, K) * rows * bnh_round_up(N, 4) : 0));
+  return (size_t)(lora_tu_bytes(rows, r) + (rows <= few ? 4 * few_slices(N, K) * rows * bnh_round_up(N, 4) : 0));
 }
 
 int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const uint16_t *w, int ldw, int N, int K,
@@ -614,7 +629,7 @@ int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const 
   const size_t need = bnh_pw_lora_work_bytes(M, B, N, K, ad ? L->r : 0);
   BNH_REQ(need == 0 || (work && on(work, 16) && work_bytes >= need));
   LoraDev p = {x, w, ad ? L->a : nullptr, ad ? L->b : nullptr, bias, ad ? L->scale : nullptr, ad ? idx : nullptr,
-               (uint16_t *)work, x_ws, lda, ldw, M, N, K, ad ? L->n : 0, ad ? L->r : 0,
+               (uint16_t *)work, ad ? (float *)((char *)work + lora_t_bytes((long long)M * B, L->r)) : nullptr, x_ws, lda, ldw, M, N, K, ad ? L->n : 0, ad ? L->r : 0,
                ad ? (int)bnh_round_up(L->r, 32) : 0, B == 1 || x_ws == (long long)M * lda,
                (long long)M * B, 1.0 / M};
   EpiDev d = {e->act, e->ldo, e->ldr, e->out, e->res, e->out_ws, e->res_ws,
