@@ -534,6 +534,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
   });
 }
 
+// ALL: for rows, ranks and outputs of every alignment, else for aligned ones alone
 template <int BM, int BN, int WM, int WN, int BK, int RING, bool ALL>
 int lora_tiles(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipStream_t s) {
   const long long nm = bnh_ceil_div(p.rows, BM), nn = bnh_ceil_div(p.N, BN);
@@ -541,11 +542,15 @@ int lora_tiles(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipS
   const dim3 grid((unsigned)(nm * nn)), block(64 * WM * WN);
 #define GO(V, VR, VO) \
   hipLaunchKernelGGL((k_lora_gemm<BM, BN, WM, WN, BK, RING, V, VR, VO>), grid, block, 0, s, p, d, (int)nm, (int)nn)
-  if (v && vr && vo) GO(true, true, true);
-  else if (v && vo) GO(true, false, true);
-  else if (v) GO(true, false, false);
-  else if (vo) GO(false, false, true);
-  else GO(false, false, false);
+  if constexpr (ALL) {
+    if (v && vr && vo) GO(true, true, true);
+    else if (v && vo) GO(true, false, true);
+    else if (v) GO(true, false, false);
+    else if (vo) GO(false, false, true);
+    else GO(false, false, false);
+  } else {
+    GO(true, true, true);
+  }
 #undef GO
   BNH_HIP(hipGetLastError());
   return 0;
@@ -629,9 +634,9 @@ int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const 
   const size_t need = bnh_pw_lora_work_bytes(M, B, N, K, ad ? L->r : 0);
   BNH_REQ(need == 0 || (work && on(work, 16) && work_bytes >= need));
   LoraDev p = {x, w, ad ? L->a : nullptr, ad ? L->b : nullptr, bias, ad ? L->scale : nullptr, ad ? idx : nullptr,
-               (uint16_t *)work, ad ? (float *)((char *)work + lora_t_bytes((long long)M * B, L->r)) : nullptr, x_ws, lda, ldw, M, N, K, ad ? L->n : 0, ad ? L->r : 0,
-               ad ? (int)bnh_round_up(L->r, 32) : 0, B == 1 || x_ws == (long long)M * lda,
-               (long long)M * B, 1.0 / M};
+               (uint16_t *)work, ad ? (float *)((char *)work + lora_t_bytes((long long)M * B, L->r)) : nullptr, x_ws, lda, ldw,
+               M, N, K, ad ? L->n : 0, ad ? L->r : 0, ad ? (int)bnh_round_up(L->r, 32) : 0,
+               B == 1 || x_ws == (long long)M * lda, (long long)M * B, 1.0 / M};
   EpiDev d = {e->act, e->ldo, e->ldr, e->out, e->res, e->out_ws, e->res_ws,
               B == 1 || (e->out_ws == (long long)M * e->ldo && (!e->res || e->res_ws == (long long)M * e->ldr))};
   hipStream_t s = bnh_stream(stream);
