@@ -58,6 +58,8 @@ extern "C" int bnh_gemm_f16_mfma_body(const uint16_t *A, long long a_ws, int lda
 extern "C" int bnh_pwdw_f32_plan(int C, int Kp, int H, int W, int k, int s, int pt, int pl, int form, int Ho, int Wo);
 
 static inline hipStream_t bnh_stream(void *s) { return (hipStream_t)s; }
+// blocks of `threads` threads to a launch: 2^32 threads in one grid dimension wrap around, or are refused
+static constexpr long long bnh_most_blocks(int threads) { return (1LL << 31) / threads; }
 static inline long long bnh_ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 static inline long long bnh_round_up(long long a, long long b) { return bnh_ceil_div(a, b) * b; }
 #endif

@@ -106,16 +106,16 @@ __device__ __forceinline__ void norm(float (&u)[NV * VEC], int kind, float eps, 
   }
 }
 
-// T threads to a row, a block of 256 or T
+// T threads to a row, a block of 256 or T; rows from row0
 template <typename TF, typename TX, int T, int VEC, int NV>
 __global__ __launch_bounds__(T > 256 ? T : 256) void k_block_norm(NormDev p, int M, double rM, int C, float rC,
-                                                                      int rows) {
+                                                                      unsigned row0, unsigned rows) {
   constexpr int RPB = T < 256 ? 256 / T : 1;  // rows to a block
   __shared__ float s[T > 64 ? T / 64 : 1];
   const int t = threadIdx.x % T;
-  const int row = (int)blockIdx.x * RPB + (int)threadIdx.x / T;
+  const unsigned row = row0 + blockIdx.x * RPB + threadIdx.x / T;
   if (T <= 64 && row >= rows) return;  // all threads of a row, and no barrier in these forms
-  const int w = bnh_div(row, M, rM), m = row - w * M;
+  const int w = bnh_div(row, M, rM), m = (int)row - w * M;
   float u[NV * VEC], g[NV * VEC], y[NV * VEC];
   const TF *f = p.f ? (const TF *)p.f + w * p.f_ws + (long long)m * p.ldf : nullptr;
   const TF *gate = p.gate ? (const TF *)p.gate + w * p.g_ws + (long long)m * p.ldg : nullptr;
@@ -169,14 +169,18 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_block_norm(NormDev p, int
 
 template <typename TF, typename TX, int VEC>
 int run(const NormDev &d, int M, int C, int B, hipStream_t s) {
-  const int rows = M * B;
+  const unsigned rows = (unsigned)M * B;
   const double rM = 1.0 / M;
   const float rC = 1.f / (float)C;
 #define GO(T, E)                                                                                                        \
   do {                                                                                                                  \
-    hipLaunchKernelGGL((k_block_norm<TF, TX, T, VEC, (E) / VEC>), dim3((unsigned)bnh_ceil_div(rows, T < 256 ? 256 / T : 1)), \
-                       dim3(T < 256 ? 256 : T), 0, s, d, M, rM, C, rC, rows);                                           \
-    BNH_HIP(hipGetLastError());                                                                                         \
+    constexpr int NT = T < 256 ? 256 : T, RPB = NT / T;                                                                 \
+    const long long most = bnh_most_blocks(NT), blocks = bnh_ceil_div(rows, RPB);                                       \
+    for (long long b0 = 0; b0 < blocks; b0 += most) {                                                                   \
+      hipLaunchKernelGGL((k_block_norm<TF, TX, T, VEC, (E) / VEC>), dim3((unsigned)(blocks - b0 < most ? blocks - b0 : most)), \
+                         dim3(NT), 0, s, d, M, rM, C, rC, (unsigned)(b0 * RPB), rows);                                  \
+      BNH_HIP(hipGetLastError());                                                                                       \
+    }                                                                                                                   \
     return 0;                                                                                                           \
   } while (0)
   // 20 M values with 8 or 16 a lane: C 64 73 us by 16 threads a row and 212 by 64; C 512 55 by 64 and 100 by 256; C 768 68
