@@ -143,9 +143,9 @@ __device__ __forceinline__ void lora_down(const LoraDev &p, long long tile, unsi
   }
 }
 template <int RT, bool V>
-__global__ __launch_bounds__(256) void k_lora_down(LoraDev p) {
+__global__ __launch_bounds__(256) void k_lora_down(LoraDev p, long long tile0) {
   __shared__ __attribute__((aligned(16))) float s[768 * RT];
-  lora_down<RT, V>(p, blockIdx.x, blockIdx.y, s);
+  lora_down<RT, V>(p, tile0 + blockIdx.x, blockIdx.y, s);
 }
 
 __device__ __forceinline__ float lora_act(float y, int act) {
@@ -288,7 +288,7 @@ __device__ __forceinline__ void lora_tile(unsigned lb, int nm, int nn, int *tm, 
 // row is permuted instead). The first operand of the matrix instruction is the weights': a lane's accumulators are
 // four channels of one row.
 template <int BM, int BN, int WM, int WN, int BK, int RING, bool DMA, bool VR, bool VO>
-__global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e, int nm, int nn) {
+__global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e, int tm0, int nm, int nn) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, CH = BK / 8, RPI = 64 / CH;
   constexpr int NL = (BM + BN) * CH / 64 / NW, ST = DMA ? RING : 2, SH = (BM + BN) * BK;  // loads a wave; stages, their halves
   constexpr int XS = 16 * TN + 4;                                                   // an exchange row, floats
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, q4 = lane >> 4;
   int tm, tn;
   lora_tile(bnh_xcd_block(blockIdx.x, gridDim.x), nm, nn, &tm, &tn);
-  const long long r0 = (long long)tm * BM;
+  const long long r0 = (long long)(tm0 + tm) * BM;
   const int n0 = tn * BN;
   auto fx = [](int row) { return CH == 4 ? (row >> 2) & 3 : (row >> 1) & 7; };
 
@@ -538,21 +538,25 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
 template <int BM, int BN, int WM, int WN, int BK, int RING, bool ALL>
 int lora_tiles(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipStream_t s) {
   const long long nm = bnh_ceil_div(p.rows, BM), nn = bnh_ceil_div(p.N, BN);
-  if (nm * nn >= (1LL << 31)) return bnh_fail("bnh_pw_lora: %lld x %d outputs are too many tiles", p.rows, p.N);
-  const dim3 grid((unsigned)(nm * nn)), block(64 * WM * WN);
+  const long long most = bnh_most_blocks(64 * WM * WN) / nn;  // N < 2^24: 16 at least
+  const dim3 block(64 * WM * WN);
+  for (long long m0 = 0; m0 < nm; m0 += most) {
+    const int n = (int)(nm - m0 < most ? nm - m0 : most);
+    const dim3 grid((unsigned)(n * nn));
 #define GO(V, VR, VO) \
-  hipLaunchKernelGGL((k_lora_gemm<BM, BN, WM, WN, BK, RING, V, VR, VO>), grid, block, 0, s, p, d, (int)nm, (int)nn)
-  if constexpr (ALL) {
-    if (v && vr && vo) GO(true, true, true);
-    else if (v && vo) GO(true, false, true);
-    else if (v) GO(true, false, false);
-    else if (vo) GO(false, false, true);
-    else GO(false, false, false);
-  } else {
-    GO(true, true, true);
-  }
+  hipLaunchKernelGGL((k_lora_gemm<BM, BN, WM, WN, BK, RING, V, VR, VO>), grid, block, 0, s, p, d, (int)m0, n, (int)nn)
+    if constexpr (ALL) {
+      if (v && vr && vo) GO(true, true, true);
+      else if (v && vo) GO(true, false, true);
+      else if (v) GO(true, false, false);
+      else if (vo) GO(false, false, true);
+      else GO(false, false, false);
+    } else {
+      GO(true, true, true);
+    }
 #undef GO
-  BNH_HIP(hipGetLastError());
+    BNH_HIP(hipGetLastError());
+  }
   return 0;
 }
 // Rows up to which w's bytes bound the product: 32 rows, 1,536 x 1,536 12.8 us and 25.8 on the tiles; 64 rows, 1,536 x 6,144
@@ -648,17 +652,20 @@ int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const 
                   (!e->res || (e->ldr % 8 == 0 && on(e->res, 16) && (B == 1 || e->res_ws % 8 == 0)));
   if (p.rows <= few) return lora_few(p, d, ad ? dy : 0, v && (!ad || va), vr || !ad, vo, work, s);
   if (ad) {
-    const dim3 grid((unsigned)bnh_ceil_div(p.rows, 16), (unsigned)dy);
-#define GO(RT)                                                                   \
-  if (va) hipLaunchKernelGGL((k_lora_down<RT, true>), grid, dim3(256), 0, s, p); \
-  else hipLaunchKernelGGL((k_lora_down<RT, false>), grid, dim3(256), 0, s, p)
-    if (p.r <= 16) GO(1);
-    else if (p.r <= 32) GO(2);
-    else if (p.r <= 64) GO(4);
-    else if (p.r <= 128) GO(8);
-    else GO(16);
+    const long long tiles = bnh_ceil_div(p.rows, 16), most = bnh_most_blocks(256);
+    for (long long t0 = 0; t0 < tiles; t0 += most) {
+      const dim3 grid((unsigned)(tiles - t0 < most ? tiles - t0 : most), (unsigned)dy);
+#define GO(RT)                                                                       \
+  if (va) hipLaunchKernelGGL((k_lora_down<RT, true>), grid, dim3(256), 0, s, p, t0); \
+  else hipLaunchKernelGGL((k_lora_down<RT, false>), grid, dim3(256), 0, s, p, t0)
+      if (p.r <= 16) GO(1);
+      else if (p.r <= 32) GO(2);
+      else if (p.r <= 64) GO(4);
+      else if (p.r <= 128) GO(8);
+      else GO(16);
 #undef GO
-    BNH_HIP(hipGetLastError());
+      BNH_HIP(hipGetLastError());
+    }
   }
   return lora_gemm(p, d, v, vr || !ad, vo, s);
 }

@@ -7,6 +7,13 @@ from test_gpu_context import say
 pytestmark = pytest.mark.gpu
 
 
+def part(H, ptr, n, dtype):
+    """n values from a device address."""
+    a = np.empty(n, dtype)
+    H.check(H.lib().bnh_memcpy_d2h(a.ctypes.data, ptr, a.nbytes))
+    return a
+
+
 def test_norm_many_rows(hip):
     """2^28 + rows of one value, 16 threads each: windows that share their input."""
     H, M, B = hip, 1 << 14, (1 << 14) + 3
@@ -17,3 +24,43 @@ def test_norm_many_rows(hip):
     H.check(H.lib().bnh_block_norm(a, M, 1, B, None), "block_norm")
     H.sync()
     assert (y.numpy().reshape(B, M) == x).all()
+
+
+def test_adapters_many_rows(hip):
+    """2^28 + rows, windows of two adapters and of none."""
+    H, M, B, K, N, r = hip, 1 << 14, (1 << 14) + 3, 8, 8, 4
+    say("adapters many rows")
+    rng = np.random.default_rng(0)
+    x = rng.integers(-4, 5, (M, K)).astype(np.float16)
+    w, a = rng.integers(-3, 4, (N, K)).astype(np.float16), rng.integers(-2, 3, (2, r, K)).astype(np.float16)
+    b = rng.integers(-2, 3, (2, N, r)).astype(np.float16)
+    idx = (np.arange(B) % 3 - 1).astype(np.int32)
+    dx, dw, da, db, di = (H.DeviceArray.from_host(z) for z in (x, w, a, b, idx))
+    out = H.DeviceArray.zeros((B * M * N,), np.float16)
+    wb = H.lib().bnh_pw_lora_work_bytes(M, B, N, K, r)
+    ws = H.DeviceArray((wb,), np.uint8)
+    H.check(H.lib().bnh_pw_lora(dx.ptr, 0, K, M, B, dw.ptr, K, N, K, None, H.Lora(2, r, da.ptr, db.ptr, None), di.ptr,
+                                H.Epi16(0, out.ptr, M * N, N, 0, 0, None, 0, 0), ws.ptr, wb, None), "pw_lora")
+    H.sync()
+    f = [z.astype(np.float64) for z in (x, w, a, b)]
+    want = [f[0] @ f[1].T] + [f[0] @ f[1].T + (f[0] @ f[2][j].T) @ f[3][j].T for j in range(2)]
+    assert max(np.abs(z).max() for z in want) < 2048  # whole numbers: fp16 holds them, the first product has few
+    for i in (0, 1, 2, 255, 256, 8191, 8192, B - 4, B - 3, B - 2, B - 1):
+        got = part(H, out.ptr + 2 * i * M * N, M * N, np.float16).reshape(M, N)
+        assert np.array_equal(got, want[idx[i] + 1]), i
+
+
+def test_projection_most_rows(hip):
+    """2^31 - 2 rows of one value each, tiles of 128."""
+    H, M, B = hip, 42966, 49981
+    say("projection most rows")
+    x = (np.arange(M) % 1000).astype(np.float16)
+    dx, dw = H.DeviceArray.from_host(x), H.DeviceArray.from_host(np.array([2], np.float16))
+    out = H.DeviceArray.zeros((B * M,), np.float16)
+    wb = H.lib().bnh_pw_lora_work_bytes(M, B, 1, 1, 0)
+    assert wb == 0
+    H.check(H.lib().bnh_pw_lora(dx.ptr, 0, 1, M, B, dw.ptr, 1, 1, 1, None, None, None,
+                                H.Epi16(0, out.ptr, M, 1, 0, 0, None, 0, 0), None, 0, None), "pw_lora")
+    H.sync()
+    for i in (0, 1, B // 2, B - 2, B - 1):
+        assert np.array_equal(part(H, out.ptr + 2 * i * M, M, np.float16), 2 * x), i
