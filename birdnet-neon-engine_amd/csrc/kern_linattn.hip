@@ -19,6 +19,7 @@ struct LaDev {
   float *s1;
   const int32_t *start, *len, *slot;
   int ldq, ldk, ldv, ldo, ldg, H, rq, rk, rv, dk, dv, slots, T, rows;  // rq: heads that share a q head
+  int b0;  // the launch's first sequence
   float scale;
 };
 
@@ -47,7 +48,8 @@ __global__ __launch_bounds__(256) void k_la_step(LaDev p, int nsl) {
   __shared__ float s_q[2][256], s_k[2][256];
   __shared__ __attribute__((aligned(16))) float s_r[2][4][4 * LANES];
   const int tid = threadIdx.x, ln = tid % LANES, rg = tid / LANES;
-  const int sl = (int)(blockIdx.x % nsl), h = (int)(blockIdx.x / nsl % p.H), b = (int)(blockIdx.x / nsl / p.H);
+  const int sl = (int)(blockIdx.x % nsl), h = (int)(blockIdx.x / nsl % p.H);
+  const int b = p.b0 + (int)(blockIdx.x / nsl / p.H);
   const int col = sl * 4 * LANES + 4 * ln;
   int first;
   const int n = la_rows(p, b, &first);
@@ -133,16 +135,20 @@ __global__ __launch_bounds__(256) void k_la_step(LaDev p, int nsl) {
 }
 
 template <typename T, int LANES, bool VS>
-int step_run(const LaDev &d, int B, hipStream_t s) {
+int step_run(LaDev d, int B, hipStream_t s) {
   constexpr int RG = 256 / LANES;
   const int nsl = (int)bnh_ceil_div(d.dv, 4 * LANES), kr = (int)bnh_ceil_div(d.dk, RG);
-  const dim3 grid((unsigned)((long long)nsl * d.H * B)), block(256);
+  const int most = (int)(bnh_most_blocks(256) / ((long long)nsl * d.H));  // sequences; H <= 2^16, dv <= 2^8: 16 at least
+  for (long long b0 = 0; b0 < B; b0 += most) {
+    d.b0 = (int)b0;
+    const dim3 grid((unsigned)((long long)nsl * d.H * (B - b0 < most ? B - b0 : most))), block(256);
 #define GO(KR) hipLaunchKernelGGL((k_la_step<T, LANES, KR, VS>), grid, block, 0, s, d, nsl)
-  if (kr <= 256 / RG / 4) GO(256 / RG / 4);
-  else if (kr <= 256 / RG / 2) GO(256 / RG / 2);
-  else GO(256 / RG);
+    if (kr <= 256 / RG / 4) GO(256 / RG / 4);
+    else if (kr <= 256 / RG / 2) GO(256 / RG / 2);
+    else GO(256 / RG);
 #undef GO
-  BNH_HIP(hipGetLastError());
+    BNH_HIP(hipGetLastError());
+  }
   return 0;
 }
 
@@ -286,7 +292,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
   unsigned lb = bnh_xcd_block(blockIdx.x, gridDim.x);
   const int sl = (int)(lb % nsl), h = (int)(lb / nsl % p.H);
   lb /= nsl * p.H;
-  const int pc = (int)(lb % (OUT ? npc : npc - 1)), b = (int)(lb / (OUT ? npc : npc - 1));
+  const int pc = (int)(lb % (OUT ? npc : npc - 1)), b = p.b0 + (int)(lb / (OUT ? npc : npc - 1));
   int first;
   const int n = la_rows(p, b, &first), slot = la_slot(p, b);
   const int r0 = pc * pcr;
@@ -785,7 +791,7 @@ size_t plan_bytes(const Plan &r) {
 }
 
 template <typename T, int DKT, int NW, int C, bool V>
-int chunk_run(const LaDev &d, const Plan &r, void *work, hipStream_t s) {
+int chunk_run(LaDev d, const Plan &r, int B, void *work, hipStream_t s) {
   float *part = (float *)work, *pdec = part ? (float *)((char *)work + bnh_round_up(4 * r.states * r.npc * r.floats, 256)) : nullptr;
   const dim3 block(64 * NW);
   if (r.npc > 1) {
@@ -799,22 +805,28 @@ int chunk_run(const LaDev &d, const Plan &r, void *work, hipStream_t s) {
       BNH_HIP(hipGetLastError());
     }
   }
-  hipLaunchKernelGGL((k_la_chunk<T, DKT, NW, C, V, true>), dim3((unsigned)(r.states * r.npc)), block, 0, s, d, r.nsl, r.npc,
-                     r.pcr, part, pdec);
-  BNH_HIP(hipGetLastError());
+  // sequences a launch; those in pieces are far fewer (states of 512 blocks at most), and go in one
+  const long long per = (long long)r.nsl * d.H * r.npc;
+  const int most = (int)(bnh_most_blocks(64 * NW) / per);
+  for (long long b0 = 0; b0 < B; b0 += most) {
+    d.b0 = (int)b0;
+    hipLaunchKernelGGL((k_la_chunk<T, DKT, NW, C, V, true>), dim3((unsigned)(per * (B - b0 < most ? B - b0 : most))), block, 0,
+                       s, d, r.nsl, r.npc, r.pcr, part, pdec);
+    BNH_HIP(hipGetLastError());
+  }
   return 0;
 }
 template <typename T, int NW, int C, bool V>
-int chunk_dk(const LaDev &d, const Plan &r, void *work, hipStream_t s) {
-  if (r.dkt == 1) return chunk_run<T, 1, NW, C, V>(d, r, work, s);
-  if (r.dkt == 2) return chunk_run<T, 2, NW, C, V>(d, r, work, s);
-  if (r.dkt == 4) return chunk_run<T, 4, NW, C, V>(d, r, work, s);
-  return chunk_run<T, 8, NW, C, V>(d, r, work, s);
+int chunk_dk(const LaDev &d, const Plan &r, int B, void *work, hipStream_t s) {
+  if (r.dkt == 1) return chunk_run<T, 1, NW, C, V>(d, r, B, work, s);
+  if (r.dkt == 2) return chunk_run<T, 2, NW, C, V>(d, r, B, work, s);
+  if (r.dkt == 4) return chunk_run<T, 4, NW, C, V>(d, r, B, work, s);
+  return chunk_run<T, 8, NW, C, V>(d, r, B, work, s);
 }
 template <typename T, int C>
-int chunk_go(const LaDev &d, const Plan &r, bool v, void *work, hipStream_t s) {
-  if (r.nw == 8) return v ? chunk_dk<T, 8, C, true>(d, r, work, s) : chunk_dk<T, 8, C, false>(d, r, work, s);
-  return v ? chunk_dk<T, 4, C, true>(d, r, work, s) : chunk_dk<T, 4, C, false>(d, r, work, s);
+int chunk_go(const LaDev &d, const Plan &r, int B, bool v, void *work, hipStream_t s) {
+  if (r.nw == 8) return v ? chunk_dk<T, 8, C, true>(d, r, B, work, s) : chunk_dk<T, 8, C, false>(d, r, B, work, s);
+  return v ? chunk_dk<T, 4, C, true>(d, r, B, work, s) : chunk_dk<T, 4, C, false>(d, r, B, work, s);
 }
 
 int la_check(const bnh_la *p, int T, int B) {
@@ -847,7 +859,7 @@ int bnh_linattn(const bnh_la *p, int T, int B, int rows, const int32_t *start, c
   BNH_REQ(on(p->q, es) && on(p->k, es) && on(p->v, es) && on(p->o, es) && on(p->g, 4) && on(p->s0, 4) && on(p->s1, 4));
   BNH_REQ(on(p->slot, 4) && on(start, 4) && on(len, 4));
   LaDev d = {p->q, p->k, p->v, p->o, p->g, p->s0, p->s1, start, len, p->slot, p->ldq, p->ldk, p->ldv, p->ldo, p->ldg,
-             p->H, p->H / p->Hq, p->H / p->Hk, p->H / p->Hv, p->dk, p->dv, p->slots, T, rows, p->scale};
+             p->H, p->H / p->Hq, p->H / p->Hk, p->H / p->Hv, p->dk, p->dv, p->slots, T, rows, 0, p->scale};
   const bool vs = p->dv % 4 == 0 && on(p->s0, 16) && on(p->s1, 16);
   hipStream_t s = bnh_stream(stream);
   const Plan r = plan(p, T, B);
@@ -858,7 +870,7 @@ int bnh_linattn(const bnh_la *p, int T, int B, int rows, const int32_t *start, c
     const int ve = 16 / (int)es;
     const bool v = on(p->q, 16) && on(p->k, 16) && on(p->v, 16) && on(p->o, 16) && p->ldq % ve == 0 && p->ldk % ve == 0 &&
                    p->ldv % ve == 0 && p->ldo % ve == 0 && p->dk % ve == 0 && p->dv % ve == 0;
-    return p->f16 ? chunk_go<h16, 64>(d, r, v, work, s) : chunk_go<float, 32>(d, r, v, work, s);
+    return p->f16 ? chunk_go<h16, 64>(d, r, B, v, work, s) : chunk_go<float, 32>(d, r, B, v, work, s);
   }
   return p->f16 ? step_go<h16>(d, B, vs, s) : step_go<float>(d, B, vs, s);
 }

@@ -64,3 +64,45 @@ def test_projection_most_rows(hip):
     H.sync()
     for i in (0, 1, B // 2, B - 2, B - 1):
         assert np.array_equal(part(H, out.ptr + 2 * i * M, M, np.float16), 2 * x), i
+
+
+def test_linattn_many_states(hip):
+    """More than 2^23 heads and sequences of two slices of columns each, a row a sequence."""
+    H, heads, B, dv = hip, 1 << 16, 129, 129
+    say("linattn many states")
+    rng = np.random.default_rng(1)
+    q, k, v = (rng.integers(-5, 6, (B, n)).astype(np.float16) for n in (1, 1, dv))
+    dq, dk, dv_, g = (H.DeviceArray.from_host(z) for z in (q, k, v, np.zeros(heads, np.float32)))
+    o = H.DeviceArray.zeros((B * heads * dv,), np.float16)
+    a = H.LinAttn(q=dq.ptr, k=dk.ptr, v=dv_.ptr, o=o.ptr, f16=1, ldq=1, ldk=1, ldv=dv, ldo=heads * dv, H=heads, Hq=1, Hk=1,
+                  Hv=1, dk=1, dv=dv, g=g.ptr, ldg=0, scale=1.0)
+    H.check(H.lib().bnh_linattn(a, 1, B, B, None, None, None, 0, None), "linattn")
+    H.sync()
+    for i in (0, 1, 63, 64, B - 2, B - 1):
+        got = part(H, o.ptr + 2 * i * heads * dv, heads * dv, np.float16).reshape(heads, dv)
+        assert (got == q[i] * k[i] * v[i]).all(), i
+
+
+def test_linattn_many_chunks(hip):
+    """More than 2^23 blocks of chunks, most of them of sequences without a row."""
+    H, heads, B, T, d = hip, 1 << 16, 129, 9, 65
+    say("linattn many chunks")
+    rng = np.random.default_rng(2)
+    full = [0, 64, 127, 128]
+    rows = T * len(full)
+    lens, start = np.zeros(B, np.int32), np.zeros(B, np.int32)
+    lens[full], start[full] = T, T * np.arange(len(full))
+    q, k, v = (rng.integers(-3, 4, (rows, n)).astype(np.float16) for n in (1, 1, d))
+    dq, dk, dv, ds, dl, g = (H.DeviceArray.from_host(z) for z in (q, k, v, start, lens, np.zeros(heads, np.float32)))
+    o = H.DeviceArray.zeros((rows * heads * d,), np.float16)
+    a = H.LinAttn(q=dq.ptr, k=dk.ptr, v=dv.ptr, o=o.ptr, f16=1, ldq=1, ldk=1, ldv=d, ldo=heads * d, H=heads, Hq=1, Hk=1,
+                  Hv=1, dk=1, dv=d, g=g.ptr, ldg=0, scale=1.0)
+    assert H.lib().bnh_linattn_work_bytes(a, T, B) == 0
+    H.check(H.lib().bnh_linattn(a, T, B, rows, ds.ptr, dl.ptr, None, 0, None), "linattn")
+    H.sync()
+    got = o.numpy().reshape(rows, heads, d)
+    for i in range(len(full)):
+        s = slice(i * T, i * T + T)
+        kv = (k[s].astype(np.float64) * v[s]).cumsum(0)
+        want = q[s].astype(np.float64) * kv
+        assert np.abs(want).max() < 2048 and (got[s] == want[:, None]).all(), i
