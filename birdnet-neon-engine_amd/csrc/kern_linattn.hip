@@ -173,11 +173,13 @@ int step_go(const LaDev &d, int B, bool vs, hipStream_t s) {
 // product with q's rows, so it never passes through LDS. q, k and v of the next chunk are loaded into registers while this
 // one's are multiplied out of LDS; k's and v's transposes come out of LDS through ds_read_b64_tr_b16.
 //
-// fp16 rows: the factors of a product have to be fp16, its sums are fp32. Scores are scaled row by row and the state
-// column by column by powers of two before they are rounded (their largest to 2^12..2^13), so neither overflows and both
-// keep 11 bits, as the rounded output does. The state itself is not rounded: its update takes v_j e^{c_C - c_j}, the
-// largest of the chunk's by column scaled to 2^14..2^15 (the state's own unit from then on), in two fp16 parts, 22 bits, against
-// the exact k. fp32 rows run on the fp32 MFMA, unscaled and unsplit.
+// fp16 rows: the factors of a product have to be fp16, its sums are fp32. Scores, the state and what is added to it go in as
+// two fp16 parts each, 22 bits, against the exact v, q and k. Scores are scaled row by row and the state column by column by
+// powers of two first (their largest to 2^12..2^13), so neither overflows. The state itself is not rounded: its update takes
+// v_j e^{c_C - c_j}, the largest of the chunk's by column scaled to 2^14..2^15 (the state's own unit from then on). With one
+// part for scores and state the outputs' relative error was 2.9e-4 instead of the 2.1e-4 of fp16 outputs as such, and several
+// times the outputs' own rounding where their terms cancel; the second parts cost 17 us of the 139 below, and 12 of the 136.
+// fp32 rows run on the fp32 MFMA, unscaled and unsplit.
 //
 // 12 heads of 128 x 128 in fp16: 17,280 rows of one sequence 126 us (22 pieces of 13 chunks: what the pieces add 34, the
 // join 9, the outputs 78; 214 MB would take 42), 24 sequences of up to 720 rows 126 us. A chunk takes a block 12,000
@@ -282,7 +284,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
   constexpr int NK = C / RK > 0 ? C / RK : 1, NV = C / RV > 0 ? C / RV : 1;
   typedef typename Frag<T>::V FV;
   typedef typename Frag<T>::H FH;
-  __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SQ : 1], s_k[C * SK], s_v[C * SV], s_p[2][OUT ? C * SP : 1];
+  __shared__ __attribute__((aligned(16))) T s_q[OUT ? C * SQ : 1], s_k[C * SK], s_v[C * SV], s_p[2][OUT ? C * SP : 1],
+      s_l[2][OUT && F16 ? C * SP : 1];                         // F16: the scores' second parts
   __shared__ double s_c[2][64];                              // c_i
   __shared__ __attribute__((aligned(16))) float s_w[2][64];  // e^{c_C - c_j}
   __shared__ float s_e[2][64], s_d[2];                       // e^{c_i}; e^{c_C}
@@ -338,6 +341,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     for (int i = tid; i < C / 32 * 256; i += NT)
       s_p[0][(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] =
           s_p[1][(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] = (T)0.f;
+    if (F16)
+      for (int i = tid; i < C / 32 * 256; i += NT)
+        s_l[0][(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] =
+            s_l[1][(i / 256 * 32 + i % 256 / 16) * SP + i / 256 * 32 + 16 + i % 16] = (T)0.f;
   }
 
   const int kr = tid / (KD / VE), kc = tid % (KD / VE) * VE, vr = tid / (DV / VE), vc = tid % (DV / VE) * VE;
@@ -506,19 +513,28 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
             m = fmaxf(m, fabsf(a[c][r]));
           }
         float dn = 1.f;
+        uint64_t keep = ~0ull;  // an infinity has no second part, nor has its row
         if (F16) {
           m = fmaxf(m, __shfl_xor(m, 16));
           m = fmaxf(m, __shfl_xor(m, 32));
+          keep = m - m == 0.f ? ~0ull : 0;
           const int x = scale_exp(m);
           dn = ldexpf(1.f, -x);
           if (q4 == 0) s_x[u][jj][i] = x;
         }
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          FH y;
+          FH y, z;
 #pragma unroll
-          for (int r = 0; r < 4; r++) y[r] = (T)(F16 ? a[c][r] * dn : a[c][r]);
-          if (c == 0 || two) *(FH *)(s_p[u] + i * SP + 32 * jj + 16 * c + 4 * q4) = y;
+          for (int r = 0; r < 4; r++) {
+            const float x = F16 ? a[c][r] * dn : a[c][r];
+            y[r] = (T)x;
+            if (F16) z[r] = (T)(x - (float)y[r]);
+          }
+          if (c == 0 || two) {
+            *(FH *)(s_p[u] + i * SP + 32 * jj + 16 * c + 4 * q4) = y;
+            if constexpr (F16) *(uint64_t *)(s_l[u] + i * SP + 32 * jj + 16 * c + 4 * q4) = __builtin_bit_cast(uint64_t, z) & keep;
+          }
         }
       }
     }
@@ -550,8 +566,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     v4f a[C / 16];
     float xs[4];  // 2^x of the accumulators' columns 4 q4 + r
     if constexpr (OUT) {
-      FV sf[DKT];
       float dn = 1.f;
+      uint32_t keep = ~0u;
       if (F16) {
         float m = 0.f;
 #pragma unroll
@@ -561,21 +577,34 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
         const int x = scale_exp(m);
+        keep = m - m == 0.f ? ~0u : 0;
         const float up = ldexpf(1.f, x + ux);
         dn = ldexpf(1.f, -x);
 #pragma unroll
         for (int r = 0; r < 4; r++) xs[r] = __shfl(up, 4 * q4 + r);
       }
 #pragma unroll
-      for (int d = 0; d < DKT; d++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) sf[d][e] = (T)(F16 ? S[2 * d + e / 4][e % 4] * dn : S[2 * d + e / 4][e % 4]);
-#pragma unroll
       for (int ib = 0; ib < C / 16; ib++) a[ib] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int d = 0; d < DKT; d++)
+      for (int d = 0; d < DKT; d++) {
+        FV sf, sl, x[C / 16];
 #pragma unroll
-        for (int ib = 0; ib < C / 16; ib++) a[ib] = mma(sf[d], row44<T>(s_q + (16 * ib + lr) * SQ + 32 * d + 4 * q4), a[ib]);
+        for (int ib = 0; ib < C / 16; ib++) x[ib] = row44<T>(s_q + (16 * ib + lr) * SQ + 32 * d + 4 * q4);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float y = F16 ? S[2 * d + e / 4][e % 4] * dn : S[2 * d + e / 4][e % 4];
+          sf[e] = (T)y;
+          if (F16) sl[e] = (T)(y - (float)sf[e]);
+        }
+#pragma unroll
+        for (int ib = 0; ib < C / 16; ib++) a[ib] = mma(sf, x[ib], a[ib]);
+        if constexpr (F16) {
+          typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+          sl = __builtin_bit_cast(FV, __builtin_bit_cast(u4, sl) & (u4){keep, keep, keep, keep});
+#pragma unroll
+          for (int ib = 0; ib < C / 16; ib++) a[ib] = mma(sl, x[ib], a[ib]);
+        }
+      }
     }
     // the state's update
     FV hi[C / 32], lo[C / 32];
@@ -654,10 +683,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
       for (int ib = 0; ib < C / 16; ib++) {  // the state's part and each step of 32 columns have a unit of their own
         const int i = 16 * ib + lr;
         const float ec = s_e[u][i];
-        const v4f z = {0.f, 0.f, 0.f, 0.f}, y0 = mma(vf[0], row44<T>(s_p[u] + i * SP + 4 * q4), z);
+        v4f y0 = mma(vf[0], row44<T>(s_p[u] + i * SP + 4 * q4), (v4f){0.f, 0.f, 0.f, 0.f});
+        if (F16) y0 = mma(vf[0], row44<T>(s_l[u] + i * SP + 4 * q4), y0);
         const float u0 = F16 ? ldexpf(1.f, s_x[u][0][i]) : 1.f;
         if (C == 64 && ib >= 2) {
-          const v4f y1 = mma(vf[C / 32 - 1], row44<T>(s_p[u] + i * SP + 32 + 4 * q4), z);
+          v4f y1 = mma(vf[C / 32 - 1], row44<T>(s_p[u] + i * SP + 32 + 4 * q4), (v4f){0.f, 0.f, 0.f, 0.f});
+          if (F16) y1 = mma(vf[C / 32 - 1], row44<T>(s_l[u] + i * SP + 32 + 4 * q4), y1);
           const float u1 = F16 ? ldexpf(1.f, s_x[u][1][i]) : 1.f;
 #pragma unroll
           for (int r = 0; r < 4; r++) {

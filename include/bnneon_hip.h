@@ -483,8 +483,8 @@ typedef struct {
  * w fp16 rows [N][ldw >= K], bias fp32 [N] (NULL: 0), idx int32 [B] on the device; L NULL: no adapters. The epilogue is
  * e's with rows only (opad 0; act 1 is the fp32 SiLU x / (1 + e^-x)): fp16 MFMA with fp32 sums over all of K and r, a
  * and x's product rounded to fp16's 11 bits in between (scaled by a power of two for each row, so it may lie outside fp16's
- * range), one rounding at the end. A row depends on its own window's adapter alone, whatever the others hold. Windows of one adapter side by side are fastest. work: device scratch of at least
- * bnh_pw_lora_work_bytes bytes, 16-byte aligned. */
+ * range), one rounding at the end. A row depends on its own window's adapter alone, whatever the others hold. Windows of
+ * one adapter side by side are fastest. work: device scratch of at least bnh_pw_lora_work_bytes bytes, 16-byte aligned. */
 size_t bnh_pw_lora_work_bytes(int M, int B, int N, int K, int r);
 int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const uint16_t *w, int ldw, int N, int K,
                 const float *bias, const bnh_lora *L, const int32_t *idx, const bnh_epi16 *e, void *work,
@@ -515,6 +515,8 @@ typedef struct {
 /* B sequences of at most T rows among `rows` rows: sequence i has the len[i] rows from start[i] (int32 [B] on the device;
  * NULL: T rows each, from i T), cut to T and to [0, rows), and none from a start outside; one of no rows leaves its state as it is. Sequences share no
  * rows. T up to 8 (1: a live station's new window) runs the recurrence, more rows a chunked form of it with matrix products.
+ * Sums are fp32; of fp16 rows, scores and states are factors of 22 bits in the chunked form. The workspace's size depends on
+ * f16, H, dk, dv, T and B, and fewer sequences can need more (longer ones are cut into pieces): ask for each shape.
  * work: device scratch of at least bnh_linattn_work_bytes bytes, 16-byte aligned (0 bytes for some shapes: NULL is
  * allowed then). */
 size_t bnh_linattn_work_bytes(const bnh_la *p, int T, int B);

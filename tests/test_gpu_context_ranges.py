@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_context import LaCase, say
+from test_gpu_context import LaCase, near, say
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,21 @@ def test_small_scores(hip, f16, T):
     c = LaCase(hip, [T], 2, 2, 2, 2, 16, 48, f16, gscale=0.1, s0=False, seed=T, edit=edit)
     c.run()
     c.check("small scores")
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("lens,heads,dk,dv", [([64, 9, 200], 4, 128, 128), ([700], 3, 64, 48), ([300, 40], 2, 256, 200),
+                                              ([130], 2, 24, 97)], ids=str)
+def test_factors_of_22_bits(hip, f16, lens, heads, dk, dv):
+    """Outputs whose terms cancel are those of sums in 32 bits of factors of 22 bits (two parts of 11, each of scores and state),
+    not of factors of the rows' own type."""
+    say(f"la factors lens {lens} dk {dk} dv {dv} f16 {f16}")
+    c = LaCase(hip, lens, heads, heads, heads, heads, dk, dv, f16, gscale=0.05, seed=dk)
+    c.run()
+    o = c.do.get()[0]
+    for i in range(len(lens)):
+        (wo, _, eo, _, mo), _ = c.want(i)
+        s, n = c.sequence(i)
+        if f16:  # and of the smallest step of a part beside the largest of its row or column, 2^-37
+            eo = eo + 3 * 2.0 ** -22 * mo + 2.0 ** -34 * mo.max(-1, keepdims=True)
+        near(o[s:s + n], wo.reshape(n, heads * dv), eo.reshape(n, heads * dv), f"o[{i}]", f16)
