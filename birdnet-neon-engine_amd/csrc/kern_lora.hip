@@ -1,9 +1,10 @@
 // A shared fp16 projection with low-rank adapters of many requests beside it (bnh_pw_lora):
 //   out = act(W x + bias + s_j B_j (A_j x)) (+ res), j the adapter of the row's window.
 //
-// Two launches. k_lora_down computes t = s_j A_j x for every row with an adapter, rounded to fp16: the factor that the
-// matrix instruction of the second product takes. A row's t is scaled by a power of two first (its largest to 2^14..2^15), so
-// that it keeps 11 bits whatever its size; the row's product takes the unit back in fp32. k_lora_gemm computes W x on fp16 MFMA
+// Two launches. k_lora_down computes t = s_j A_j x for every row with an adapter, as two fp16 parts (22 bits): factors that
+// the matrix instruction of the second product takes. A row's t is scaled by a power of two first (its largest to 2^14..2^15),
+// so that it keeps them whatever its size; the row's product takes the unit back in fp32. Up to 16 ranks both parts fit
+// one matrix instruction, against b's ranks twice. k_lora_gemm computes W x on fp16 MFMA
 // with fp32 sums and adds the product of t with the adapter's B to the sums it has, so that the adapter costs no pass over
 // the output. Rows of one matrix instruction are independent of each other, so a block of 16 rows whose adapters differ
 // multiplies all of them by each of the adapters in it and every row keeps its own: nothing of another request's adapter,
@@ -57,7 +58,7 @@ struct LoraDev {
   uint16_t *t;
   float *u;  // the unit of each row of t
   long long x_ws;
-  int lda, ldw, M, N, K, n, r, r32;  // r32: r rounded up to 32, t's row
+  int lda, ldw, M, N, K, n, r, half, r32;  // t's row: r32 values, its first parts from 0 and its second ones from half
   bool line;                         // x's windows follow each other: rows lda apart throughout
   long long rows;
   double rM;
@@ -69,7 +70,7 @@ __device__ __forceinline__ int lora_id(const LoraDev &p, int win) {  // -1: none
 }
 
 // t of the 16 rows from 16 tile for the which-th different adapter among them; the block's four waves take every fourth
-// step of 32 of K. RT: 16-column tiles of r32; s: 768 RT floats of LDS
+// step of 32 of K. RT: 16-column tiles of half a row of t; s: 768 RT floats of LDS
 template <int RT, bool V>
 __device__ __forceinline__ void lora_down(const LoraDev &p, long long tile, unsigned which, float *s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, kc = (lane >> 4) * 8;
@@ -137,9 +138,12 @@ __device__ __forceinline__ void lora_down(const LoraDev &p, long long tile, unsi
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       const int c = 16 * t + lr;
-      if (c < p.r32) p.t[r * p.r32 + c] = c < p.r ? hbits((h16)ldexpf(acc[t][e], -x)) : 0;
+      if (c >= p.half) continue;
+      const float y = c < p.r ? ldexpf(acc[t][e], -x) : 0.f;
+      const h16 hi = (h16)y;
+      p.t[r * p.r32 + c] = hbits(hi);
+      p.t[r * p.r32 + p.half + c] = hbits(y - y == 0.f ? (h16)(y - (float)hi) : (h16)0.f);
     }
-    if (RT == 1) p.t[r * p.r32 + 16 + lr] = 0;
   }
 }
 template <int RT, bool V>
@@ -242,13 +246,13 @@ __global__ __launch_bounds__(256) void k_lora_few_out(LoraDev p, EpiDev e, int k
   if (id >= 0) {
     const uint16_t *t = p.t + (long long)row * p.r32, *b = p.b + ((long long)id * p.N + n) * p.r;
     for (int k = 0; k < p.r; k += 8) {
-      const v8h x = *(const v8h *)(t + k);
+      const v8h x = *(const v8h *)(t + k), xl = *(const v8h *)(t + p.half + k);
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         if (n + c >= p.N) continue;
         const v8h z = ld8<VR>(b + (long long)c * p.r + k, p.r - k);
 #pragma unroll
-        for (int l = 0; l < 8; l++) u[c] = __builtin_fmaf((float)x[l], (float)z[l], u[c]);
+        for (int l = 0; l < 8; l++) u[c] = __builtin_fmaf((float)x[l] + (float)xl[l], (float)z[l], u[c]);
       }
     }
     const float un = p.u[row];
@@ -330,11 +334,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
     const long long row = r0 + wm + 16 * i + lr < p.rows ? r0 + wm + 16 * i + lr : p.rows - 1;
     id[i] = p.idx ? p.idx[bnh_div(row, p.M, p.rM)] : -1;
   });
-  // the adapters' operands: t of the wave's rows and b of the first adapter among them, for ranks k to k + 31
-  const uint16_t *bp[TN];
+  // the adapters' operands: values k to k + 31 of t of the wave's rows, and b of the first adapter among them for their ranks
+  const int rank = p.half == 16 ? 8 * (q4 & 1) : 8 * q4;  // half is 16 or a multiple of 32
+  uint32_t bp[TN];  // into an adapter's b: N < 2^24, r <= 2^8
 #pragma unroll
   for (int j = 0; j < TN; j++)
-    bp[j] = p.b + (long long)(n0 + wn + 16 * j + lr < p.N ? n0 + wn + 16 * j + lr : p.N - 1) * p.r + 8 * q4;
+    bp[j] = (uint32_t)(n0 + wn + 16 * j + lr < p.N ? n0 + wn + 16 * j + lr : p.N - 1) * (uint32_t)p.r + (uint32_t)rank;
   v8h ax[TM], bn[TN];
   float un[TM];
   uint32_t todo[TM];
@@ -346,12 +351,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_lora_gemm(LoraDev p, EpiDev e,
       if (next < 0 && todo[i]) next = __builtin_amdgcn_readlane(id[i], __builtin_ctz(todo[i]));
     });
     if (next >= 0) {
+      const int from = k < p.half ? k : k - p.half;
       each<TM>([&](auto tile) {
         constexpr int i = decltype(tile)::value;
         todo[i] &= ~(uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && id[i] == next);
       });
 #pragma unroll
-      for (int j = 0; j < TN; j++) bn[j] = ld8<VR>(bp[j] + (long long)next * p.N * p.r + k, p.r - k - 8 * q4);
+      for (int j = 0; j < TN; j++) bn[j] = ld8<VR>(p.b + (long long)next * p.N * p.r + from + bp[j], p.r - from - rank);
     }
   };
   auto ahead = [&](int k) {
@@ -567,7 +573,8 @@ long long few_slices(int N, int K) {
   const long long want = bnh_ceil_div(512, bnh_ceil_div(N, 32)), most = bnh_ceil_div(K, 128);
   return want < most ? want : most;
 }
-long long lora_t_bytes(long long rows, int r) { return bnh_round_up(rows * bnh_round_up(r, 32) * 2, 256); }
+int lora_half(int r) { return r == 0 ? 0 : r <= 16 ? 16 : (int)bnh_round_up(r, 32); }
+long long lora_t_bytes(long long rows, int r) { return bnh_round_up(rows * 2 * lora_half(r) * 2, 256); }
 long long lora_tu_bytes(long long rows, int r) { return lora_t_bytes(rows, r) + (r ? bnh_round_up(rows * 4, 256) : 0); }
 
 int lora_few(const LoraDev &p, const EpiDev &d, int dy, bool v, bool vr, bool vo, void *work, hipStream_t s) {
@@ -639,7 +646,7 @@ int bnh_pw_lora(const uint16_t *x, long long x_ws, int lda, int M, int B, const 
   BNH_REQ(need == 0 || (work && on(work, 16) && work_bytes >= need));
   LoraDev p = {x, w, ad ? L->a : nullptr, ad ? L->b : nullptr, bias, ad ? L->scale : nullptr, ad ? idx : nullptr,
                (uint16_t *)work, ad ? (float *)((char *)work + lora_t_bytes((long long)M * B, L->r)) : nullptr, x_ws, lda, ldw,
-               M, N, K, ad ? L->n : 0, ad ? L->r : 0, ad ? (int)bnh_round_up(L->r, 32) : 0,
+               M, N, K, ad ? L->n : 0, ad ? L->r : 0, ad ? lora_half(L->r) : 0, ad ? 2 * lora_half(L->r) : 0,
                B == 1 || x_ws == (long long)M * lda, (long long)M * B, 1.0 / M};
   EpiDev d = {e->act, e->ldo, e->ldr, e->out, e->res, e->out_ws, e->res_ws,
               B == 1 || (e->out_ws == (long long)M * e->ldo && (!e->res || e->res_ws == (long long)M * e->ldr))};

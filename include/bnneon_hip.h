@@ -482,7 +482,7 @@ typedef struct {
  * out = act(w x + bias + scale[j] b[j] (a[j] x)) (+ res), j = idx[i]; no adapter for a j outside [0, L->n).
  * w fp16 rows [N][ldw >= K], bias fp32 [N] (NULL: 0), idx int32 [B] on the device; L NULL: no adapters. The epilogue is
  * e's with rows only (opad 0; act 1 is the fp32 SiLU x / (1 + e^-x)): fp16 MFMA with fp32 sums over all of K and r, a
- * and x's product rounded to fp16's 11 bits in between (scaled by a power of two for each row, so it may lie outside fp16's
+ * and x's product rounded to 22 bits in between (two fp16 parts in a unit of the row's, so it may lie outside fp16's
  * range), one rounding at the end. A row depends on its own window's adapter alone, whatever the others hold. Windows of
  * one adapter side by side are fastest. work: device scratch of at least bnh_pw_lora_work_bytes bytes, 16-byte aligned. */
 size_t bnh_pw_lora_work_bytes(int M, int B, int N, int K, int r);

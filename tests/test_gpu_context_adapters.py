@@ -50,3 +50,22 @@ def test_first_product_not_finite(hip, M, B):
     fine = np.isfinite(want)
     assert not fine.all() and not np.isfinite(got[~fine]).any()
     near(got[fine], want[fine], err[fine], "finite", True)
+
+
+@pytest.mark.parametrize("M,B", [(1, 7), (1, 60), (5, 30), (90, 3)])
+@pytest.mark.parametrize("r", [1, 7, 8, 16, 17, 24, 32, 40, 64, 100, 256])
+def test_first_product_of_22_bits(hip, M, B, r):
+    """The adapters' part alone, whose terms cancel: as from a first product of 22 bits, not of the rows' own type."""
+    def edit(c):
+        c.w[:] = 0
+
+    say(f"lora first product of 22 bits M {M} B {B} r {r}")
+    c = LoraCase(hip, B, M, 136, 264, r, 5, bias=False, seed=r, edit=edit)
+    want, err = R.lora(c.x, c.w, c.bias, c.a, c.b, c.scale, c.idx, c.act, c.res)
+    for i, j in enumerate(c.idx):
+        if j >= 0:
+            t = np.abs(c.scale[j] * (c.x[i].astype(np.float64) @ c.a[j].astype(np.float64).T))
+            lost = (R.HU - 2.0 ** -22) * t + R.TINY - t.max(-1, keepdims=True) * 2.0 ** -38
+            err[i] -= 1.1 * lost @ np.abs(c.b[j].astype(np.float64)).T
+    assert (err >= 0).all()
+    near(c.run(), want, err, "22 bits", True)
