@@ -453,6 +453,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     __syncthreads();
     if (!s_bad) return C;
     if (at & 1) {
+      most = 0.f;
 #pragma unroll
       for (int t = 0; t < 2 * DKT; t++) S[t] = (v4f){0.f, 0.f, 0.f, 0.f};
     }

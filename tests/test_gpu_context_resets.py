@@ -69,3 +69,26 @@ def test_no_reset_keeps_nonfinite(hip, f16, T):
     s1 = c.ds1.numpy()
     assert not np.isfinite(s1[0, 1, 3, 5]) and not np.isfinite(s1[:, 0, 2, 7]).any()
     assert np.isfinite(s1[1, 1]).all() and np.isfinite(s1[:, 2]).all()
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("T,at", [(6, 3), (64, 32), (150, 64), (150, 100), (700, 299)])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_small_values_after_nonfinite(hip, f16, T, at, bad):
+    """An infinity that a reset has cleared leaves the small values after it their precision."""
+    def edit(c):
+        d = slice((c.hq + c.hk) * c.dk, None)
+        c.qkv[:, d] = (c.qkv[:, d].astype(np.float32) * 2e-4).astype(c.qkv.dtype)
+        c.qkv[at - 2, d] = bad
+        c.g[at] = -np.inf
+
+    say(f"la small after {bad} T {T} at {at} f16 {f16}")
+    c = LaCase(hip, [T], 2, 2, 2, 2, 32, 48, f16, gscale=0.1, seed=T + at, edit=edit)
+    c.run()
+    o, s1 = c.do.get()[0].reshape(c.rows, 2, 48)[at:T], c.ds1.numpy()
+    q, k, v = (z.reshape(-1, 2, d) for z, d in zip(np.split(c.qkv[at:T].astype(np.float64), [64, 128], 1), (32, 32, 48)))
+    wo, ws, eo, es, mo = R.linattn(q, k, v, c.g[at:T], c.scale, np.zeros((2, 32, 48)))
+    if f16:
+        eo = eo + 3 * HU * mo + 2.0 ** -20 * mo.max(-1, keepdims=True)
+    near(o, wo, eo, "o", f16)
+    near(s1[0], ws, es, "s")
