@@ -18,8 +18,10 @@ from . import hip
 
 class ContextNet:
     def __init__(self, dim=1536, heads=12, layers=2, stations=24, rank=16, seed=0):
-        if dim % heads or dim // heads > 256 or dim > 16384:
+        if heads < 1 or dim < 1 or dim % heads or dim // heads > 256 or dim > 16384:
             raise ValueError(f"dim {dim} is not {heads} heads of at most 256")
+        if layers < 1 or stations < 1 or not 1 <= rank <= 256:
+            raise ValueError(f"{layers} layers of {stations} stations' adapters of rank {rank}: one at least, rank up to 256")
         self.dim, self.heads, self.layers, self.stations, self.rank = dim, heads, layers, stations, rank
         rng = np.random.default_rng(seed)
 
