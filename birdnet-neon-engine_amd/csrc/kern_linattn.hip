@@ -169,8 +169,8 @@ int step_go(const LaDev &d, int B, bool vs, hipStream_t s) {
 // large, and g below -1e4 (whose e^g is 0) counts as -1e4, so that a reset's infinity does not cancel another's.
 //
 // A block of four or eight waves owns 64 or 128 columns of one state over one piece of one sequence. The state stays in the
-// accumulators of the waves (16 columns each, all of dk): their layout is, for pairs of 16-row tiles, that of the first operand of the
-// product with q's rows, so it never passes through LDS. q, k and v of the next chunk are loaded into registers while this
+// accumulators of the waves (16 columns each, all of dk): their layout is, for pairs of 16-row tiles, that of the first operand
+// of the product with q's rows, so it never passes through LDS. q, k and v of the next chunk are loaded into registers while this
 // one's are multiplied out of LDS; k's and v's transposes come out of LDS through ds_read_b64_tr_b16.
 //
 // fp16 rows: the factors of a product have to be fp16, its sums are fp32. Scores, the state and what is added to it go in as
@@ -178,13 +178,15 @@ int step_go(const LaDev &d, int B, bool vs, hipStream_t s) {
 // powers of two first (their largest to 2^12..2^13), so neither overflows. The state itself is not rounded: its update takes
 // v_j e^{c_C - c_j}, the largest of the chunk's by column scaled to 2^14..2^15 (the state's own unit from then on). With one
 // part for scores and state the outputs' relative error was 2.9e-4 instead of the 2.1e-4 of fp16 outputs as such, and several
-// times the outputs' own rounding where their terms cancel; the second parts cost 17 us of the 139 below, and 12 of the 136.
+// times the outputs' own rounding where their terms cancel; the second parts cost 17 us of the 141 below, and 12 of the 136.
 // fp32 rows run on the fp32 MFMA, unscaled and unsplit.
 //
-// 12 heads of 128 x 128 in fp16: 17,280 rows of one sequence 126 us (22 pieces of 13 chunks: what the pieces add 34, the
-// join 9, the outputs 78; 214 MB would take 42), 24 sequences of up to 720 rows 126 us. A chunk takes a block 12,000
-// cycles, 2,000 of them on the matrix cores: its phases (scores, state product, update, outputs) wait on LDS and on each
-// other, with two waves a SIMD at 219 registers; four waves of 128 registers spill and take 1.5 times as long.
+// 12 heads of 128 x 128 in fp16: 17,280 rows of one sequence 136 us (21 pieces of 13 chunks: what the pieces add 38, the
+// join 10, the outputs 89; 214 MB would take 42), 24 sequences of up to 720 rows 141 us. A chunk takes a block 12,000 to
+// 13,000 cycles, 2,000 of them on the matrix cores: its phases (scores, state product, update, outputs) wait on LDS and on
+// each other, with two waves a SIMD at 210 registers; four waves of 128 registers spill and take 1.5 times as long. The
+// blocks of an XCD are neighbours in the sequences' order (bnh_xcd_block): with sequences of unequal lengths that lie sorted,
+// as in the second of these, the XCD of the longest has 23 chunks one after another where an even spread would have 12.
 //
 // A row's v that is not finite would reach earlier rows of its chunk as 0 x inf; it is taken out of the product and added to
 // the rows that see it one by one (a wave that finds none skips this). A row that starts the state anew (e^g is 0) takes
@@ -534,7 +536,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
           }
           if (c == 0 || two) {
             *(FH *)(s_p[u] + i * SP + 32 * jj + 16 * c + 4 * q4) = y;
-            if constexpr (F16) *(uint64_t *)(s_l[u] + i * SP + 32 * jj + 16 * c + 4 * q4) = __builtin_bit_cast(uint64_t, z) & keep;
+            if constexpr (F16)
+              *(uint64_t *)(s_l[u] + i * SP + 32 * jj + 16 * c + 4 * q4) = __builtin_bit_cast(uint64_t, z) & keep;
           }
         }
       }
@@ -753,7 +756,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DKT <= 2 ? 4 : 1) void k
     float *w = part + pst + (long long)pc * (KD * DV) + wave * (KD * 16) + 4 * lane;
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++) *(v4f *)(w + 256 * t) = S[t];
-    if (wave == NW - 1 && lane == 0) pdec[(((long long)b * p.H + h) * nsl + sl) * (npc - 1) + pc] = anew ? -1.f : expf((float)ctot);
+    if (wave == NW - 1 && lane == 0)
+      pdec[(((long long)b * p.H + h) * nsl + sl) * (npc - 1) + pc] = anew ? -1.f : expf((float)ctot);
   } else if (p.s1 && slot >= 0 && r0 + pcr >= n) {
 #pragma unroll
     for (int t = 0; t < 2 * DKT; t++)
@@ -807,7 +811,8 @@ Plan plan(const bnh_la *p, int T, int B) {
   r.npc = 1;
   r.pcr = T;
   if (r.chunk) {
-    // as many blocks as the card holds at once: one a compute unit where a block's registers and LDS take half of it or more
+    // pieces for about as many blocks as the card holds at once (one a compute unit where a block's registers and LDS take half
+    // of it or more), rounded up to a whole number for each state
     long long want = bnh_ceil_div(p->f16 && r.dkt >= 4 ? 256 : 512, r.states);
     const long long most = bnh_ceil_div(T, 4 * r.c);
     if (want > most) want = most;
@@ -824,7 +829,8 @@ size_t plan_bytes(const Plan &r) {
 
 template <typename T, int DKT, int NW, int C, bool V>
 int chunk_run(LaDev d, const Plan &r, int B, void *work, hipStream_t s) {
-  float *part = (float *)work, *pdec = part ? (float *)((char *)work + bnh_round_up(4 * r.states * r.npc * r.floats, 256)) : nullptr;
+  float *part = (float *)work;
+  float *pdec = part ? (float *)((char *)work + bnh_round_up(4 * r.states * r.npc * r.floats, 256)) : nullptr;
   const dim3 block(64 * NW);
   if (r.npc > 1) {
     hipLaunchKernelGGL((k_la_chunk<T, DKT, NW, C, V, false>), dim3((unsigned)(r.states * (r.npc - 1))), block, 0, s, d, r.nsl,

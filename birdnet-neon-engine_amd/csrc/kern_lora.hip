@@ -4,16 +4,17 @@
 // Two launches. k_lora_down computes t = s_j A_j x for every row with an adapter, as two fp16 parts (22 bits): factors that
 // the matrix instruction of the second product takes. A row's t is scaled by a power of two first (its largest to 2^14..2^15),
 // so that it keeps them whatever its size; the row's product takes the unit back in fp32. Up to 16 ranks both parts fit
-// one matrix instruction, against b's ranks twice. k_lora_gemm computes W x on fp16 MFMA
-// with fp32 sums and adds the product of t with the adapter's B to the sums it has, so that the adapter costs no pass over
-// the output. Rows of one matrix instruction are independent of each other, so a block of 16 rows whose adapters differ
-// multiplies all of them by each of the adapters in it and every row keeps its own: nothing of another request's adapter,
-// not even an infinity or a NaN, reaches it. Up to 64 rows, where w's bytes are the bound, k_lora_few computes slices of
-// K beside the first products and k_lora_few_out adds them up.
+// one matrix instruction, against b's ranks twice. k_lora_gemm computes W x on fp16 MFMA with fp32 sums and adds the product
+// of t with the adapter's B to the sums it has, so that the adapter costs no pass over the output. Rows of one matrix
+// instruction are independent of each other, so a block of 16 rows whose adapters differ multiplies all of them by each of
+// the adapters in it and every row keeps its own: nothing of another request's adapter, not even an infinity or a NaN,
+// reaches it. Up to 64 rows, where w's bytes are the bound, k_lora_few computes slices of K beside the first products and
+// k_lora_few_out adds them up.
 //
-// Measured: 17,280 rows, K 1,536, N 6,144, rank 16 of 24 stations in 416 us (0.79 PFLOP/s; a library product of the same
-// size without adapters 350): k_lora_down 17, the rest k_lora_gemm, of which the adapters' products, an idx, t and b read
-// a tile, are 45. 24 rows of 24 stations, 1,536 x 1,536: 6.7 us and 5.3, the latencies of two short launches (w is 1 us).
+// Measured: 17,280 rows, K 1,536, N 6,144, rank 16 of 24 stations in 394 to 450 us by the card's clock (419: 0.79 PFLOP/s; a
+// library product of the same size without adapters 350): k_lora_down 18, the rest k_lora_gemm, of which the adapters'
+// products, an idx, t and b read a tile, are about 15 (394 with adapters and 361 without, on one card). 24 rows of 24
+// stations, 1,536 x 1,536: 7.1 us and 6.1, the latencies of two short launches (w is 1 us).
 #include <type_traits>
 
 #include "bnh_internal.h"
@@ -287,8 +288,8 @@ __device__ __forceinline__ void lora_tile(unsigned lb, int nm, int nn, int *tm, 
 // BM rows x BN channels a block of WM x WN waves. The operands' steps of BK values of K (a 128-byte line of each row: half
 // lines cost twice the L2 reads) pass through a ring of LDS stages that global loads fill directly (DMA: rows that are
 // 16-byte aligned), with one barrier a step; the loads are issued between the products, not in one go ahead of the
-// LDS reads. Without DMA through registers into two stages. A row's 16-byte chunks lie in LDS at chunk ^ f(row), so that the 16 rows of a
-// fragment's read fall on different banks (the loads write 16 bytes a lane in lane order, so the lane's chunk of the
+// LDS reads. Without DMA through registers into two stages. A row's 16-byte chunks lie in LDS at chunk ^ f(row), so that the
+// 16 rows of a fragment's read fall on different banks (the loads write 16 bytes a lane in lane order, so the lane's chunk of the
 // row is permuted instead). The first operand of the matrix instruction is the weights': a lane's accumulators are
 // four channels of one row.
 template <int BM, int BN, int WM, int WN, int BK, int RING, bool DMA, bool VR, bool VO>
@@ -565,8 +566,9 @@ int lora_tiles(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipS
   }
   return 0;
 }
-// Rows up to which w's bytes bound the product: 32 rows, 1,536 x 1,536 12.8 us and 25.8 on the tiles; 64 rows, 1,536 x 6,144
-// 19.9 and 26.2
+// Rows up to which the few-row form runs, for its four row tiles: 32 rows, 1,536 x 1,536 12.8 us and 25.8 on the tiles; 64 rows,
+// 1,536 x 6,144 19.9 and 26.2; 64 rows, 1,536 x 1,536 14.6, and 66 rows on the tiles 24.0. Where it would stop being the
+// faster one has not been measured: it is still ahead at 64.
 constexpr long long few = 64;
 // slices of K of the few-row form: two blocks a compute unit, and a step of 32 a wave at least
 long long few_slices(int N, int K) {
@@ -610,7 +612,8 @@ int lora_few(const LoraDev &p, const EpiDev &d, int dy, bool v, bool vr, bool vo
 // The largest tile that still gives every compute unit one: a large tile reads its operands from L2 and LDS less often.
 // Over 17,280 x 6,144 outputs and K 1,536 (no adapters) 256 x 192 takes 382 us, 128 x 128 398, 64 x 64 530; over 1,024 x
 // 6,144 40, 31 and 33 us; over 2,048 x 1,536 38, 26 and 18. Rows that are not 16-byte aligned pass through registers,
-// which the largest tile has none left for.
+// which the largest tile has none left for; it is not built for ranks that are no multiple of 8 either (rank 12 of the
+// first: 440 us on 128 x 128, 414 on 256 x 192).
 int lora_gemm(const LoraDev &p, const EpiDev &d, bool v, bool vr, bool vo, hipStream_t s) {
   if (v && vr && vo && bnh_ceil_div(p.rows, 256) * bnh_ceil_div(p.N, 192) >= 256)
     return lora_tiles<256, 192, 4, 2, 64, 2, false>(p, d, v, vr, vo, s);
