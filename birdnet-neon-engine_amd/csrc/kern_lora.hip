@@ -4,7 +4,8 @@
 // Two launches. k_lora_down computes t = s_j A_j x for every row with an adapter, as two fp16 parts (22 bits): factors that
 // the matrix instruction of the second product takes. A row's t is scaled by a power of two first (its largest to 2^14..2^15),
 // so that it keeps them whatever its size; the row's product takes the unit back in fp32. Up to 16 ranks both parts fit
-// one matrix instruction, against b's ranks twice. k_lora_gemm computes W x on fp16 MFMA with fp32 sums and adds the product
+// one matrix instruction, against b's ranks twice; more ranks take each product again (4,096 rows, 1,536 x 1,536, rank 64 63 us,
+// 57 with one part). k_lora_gemm computes W x on fp16 MFMA with fp32 sums and adds the product
 // of t with the adapter's B to the sums it has, so that the adapter costs no pass over the output. Rows of one matrix
 // instruction are independent of each other, so a block of 16 rows whose adapters differ multiplies all of them by each of
 // the adapters in it and every row keeps its own: nothing of another request's adapter, not even an infinity or a NaN,
