@@ -71,6 +71,26 @@ class LinAttn(C.Structure):
                 ("slot", vp)]
 
 
+class KvCache(C.Structure):
+    """bnh_kvcache: keys and values in pages."""
+    _fields_ = [("k", vp), ("v", vp), ("k_ps", i64), ("v_ps", i64),
+                ("f16", i32), ("pages", i32), ("page", i32), ("Hk", i32),
+                ("dk", i32), ("dv", i32), ("lo", vp), ("hi", vp),
+                ("table", vp), ("ldt", i32), ("past", vp)]
+
+
+class Rotary(C.Structure):
+    """bnh_rotary: the rotation of rows by their positions."""
+    _fields_ = [("rd", i32), ("pairs", i32), ("freq", vp), ("pos", vp)]
+
+
+class KvAttn(C.Structure):
+    """bnh_kvattn: attention over a paged cache, or its pages' selection."""
+    _fields_ = [("q", vp), ("ldq", i32), ("o", vp), ("ldo", i32), ("H", i32),
+                ("scale", C.c_float), ("window", i32), ("sel", vp),
+                ("nsel", i32)]
+
+
 _SIGS = {
     "bnh_last_error": (C.c_char_p, []),
     "bnh_device_count": (i32, []),
@@ -187,6 +207,12 @@ _SIGS = {
                           C.c_size_t, vp]),
     "bnh_linattn_work_bytes": (C.c_size_t, [C.POINTER(LinAttn), i32, i32]),
     "bnh_linattn": (i32, [C.POINTER(LinAttn), i32, i32, i32, vp, vp, vp, C.c_size_t, vp]),
+    "bnh_kv_append": (i32, [C.POINTER(KvCache), C.POINTER(Rotary), vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32,
+                            vp, vp, vp]),
+    "bnh_kv_attn_work_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvAttn), i32, i32, i32]),
+    "bnh_kv_attn": (i32, [C.POINTER(KvCache), C.POINTER(KvAttn), i32, i32, i32, vp, vp, vp, C.c_size_t, vp]),
+    "bnh_kv_select_work_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvAttn), i32, i32, i32]),
+    "bnh_kv_select": (i32, [C.POINTER(KvCache), C.POINTER(KvAttn), i32, i32, i32, i32, i32, vp, vp, vp, C.c_size_t, vp]),
 }
 
 

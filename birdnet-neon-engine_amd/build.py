@@ -35,6 +35,8 @@ SOURCES = [
     "kern_bnorm.hip",
     "kern_lora.hip",
     "kern_linattn.hip",
+    "kern_kv.hip",
+    "kern_kvattn.hip",
     "pkg_file.cpp",
     "rt_contract.cpp",
     "rt_pkg.cpp",

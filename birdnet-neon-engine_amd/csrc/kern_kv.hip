@@ -1,0 +1,416 @@
+// New rows into a paged cache with their rotation (bnh_kv_append), and the pages that rows look at by the pages' bounds
+// (bnh_kv_select).
+#include <float.h>
+
+#include "bnh_kv.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------- append
+// Bound by HBM: q, k and v are read once and written once. A block owns the new rows of one page for one head of keys, with the
+// query heads that read it, so that the page's bounds need no atomics: its threads are `nu` units of a head (VEC values,
+// with their partners VEC more) side by side, times as many rows as fit 256.
+struct AppDev {
+  const void *k, *v, *q;
+  void *qr;
+  const float *freq;
+  const int32_t *pos;
+  int ldk, ldv, ldq, ldr, G, rd, pairs;
+};
+
+// cos and sin of pos freq: the angle in turns in 64 bits, reduced to [-1/8, 1/8] of one about the nearest quarter, where the
+// series of sin and cos up to x^9 and x^10 are within 2e-9
+__device__ __forceinline__ void turn(int pos, float freq, float *cs, float *sn) {
+  const double t = (double)pos * (double)freq * 0.63661977236758134308;  // quarters: 2 / pi
+  const double n = __builtin_rint(t);
+  const float x = (float)((t - n) * 1.57079632679489661923), y = x * x;
+  float s = __builtin_fmaf(y, 2.7557319e-6f, -1.9841270e-4f);
+  s = __builtin_fmaf(y, s, 8.3333333e-3f);
+  s = __builtin_fmaf(y, s, -1.6666667e-1f);
+  s = __builtin_fmaf(x * y, s, x);
+  float c = __builtin_fmaf(y, -2.7557319e-7f, 2.4801587e-5f);
+  c = __builtin_fmaf(y, c, -1.3888889e-3f);
+  c = __builtin_fmaf(y, c, 4.1666667e-2f);
+  c = __builtin_fmaf(y, c, -0.5f);
+  c = __builtin_fmaf(y, c, 1.f);
+  const int k = (int)((long long)n & 3);
+  const float a = k & 1 ? s : c, b = k & 1 ? c : s;
+  *cs = k == 1 || k == 2 ? -a : a;
+  *sn = k >= 2 ? -b : b;
+}
+// the smaller and the larger of two, NaN where one is
+template <typename T>
+__device__ __forceinline__ T low(T a, T b) { return a != a ? a : b != b ? b : a < b ? a : b; }
+template <typename T>
+__device__ __forceinline__ T high(T a, T b) { return a != a ? a : b != b ? b : a > b ? a : b; }
+
+// A unit: VEC values at `a` and VEC more at `b` (pairs 0: the partners; pairs 1 and values past rd: the next ones)
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, int nu, long long blk0) {
+  typedef T W __attribute__((ext_vector_type(VEC), aligned(sizeof(T) * VEC)));
+  __shared__ T s_lo[512 * VEC], s_hi[512 * VEC];
+  const long long blk = blk0 + blockIdx.x;
+  const int g = (int)(blk % c.Hk), pt = (int)(blk / c.Hk % npt), b = (int)(blk / c.Hk / npt);
+  int first, past;
+  const int n = kv_rows(c, b, &first, &past);
+  const int pi = (past >> c.sh) + pt;                   // the sequence's page
+  const long long p0 = (long long)pi << c.sh, p1 = p0 + (1 << c.sh);
+  if (n == 0 || (pt && p0 - past >= n)) return;
+  const int t0 = pt ? (int)(p0 - past) : 0, t1 = n < p1 - past ? n : (int)(p1 - past);  // its rows
+  const int page = kv_page(c, b, pi);
+  const int off = (int)(past + t0 - p0);             // the first one's place in the page
+  const int tid = threadIdx.x, u = tid % nu, rl = tid / nu, RL = 256 / nu;
+  // the unit's values of a head
+  const int half = p.rd / 2, nr = p.pairs ? 0 : (half + VEC - 1) / VEC;  // units of partners
+  const bool apart = u < nr;                                             // VEC values and their partners
+  const int rest = p.pairs ? 0 : p.rd;                                   // then pairs of VEC side by side from here
+  const int a = apart ? u * VEC : rest + 2 * (u - nr) * VEC, bb = apart ? a + half : a + VEC;
+  const int na = apart ? half : c.dk, nb = apart ? p.rd : c.dk;          // where the values end
+  W lo[2], hi[2];
+#pragma unroll
+  for (int i = 0; i < VEC; i++) lo[0][i] = lo[1][i] = (T)INFINITY, hi[0][i] = hi[1][i] = (T)-INFINITY;
+  T *kc = (T *)c.k + (page < 0 ? 0 : page * c.k_ps + ((long long)g << c.sh) * c.dk);
+  if (rl < RL) {
+    for (int t = t0 + rl; t < t1; t += RL) {
+      const long long r = (long long)first + t;
+      float cs[VEC], sn[VEC];
+      const int pos = p.pos ? p.pos[r] : past + t;
+      // pairs: a unit of 2 VEC values has VEC pairs, value 2 i of the two vectors with value 2 i + 1
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        const int e = apart ? a + i : a / 2 + i;
+        cs[i] = 1.f, sn[i] = 0.f;
+        if (p.rd && (apart || p.pairs) && e < half) turn(pos, p.freq[e], &cs[i], &sn[i]);
+      }
+      auto rotate = [&](const T *src, T *dst, bool bound) {
+        W x[2];
+        if (VEC > 1) {
+          x[0] = *(const W *)(src + a), x[1] = *(const W *)(src + bb);
+        } else {
+          x[0][0] = a < na ? src[a] : (T)0, x[1][0] = bb < nb ? src[bb] : (T)0;
+        }
+        if (apart) {
+#pragma unroll
+          for (int i = 0; i < VEC; i++) {
+            const float y = (float)x[0][i], z = (float)x[1][i];
+            x[0][i] = (T)__builtin_fmaf(y, cs[i], -(z * sn[i]));
+            x[1][i] = (T)__builtin_fmaf(y, sn[i], z * cs[i]);
+          }
+        } else if (p.pairs && a < p.rd) {
+          T w[2 * VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; i++) w[i] = x[0][i], w[VEC + i] = x[1][i];
+#pragma unroll
+          for (int i = 0; i < VEC; i++) {
+            if (a + 2 * i >= p.rd) continue;
+            const float y = (float)w[2 * i], z = (float)w[2 * i + 1];
+            w[2 * i] = (T)__builtin_fmaf(y, cs[i], -(z * sn[i]));
+            w[2 * i + 1] = (T)__builtin_fmaf(y, sn[i], z * cs[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < VEC; i++) x[0][i] = w[i], x[1][i] = w[VEC + i];
+        }
+        if (VEC > 1) {
+          *(W *)(dst + a) = x[0], *(W *)(dst + bb) = x[1];
+        } else {
+          if (a < na) dst[a] = x[0][0];
+          if (bb < nb) dst[bb] = x[1][0];
+        }
+        if (bound) {
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) lo[j][i] = low(lo[j][i], x[j][i]), hi[j][i] = high(hi[j][i], x[j][i]);
+        }
+      };
+      if (page >= 0) rotate((const T *)p.k + r * p.ldk + g * c.dk, kc + (long long)(off + t - t0) * c.dk, c.lo != nullptr);
+      if (p.q)
+        for (int h = g * p.G; h < (g + 1) * p.G; h++)
+          rotate((const T *)p.q + r * p.ldq + (long long)h * c.dk, (T *)p.qr + r * p.ldr + (long long)h * c.dk, false);
+    }
+  }
+  if (page < 0) return;
+  // values as they are
+  T *vc = (T *)c.v + page * c.v_ps + (((long long)g << c.sh) + off) * c.dv;
+  const int nv = c.dv / VEC, items = (t1 - t0) * nv;
+  for (int i = tid; i < items; i += 256) {
+    const int t = i / nv, e = (i - t * nv) * VEC;
+    *(W *)(vc + (long long)t * c.dv + e) = *(const W *)((const T *)p.v + ((long long)first + t0 + t) * p.ldv + g * c.dv + e);
+  }
+  if (!c.lo) return;
+  if (rl < RL) {
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {  // [rl][value]; values past the unit's end are nobody's
+      if (a + i < na) s_lo[rl * c.dk + a + i] = lo[0][i], s_hi[rl * c.dk + a + i] = hi[0][i];
+      if (bb + i < nb) s_lo[rl * c.dk + bb + i] = lo[1][i], s_hi[rl * c.dk + bb + i] = hi[1][i];
+    }
+  }
+  __syncthreads();
+  if (tid < c.dk) {
+    const long long at = ((long long)page * c.Hk + g) * c.dk + tid;
+    T l = s_lo[tid], h = s_hi[tid];
+    const int used = RL < t1 - t0 ? RL : t1 - t0;
+    for (int i = 1; i < used; i++) l = low(l, s_lo[i * c.dk + tid]), h = high(h, s_hi[i * c.dk + tid]);
+    if (off) l = low(l, ((const T *)c.lo)[at]), h = high(h, ((const T *)c.hi)[at]);
+    ((T *)c.lo)[at] = l, ((T *)c.hi)[at] = h;
+  }
+}
+
+template <typename T, int VEC>
+int append_run(const KvDev &c, const AppDev &p, int B, hipStream_t s) {
+  const int npt = (int)(((long long)c.T + (1 << c.sh) - 2) >> c.sh) + 1;  // pages that T rows can touch
+  const int half = p.rd / 2, nr = p.pairs ? 0 : (half + VEC - 1) / VEC, left = c.dk - (p.pairs ? 0 : p.rd);
+  const int nu = nr + (left + 2 * VEC - 1) / (2 * VEC);
+  const long long blocks = (long long)B * npt * c.Hk, most = bnh_most_blocks(256);
+  for (long long b0 = 0; b0 < blocks; b0 += most) {
+    hipLaunchKernelGGL((k_kv_append<T, VEC>), dim3((unsigned)(blocks - b0 < most ? blocks - b0 : most)), dim3(256), 0, s, c, p,
+                       npt, nu, b0);
+    BNH_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------- select
+// A score's order as a whole number: larger for larger scores, 0 for a page that is not to be had
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 order_of(double x) {
+  if (x != x) x = -INFINITY;
+  const u64 b = (u64)__double_as_longlong(x == 0 ? 0.0 : x);  // -0 is 0
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+struct SelDev {
+  const void *q;
+  int32_t *sel;
+  int ldq, H, G, window, nsel, first, last;
+};
+// the row's place: its sequence's pages [lo, hi) have a token that it may see. Rows of a launch are numbered b T + t
+__device__ __forceinline__ bool sel_row(const KvDev &c, const SelDev &p, long long i, int *b, long long *row, int *lo, int *hi) {
+  *b = (int)(i / c.T);
+  const int t = (int)(i % c.T);
+  int first, past;
+  const int n = kv_rows(c, *b, &first, &past);
+  if (t >= n) return false;
+  *row = (long long)first + t;
+  const int at = past + t;
+  *lo = p.window && at >= p.window ? (at - p.window + 1) >> c.sh : 0;
+  const int h = (at >> c.sh) + 1;
+  *hi = h;
+  return true;
+}
+
+// The scores of PPB pages for one row and head of keys: 16 lanes a page, 8 values each a step. Bound by reading the bounds
+// (4 dk bytes a page and head in fp16); the products are exact in 64 bits and their sums good to 2^-50, so that no order of
+// sums can make another choice.
+constexpr int PPB = 64;
+template <typename T, bool V>
+__global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, long long row0, u64 *key) {
+  __shared__ __attribute__((aligned(16))) float s_q[16 * 256];  // up to 16 query heads at a time
+  const int pb = (int)(blockIdx.x % npb), g = (int)(blockIdx.x / npb % c.Hk);
+  const long long i = blockIdx.x / ((long long)npb * c.Hk);
+  int b, lo, hi;
+  long long row;
+  if (!sel_row(c, p, row0 + i, &b, &row, &lo, &hi)) return;
+  const int cur = hi - 1, end = hi < c.ldt ? hi : c.ldt;
+  const int tid = threadIdx.x, l = tid & 15, team = tid >> 4;
+  if (pb * PPB >= end) return;
+  u64 *out = key + (i * c.Hk + g) * c.ldt;
+  const int kd = (c.dk + 127) / 128 * 128;
+  double acc[PPB / 16];
+#pragma unroll
+  for (int j = 0; j < PPB / 16; j++) acc[j] = 0;
+  for (int h0 = 0; h0 < p.G; h0 += 16) {
+    const int nh = p.G - h0 < 16 ? p.G - h0 : 16;
+    if (h0) __syncthreads();
+    for (int x = tid; x < nh * kd; x += 256) {
+      const int h = x / kd, d = x - h * kd;
+      s_q[x] = d < c.dk ? (float)((const T *)p.q)[row * p.ldq + (long long)(g * p.G + h0 + h) * c.dk + d] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PPB / 16; j++) {
+      const int pi = pb * PPB + 16 * j + team;
+      const int page = pi >= lo && pi < end ? kv_page(c, b, pi) : -1;
+      if (page < 0) continue;
+      const T *pl = (const T *)c.lo + ((long long)page * c.Hk + g) * c.dk;
+      const T *ph = (const T *)c.hi + ((long long)page * c.Hk + g) * c.dk;
+      for (int d0 = 0; d0 < kd; d0 += 128) {
+        const int d = d0 + 8 * l;
+        const kv_vec<T, 8> xl = kv_ld<T, 8, V>(pl, d, c.dk), xh = kv_ld<T, 8, V>(ph, d, c.dk);
+        for (int h = 0; h < nh; h++) {
+          const float4 q0 = *(const float4 *)(s_q + h * kd + d), q1 = *(const float4 *)(s_q + h * kd + d + 4);
+          const float q[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            acc[j] = __builtin_fma((double)q[e], (double)(float)(q[e] >= 0.f ? xh[e] : xl[e]), acc[j]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PPB / 16; j++) {
+    const int pi = pb * PPB + 16 * j + team;
+    if (pi >= end) continue;
+    double x = acc[j];
+#pragma unroll
+    for (int m = 1; m < 16; m *= 2) x += __shfl_xor(x, m);
+    const bool there = pi >= lo && kv_page(c, b, pi) >= 0;
+    if (l == 0) out[pi] = !there ? 0 : order_of(pi < p.first || pi > cur - p.last ? (double)INFINITY : x);
+  }
+}
+
+// The nsel largest of a row's keys by their digits of 8 bits from the top, the lower pages first where the last of them are
+// equal, in ascending order
+__global__ __launch_bounds__(256) void k_kv_pick(KvDev c, SelDev p, long long row0, const u64 *key) {
+  __shared__ int s_n[256], s_w[4], s_t[4], s_b[3];
+  const int g = (int)(blockIdx.x % c.Hk);
+  const long long i = blockIdx.x / c.Hk;
+  int b, lo, hi;
+  long long row;
+  if (!sel_row(c, p, row0 + i, &b, &row, &lo, &hi)) return;
+  const int end = hi < c.ldt ? hi : c.ldt;
+  const u64 *k = key + (i * c.Hk + g) * c.ldt;
+  int32_t *out = p.sel + (row * c.Hk + g) * p.nsel;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  u64 prefix = 0, mask = 0;
+  int need = p.nsel;  // of the keys that agree with the prefix
+  bool all = false;   // all of those are taken
+  for (int shift = 56; shift >= 0 && !all; shift -= 8) {
+    s_n[tid] = 0;
+    __syncthreads();
+    for (int x = lo + tid; x < end; x += 256) {
+      const u64 y = k[x];
+      if (y && (y & mask) == prefix) atomicAdd(&s_n[y >> shift & 255], 1);
+    }
+    __syncthreads();
+    // keys in this digit and above: a suffix sum over 256 digits
+    const int n = s_n[tid];
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_down(sum, d);
+      sum += lane + d < 64 ? o : 0;
+    }
+    if (lane == 0) s_w[wave] = sum;
+    __syncthreads();
+    for (int w = wave + 1; w < 4; w++) sum += s_w[w];
+    // the digit that the last one needed has: above it fewer than need, with it need or more
+    if (tid == 0) s_b[0] = -1, s_b[2] = sum;
+    __syncthreads();
+    if (sum >= need && sum - n < need) s_b[0] = tid, s_b[1] = sum - n;
+    __syncthreads();
+    if (s_b[0] < 0) {  // fewer than need in all
+      need = s_b[2];
+      all = true;
+    } else {
+      prefix |= (u64)s_b[0] << shift;
+      mask |= 255ull << shift;
+      need -= s_b[1];
+      all = s_n[s_b[0]] == need;
+    }
+    __syncthreads();
+  }
+  // taken: above the prefix, or, in order, the first `need` that agree with it
+  int done = 0, ties = 0;
+  for (int x0 = lo; x0 < end; x0 += 256) {
+    const int x = x0 + tid;
+    const u64 y = x < end ? k[x] : 0;
+    const bool above = y && (y & mask) > prefix, tie = y && (y & mask) == prefix;
+    const u64 bt = __ballot(tie);
+    if (lane == 0) s_t[wave] = __popcll(bt);
+    __syncthreads();
+    int rank = ties + __popcll(bt & ((1ull << lane) - 1));
+    for (int w = 0; w < wave; w++) rank += s_t[w];
+    const bool take = above || (tie && rank < need);
+    const u64 bk = __ballot(take);
+    if (lane == 0) s_w[wave] = __popcll(bk);
+    __syncthreads();
+    int at = done + __popcll(bk & ((1ull << lane) - 1));
+    for (int w = 0; w < wave; w++) at += s_w[w];
+    if (take) out[at] = x;
+    done += s_w[0] + s_w[1] + s_w[2] + s_w[3];
+    ties += s_t[0] + s_t[1] + s_t[2] + s_t[3];
+    __syncthreads();
+  }
+  for (int x = done + tid; x < p.nsel; x += 256) out[x] = -1;
+}
+
+// rows of a launch: the scores of 64 MB at most, or of one row
+long long select_rows(const bnh_kvcache *c, int T, int B) {
+  const long long per = 8LL * c->Hk * c->ldt, n = (64LL << 20) / per, all = (long long)T * B;
+  return n < 1 ? 1 : n < all ? n : all;
+}
+
+int select_check(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows) {
+  if (kv_check(c, T, B, rows)) return -1;
+  BNH_REQ(p && p->H > 0 && p->H % c->Hk == 0 && p->H <= 65536 && p->nsel > 0 && p->nsel <= (1 << 20) && p->window >= 0);
+  BNH_REQ((long long)rows * c->Hk < (1LL << 31));
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bnh_kv_append(const bnh_kvcache *c, const bnh_rotary *r, const void *k, int ldk, const void *v, int ldv, const void *q,
+                  int ldq, void *qr, int ldr, int H, int T, int B, int rows, const int32_t *start, const int32_t *len,
+                  void *stream) {
+  if (kv_check(c, T, B, rows) || kv_check_buffers(c, T, B, rows, start, len)) return -1;
+  BNH_REQ(k && v && ldk >= c->Hk * c->dk && ldv >= c->Hk * c->dv);
+  BNH_REQ(!q == !qr);
+  BNH_REQ(!q || (H > 0 && H <= 65536 && H % c->Hk == 0 && ldq >= H * c->dk && ldr >= H * c->dk && (q != qr || ldq == ldr)));
+  BNH_REQ(!r || (r->rd >= 0 && r->rd <= c->dk && r->rd % 2 == 0 && (r->pairs == 0 || r->pairs == 1) && (!r->rd || r->freq)));
+  const size_t es = c->f16 ? 2 : 4;
+  BNH_REQ(kv_on(k, es) && kv_on(v, es) && kv_on(q, es) && kv_on(qr, es));
+  BNH_REQ(!r || (kv_on(r->freq, 4) && kv_on(r->pos, 4)));
+  const KvDev d = kv_dev(c, T, rows, start, len);
+  const int rd = r ? r->rd : 0, pairs = r ? r->pairs : 0, ve = 16 / (int)es;
+  const AppDev p = {k, v, q, qr, r ? r->freq : nullptr, r ? r->pos : nullptr, ldk, ldv, ldq, ldr, q ? H / c->Hk : 0, rd, pairs};
+  bool vec = c->dk % (2 * ve) == 0 && c->dv % ve == 0 && rd % (2 * ve) == 0 && c->k_ps % ve == 0 && c->v_ps % ve == 0;
+  for (const void *x : {(const void *)c->k, (const void *)c->v, k, v, q, (const void *)qr}) vec = vec && kv_on(x, 16);
+  vec = vec && ldk % ve == 0 && ldv % ve == 0 && (!q || (ldq % ve == 0 && ldr % ve == 0));
+  hipStream_t s = bnh_stream(stream);
+  if (c->f16) return vec ? append_run<h16, 8>(d, p, B, s) : append_run<h16, 1>(d, p, B, s);
+  return vec ? append_run<float, 4>(d, p, B, s) : append_run<float, 1>(d, p, B, s);
+}
+
+size_t bnh_kv_select_work_bytes(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows) {
+  if (select_check(c, p, T, B, rows)) return 0;
+  return (size_t)(select_rows(c, T, B) * c->Hk * c->ldt * 8);
+}
+
+int bnh_kv_select(const bnh_kvcache *c, const bnh_kvattn *p, int first, int last, int T, int B, int rows,
+                  const int32_t *start, const int32_t *len, void *work, size_t work_bytes, void *stream) {
+  if (select_check(c, p, T, B, rows) || kv_check_buffers(c, T, B, rows, start, len)) return -1;
+  BNH_REQ(c->lo && p->q && p->sel && p->ldq >= p->H * c->dk && first >= 0 && last >= 0 && first <= p->nsel - last);
+  const size_t es = c->f16 ? 2 : 4;
+  BNH_REQ(kv_on(p->q, es) && kv_on(p->sel, 4));
+  const long long per = select_rows(c, T, B), all = (long long)T * B;
+  BNH_REQ(work && kv_on(work, 16) && work_bytes >= (size_t)(per * c->Hk * c->ldt * 8));
+  const KvDev d = kv_dev(c, T, rows, start, len);
+  const SelDev e = {p->q, p->sel, p->ldq, p->H, p->H / c->Hk, p->window, p->nsel, first, last};
+  const bool v = c->dk % 8 == 0 && kv_on(c->lo, 16) && kv_on(c->hi, 16);
+  const int npb = (int)bnh_ceil_div(c->ldt, PPB);
+  // rows of a launch also by its blocks
+  long long most = bnh_most_blocks(256) / ((long long)npb * c->Hk);
+  BNH_REQ(most > 0);
+  if (most > per) most = per;
+  hipStream_t s = bnh_stream(stream);
+  for (long long r0 = 0; r0 < all; r0 += most) {
+    const long long n = all - r0 < most ? all - r0 : most;
+    const dim3 grid((unsigned)(n * npb * c->Hk)), block(256);
+    u64 *key = (u64 *)work;
+    if (c->f16) {
+      if (v) hipLaunchKernelGGL((k_kv_score<h16, true>), grid, block, 0, s, d, e, npb, r0, key);
+      else hipLaunchKernelGGL((k_kv_score<h16, false>), grid, block, 0, s, d, e, npb, r0, key);
+    } else {
+      if (v) hipLaunchKernelGGL((k_kv_score<float, true>), grid, block, 0, s, d, e, npb, r0, key);
+      else hipLaunchKernelGGL((k_kv_score<float, false>), grid, block, 0, s, d, e, npb, r0, key);
+    }
+    BNH_HIP(hipGetLastError());
+    hipLaunchKernelGGL(k_kv_pick, dim3((unsigned)(n * c->Hk)), block, 0, s, d, e, r0, key);
+    BNH_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // extern "C"

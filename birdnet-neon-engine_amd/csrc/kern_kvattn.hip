@@ -1,0 +1,464 @@
+// Attention of new rows over a paged cache of keys and values (bnh_kv_attn): per row and head, over the tokens j that the row
+// sees,
+//   s_j = scale q . k_j,  o = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},  m = max_j s_j,
+// in one pass over the keys with the running m and sum, both in fp32 and base 2.
+#include <math.h>
+
+#include "bnh_kv.h"
+
+namespace {
+
+struct AttnDev {
+  const void *q;
+  void *o;
+  const int32_t *sel;
+  int ldq, ldo, G, window, nsel;  // G: query heads that share one of keys
+  float sc;                       // scale log2(e)
+};
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef h16 v8h __attribute__((ext_vector_type(8)));
+template <typename T>
+using vec8 = T __attribute__((ext_vector_type(8)));
+// 32 steps of a product: 8 of row (or column) lane & 15 in a lane, the same 8 of both operands
+__device__ __forceinline__ v4f mma(kv_vec<h16, 8> a, kv_vec<h16, 8> b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mma(kv_vec<float, 8> a, kv_vec<float, 8> b, v4f c) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+template <typename T>
+__device__ __forceinline__ bool finite(T x) { return x - x == (T)0; }
+
+// A tile of rows: MR rows and query heads of one sequence and head of keys, heads innermost; with a selection, heads of one row
+struct Tile {
+  int t0, t1;  // its first and last row
+};
+__device__ __forceinline__ void tile_row(const AttnDev &p, int tile, int m, int MR, int *t, int *h) {
+  if (p.sel) {
+    const int ht = (p.G + MR - 1) / MR;
+    *t = tile / ht;
+    *h = tile % ht * MR + m;
+    if (*h >= p.G) *t = 0x7fffffff;  // nobody's
+  } else {
+    const long long x = (long long)tile * MR + m;
+    *t = (int)(x / p.G);
+    *h = (int)(x % p.G);
+  }
+}
+
+// The streaming form, for few rows, for fp32 and for widths that the tiled form does not take: bound by reading keys and values
+// where rows are few. Four waves of a block take tiles of 32 tokens in turn, straight from memory into the matrix
+// instructions' registers: the scores' product has keys as its rows in such an order that a lane ends with the scores of 8 tokens
+// in a row, 8 q4 .. 8 q4 + 7 (q4 = lane / 16), for query lane & 15, which is what the second product's operand holds; values are
+// loaded as 8 tokens by CPL columns a lane and change places within the lane. Each wave has its own maximum and sums, joined at
+// the end over waves, and over the blocks of a split by k_kva_join. fp16: e^{s - m} goes into the product in two parts, 22 bits,
+// in units of 2^-12 so that the second part of small ones is no subnormal: the matrix cores wait for memory here.
+template <typename T, int D, int MT, bool V>
+__global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int nsp, long long blk0, float *part, float2 *pml) {
+  constexpr bool F16 = sizeof(T) == 2;
+  constexpr int DKT = D / 32, CPL = D / 16, MR = 16 * MT;
+  constexpr float OFF = F16 ? 12.f : 0.f;
+  typedef kv_vec<T, 8> FV;
+  __shared__ __attribute__((aligned(16))) float s_o[4][16 * (D + 4)];
+  __shared__ float s_m[4][MR], s_l[4][MR];
+  const long long blk = blk0 + blockIdx.x, unit = blk / nsp;
+  const int sp = (int)(blk % nsp), tile = (int)(unit % nrt), g = (int)(unit / nrt % c.Hk), b = (int)(unit / nrt / c.Hk);
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int first, past, t0, t1, hx;
+  const int n = kv_rows(c, b, &first, &past);
+  tile_row(p, tile, 0, MR, &t0, &hx);
+  if (t0 >= n) return;
+  if (p.sel) t1 = t0;
+  else tile_row(p, tile, MR - 1, MR, &t1, &hx);
+  t1 = t1 < n ? t1 : n - 1;
+  // queries
+  FV qf[MT][DKT];
+  int at[MT], since[MT];  // the last token that the lane's query sees, and the first
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    int t, h;
+    tile_row(p, tile, 16 * m + lr, MR, &t, &h);
+    const bool in = t < n;
+    at[m] = in ? past + t : -1;
+    since[m] = p.window && at[m] >= p.window ? at[m] - p.window + 1 : 0;
+    const T *q = (const T *)p.q + ((long long)first + (in ? t : t0)) * p.ldq + ((long long)g * p.G + (in ? h : 0)) * c.dk;
+#pragma unroll
+    for (int d = 0; d < DKT; d++) qf[m][d] = kv_ld<T, 8, V>(q, 32 * d + 8 * q4, in ? c.dk : 0);
+  }
+  // tokens
+  const int all0 = p.window && past + t1 >= p.window ? past + t1 - p.window + 1 : 0;  // from here and ..
+  const int all1 = past + t0;                                                         // .. up to here every query sees them
+  const long long cap = ((long long)c.ldt << c.sh) - 1;
+  const int j0 = p.window && past + t0 >= p.window ? past + t0 - p.window + 1 : 0, j1 = past + t1 < cap ? past + t1 : (int)cap;
+  const int base = j0 >> 5;
+  const int *sel = p.sel ? p.sel + (((long long)first + t0) * c.Hk + g) * p.nsel : nullptr;
+  const int nt = p.sel ? (int)((((long long)p.nsel << (c.sh - 4)) + 1) >> 1) : j1 < j0 ? 0 : (j1 >> 5) - base + 1;
+  const int per = (nt + nsp - 1) / nsp, kt0 = sp * per, kt1 = kt0 + per < nt ? kt0 + per : nt;
+
+  v4f o[MT][CPL];
+  float mx[MT], l[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    mx[m] = -INFINITY, l[m] = 0.f;
+#pragma unroll
+    for (int i = 0; i < CPL; i++) o[m][i] = (v4f){0.f, 0.f, 0.f, 0.f};
+  }
+  // the first tokens of a tile's two groups of 16, and their pages (-1: not there)
+  auto look = [&](int kt, int (&j)[2], int (&pg)[2]) {
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      if (s == 1 && c.sh > 4) {
+        j[1] = j[0] + 16, pg[1] = pg[0];
+        break;
+      }
+      pg[s] = -1, j[s] = 0;
+      if (kt >= kt1) continue;
+      int pi;
+      if (p.sel) {
+        const int x = 2 * kt + s, e = x >> (c.sh - 4);
+        if (e >= p.nsel) continue;
+        pi = sel[e];
+        if (pi < 0 || pi >= c.ldt || (e > 0 && pi <= sel[e - 1])) continue;
+        j[s] = (pi << c.sh) + ((x & ((1 << (c.sh - 4)) - 1)) << 4);
+      } else {
+        j[s] = 32 * (base + kt) + 16 * s;
+        pi = j[s] >> c.sh;
+      }
+      pg[s] = kv_page(c, b, pi);
+    }
+  };
+  int jn[2], pn[2];
+  look(kt0 + wave, jn, pn);
+  for (int kt = kt0 + wave; kt < kt1; kt += 4) {
+    int j[2] = {jn[0], jn[1]}, pg[2] = {pn[0], pn[1]};
+    look(kt + 4, jn, pn);
+    if (pg[0] < 0 && pg[1] < 0) continue;
+    const bool full = pg[0] >= 0 && pg[1] >= 0 && j[0] >= all0 && j[1] >= all0 && j[0] + 15 <= all1 && j[1] + 15 <= all1;
+    const T *kb[2], *vb[2];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {  // one that is not there is read where the other is
+      const int x = pg[s] < 0 ? 1 - s : s;
+      const long long in = ((long long)g << c.sh) + (j[x] & ((1 << c.sh) - 1));
+      kb[s] = (const T *)c.k + pg[x] * c.k_ps + in * c.dk;
+      vb[s] = (const T *)c.v + pg[x] * c.v_ps + in * c.dv;
+    }
+    const T *kp = (lr & 8 ? kb[1] : kb[0]) + (8 * (lr >> 2 & 1) + (lr & 3)) * c.dk;
+    const T *vp = (q4 & 2 ? vb[1] : vb[0]) + 8 * (q4 & 1) * c.dv;
+    FV kf[2][DKT];
+    kv_vec<T, CPL> vr[8];
+#pragma unroll
+    for (int d = 0; d < DKT; d++) {
+      kf[0][d] = kv_ld<T, 8, V>(kp, 32 * d + 8 * q4, c.dk);
+      kf[1][d] = kv_ld<T, 8, V>(kp + 4 * c.dk, 32 * d + 8 * q4, c.dk);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) vr[e] = kv_ld<T, CPL, V>(vp + e * c.dv, CPL * lr, c.dv);
+    v4f s[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; m++) s[m][0] = s[m][1] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DKT; d++)
+#pragma unroll
+      for (int m = 0; m < MT; m++) s[m][0] = mma(kf[0][d], qf[m][d], s[m][0]), s[m][1] = mma(kf[1][d], qf[m][d], s[m][1]);
+    const int jl = (q4 & 2 ? j[1] : j[0]) + 8 * (q4 & 1);  // the lane's 8 tokens
+    const bool there = (q4 & 2 ? pg[1] : pg[0]) >= 0;
+    // a value is not finite, in a tile that not every query sees all of, or one whose factors are in two parts (an infinity times
+    // a second part of 0 or of the other sign)
+    bool odd = false;
+    if constexpr (F16) {
+      typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+      u2 most = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int i = 0; i < CPL; i += 2)
+          most = __builtin_elementwise_max(most, (u2){hbits(vr[e][i]), hbits(vr[e][i + 1])} & (u2){0x7fff, 0x7fff});
+      odd = most[0] >= 0x7c00 || most[1] >= 0x7c00;
+    } else if (!full) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int i = 0; i < CPL; i++) odd = odd || !finite(vr[e][i]);
+    }
+    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    if (odd)
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int i = 0; i < CPL; i++) vr[e][i] = finite(vr[e][i]) ? vr[e][i] : (T)0;
+    if (!full) {
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const bool in = there && jl + e <= at[m] && jl + e >= since[m];
+          s[m][e / 4][e % 4] = in ? s[m][e / 4][e % 4] * p.sc : -INFINITY;
+        }
+    } else {
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[m][e / 4][e % 4] *= p.sc;
+    }
+    FV ph[MT], pl[F16 ? MT : 1];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      float top = mx[m];
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = fmaxf(top, s[m][e / 4][e % 4]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float to = (top == -INFINITY ? 0.f : top) - OFF;
+      if (__builtin_amdgcn_ballot_w64(top != mx[m])) {
+        const float a = __builtin_amdgcn_exp2f(mx[m] - OFF - to);  // 0 from -inf
+        l[m] *= a;
+#pragma unroll
+        for (int i = 0; i < CPL; i++) o[m][i] *= a;
+      }
+      mx[m] = top;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float x = __builtin_amdgcn_exp2f(s[m][e / 4][e % 4] - to);
+        l[m] += x;
+        ph[m][e] = (T)x;
+        if (F16) pl[m][e] = (T)(x - (float)ph[m][e]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < CPL; i++) {
+      FV a;
+#pragma unroll
+      for (int e = 0; e < 8; e++) a[e] = vr[e][i];
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        if (F16) o[m][i] = mma(a, pl[m], o[m][i]);
+        o[m][i] = mma(a, ph[m], o[m][i]);
+      }
+    }
+    if (odd) {  // what is not finite reaches the queries that see it one by one, not as 0 times it the others
+      float *w = s_o[wave];
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[lr * 32 + 8 * q4 + e] = (float)ph[m][e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (int k = 0; k < 32; k++) {
+          const int x = k >> 4, tk = j[x] + (k & 15);
+          if (pg[x] < 0) continue;
+          const float y = w[lr * 32 + k];
+          const bool in = tk <= at[m] && tk >= since[m];
+          const T *v = vb[x] + (k & 15) * c.dv;
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int i = 0; i < CPL; i++) {
+              const int col = CPL * (4 * q4 + r) + i;
+              const float z = col < c.dv ? (float)v[col] : 0.f;
+              if (in && !finite(z)) o[m][i][r] += y * z;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    }
+  }
+  // the four waves' sums
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    l[m] += __shfl_xor(l[m], 16);
+    l[m] += __shfl_xor(l[m], 32);
+    if (q4 == 0) s_m[wave][16 * m + lr] = mx[m], s_l[wave][16 * m + lr] = l[m];
+  }
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int i = 0; i < CPL; i++) s_o[wave][lr * (D + 4) + CPL * (4 * q4 + r) + i] = o[m][i][r];
+    __syncthreads();
+    const int x = tid >> 4, c0 = (tid & 15) * CPL, row = 16 * m + x;
+    float top = s_m[0][row], f[4], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < 4; w++) top = fmaxf(top, s_m[w][row]);
+    const float to = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - to);
+      sum += f[w] * s_l[w][row];
+    }
+    float y[CPL];
+#pragma unroll
+    for (int i = 0; i < CPL; i++) {
+      y[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) y[i] = __builtin_fmaf(f[w], s_o[w][x * (D + 4) + c0 + i], y[i]);
+    }
+    if (nsp == 1) {
+      int t, h;
+      tile_row(p, tile, row, MR, &t, &h);
+      if (t >= n) continue;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      T *out = (T *)p.o + ((long long)first + t) * p.ldo + ((long long)g * p.G + h) * c.dv;
+      if (V) {
+        kv_vec<T, CPL> z;
+#pragma unroll
+        for (int i = 0; i < CPL; i++) z[i] = (T)(y[i] * inv);
+        if (c0 < c.dv) *(kv_vec<T, CPL> *)(out + c0) = z;
+      } else {
+#pragma unroll
+        for (int i = 0; i < CPL; i++)
+          if (c0 + i < c.dv) out[c0 + i] = (T)(y[i] * inv);
+      }
+    } else {
+      const long long at = blk * MR + row;
+      if ((tid & 15) == 0) pml[at] = make_float2(top, sum);
+      if (sum != 0.f)
+#pragma unroll
+        for (int i = 0; i < CPL; i += 2) *(float2 *)(part + at * D + c0 + i) = make_float2(y[i], y[i + 1]);
+    }
+  }
+}
+
+// The blocks of a split: each row's sums over them, in order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_kva_join(KvDev c, AttnDev p, int nrt, int nsp, int MR, long long unit0, const float *part,
+                                                  const float2 *pml) {
+  constexpr int L = D / 4, R = 256 / L;  // threads to a row, rows at a time
+  const int rg = MR / R > 0 ? MR / R : 1;
+  const long long unit = unit0 + blockIdx.x / rg;
+  const int tile = (int)(unit % nrt), g = (int)(unit / nrt % c.Hk), b = (int)(unit / nrt / c.Hk);
+  const int m = (int)(blockIdx.x % rg) * R + threadIdx.x / L, c0 = threadIdx.x % L * 4;
+  int first, past, t, h;
+  const int n = kv_rows(c, b, &first, &past);
+  if (m >= MR) return;
+  tile_row(p, tile, m, MR, &t, &h);
+  if (t >= n) return;
+  const long long at = unit * nsp * MR + m;
+  float top = -INFINITY, sum = 0.f;
+  for (int s = 0; s < nsp; s++) top = fmaxf(top, pml[at + (long long)s * MR].x);
+  const float to = top == -INFINITY ? 0.f : top;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < nsp; s++) {
+    const float2 z = pml[at + (long long)s * MR];
+    if (z.y == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(z.x - to);
+    const float4 x = *(const float4 *)(part + (at + (long long)s * MR) * D + c0);
+    sum = __builtin_fmaf(f, z.y, sum);
+    y.x = __builtin_fmaf(f, x.x, y.x), y.y = __builtin_fmaf(f, x.y, y.y);
+    y.z = __builtin_fmaf(f, x.z, y.z), y.w = __builtin_fmaf(f, x.w, y.w);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T *out = (T *)p.o + ((long long)first + t) * p.ldo + ((long long)g * p.G + h) * c.dv + c0;
+  const float z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (c0 + i < c.dv) out[i] = (T)z[i];
+}
+
+// How a call is cut
+struct Plan {
+  int D, MT, nrt, nsp;
+  long long units;
+};
+Plan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
+  Plan r;
+  const int d = c->dk > c->dv ? c->dk : c->dv, G = p->H / c->Hk;
+  r.D = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  const long long m = p->nsel ? G : (long long)T * G;
+  const int big = c->f16 ? (r.D <= 128 ? 4 : 2) : r.D <= 64 ? 4 : r.D == 128 ? 2 : 1;
+  r.MT = m <= 16 ? 1 : big;
+  const int MR = 16 * r.MT;
+  r.nrt = (int)(p->nsel ? T * bnh_ceil_div(G, MR) : bnh_ceil_div(m, MR));
+  r.units = (long long)B * c->Hk * r.nrt;
+  // tiles of 32 tokens that a row tile can see
+  long long tok = (long long)c->ldt * c->page;
+  if (p->nsel) tok = (long long)p->nsel * c->page;
+  else if (p->window && p->window + MR < tok) tok = p->window + MR;
+  const long long tiles = bnh_ceil_div(tok, 32) + 1;
+  long long s = bnh_ceil_div(1024, r.units);
+  if (s > tiles / 8) s = tiles / 8;
+  r.nsp = (int)(s < 1 ? 1 : s > 128 ? 128 : s);
+  return r;
+}
+size_t plan_bytes(const Plan &r) {
+  if (r.nsp == 1) return 0;
+  return (size_t)(r.units * r.nsp * 16 * r.MT * (4 * r.D + 8));
+}
+
+template <typename T, int D, int MT, bool V>
+int rows_run(const KvDev &c, const AttnDev &p, const Plan &r, void *work, hipStream_t s) {
+  float2 *pml = (float2 *)work;
+  float *part = (float *)(pml + r.units * r.nsp * 16 * r.MT);
+  const long long blocks = r.units * r.nsp, most = bnh_most_blocks(256);
+  for (long long b0 = 0; b0 < blocks; b0 += most) {
+    hipLaunchKernelGGL((k_kva<T, D, MT, V>), dim3((unsigned)(blocks - b0 < most ? blocks - b0 : most)), dim3(256), 0, s, c, p,
+                       r.nrt, r.nsp, b0, part, pml);
+    BNH_HIP(hipGetLastError());
+  }
+  if (r.nsp == 1) return 0;
+  const int R = 256 / (D / 4), rg = 16 * MT / R > 0 ? 16 * MT / R : 1;
+  for (long long u0 = 0; u0 < r.units; u0 += most / rg) {
+    const long long u = r.units - u0 < most / rg ? r.units - u0 : most / rg;
+    hipLaunchKernelGGL((k_kva_join<T, D>), dim3((unsigned)(u * rg)), dim3(256), 0, s, c, p, r.nrt, r.nsp, 16 * MT, u0, part, pml);
+    BNH_HIP(hipGetLastError());
+  }
+  return 0;
+}
+template <typename T, int D, bool V>
+int rows_go(const KvDev &c, const AttnDev &p, const Plan &r, void *work, hipStream_t s) {
+  constexpr int big = sizeof(T) == 2 ? (D <= 128 ? 4 : 2) : D <= 64 ? 4 : D == 128 ? 2 : 1;
+  if constexpr (big > 1)
+    if (r.MT > 1) return rows_run<T, D, big, V>(c, p, r, work, s);
+  return rows_run<T, D, 1, V>(c, p, r, work, s);
+}
+template <typename T, bool V>
+int rows_d(const KvDev &c, const AttnDev &p, const Plan &r, void *work, hipStream_t s) {
+  if (r.D == 32) return rows_go<T, 32, V>(c, p, r, work, s);
+  if (r.D == 64) return rows_go<T, 64, V>(c, p, r, work, s);
+  if (r.D == 128) return rows_go<T, 128, V>(c, p, r, work, s);
+  return rows_go<T, 256, V>(c, p, r, work, s);
+}
+
+int attn_check(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows) {
+  if (kv_check(c, T, B, rows)) return -1;
+  BNH_REQ(p && p->H > 0 && p->H % c->Hk == 0 && p->H <= 65536 && p->window >= 0 && p->nsel >= 0 && p->nsel <= (1 << 20));
+  BNH_REQ((long long)T * p->H < (1LL << 31) && (long long)rows * c->Hk < (1LL << 31));
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t bnh_kv_attn_work_bytes(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows) {
+  if (attn_check(c, p, T, B, rows)) return 0;
+  return plan_bytes(plan(c, p, T, B));
+}
+
+int bnh_kv_attn(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows, const int32_t *start, const int32_t *len,
+                void *work, size_t work_bytes, void *stream) {
+  if (attn_check(c, p, T, B, rows) || kv_check_buffers(c, T, B, rows, start, len)) return -1;
+  BNH_REQ(!p->nsel == !p->sel);
+  BNH_REQ(p->q && p->o && p->ldq >= p->H * c->dk && p->ldo >= p->H * c->dv);
+  const size_t es = c->f16 ? 2 : 4;
+  BNH_REQ(kv_on(p->q, es) && kv_on(p->o, es) && kv_on(p->sel, 4));
+  const Plan r = plan(c, p, T, B);
+  const size_t need = plan_bytes(r);
+  BNH_REQ(need == 0 || (work && kv_on(work, 16) && work_bytes >= need));
+  const KvDev d = kv_dev(c, T, rows, start, len);
+  const AttnDev a = {p->q, p->o, p->sel, p->ldq, p->ldo, p->H / c->Hk, p->window, p->nsel, p->scale * 1.44269504f};
+  const int ve = 16 / (int)es, cpl = r.D / 16;
+  bool v = c->dk % 8 == 0 && c->dv % cpl == 0 && c->k_ps % ve == 0 && c->v_ps % ve == 0 && p->ldq % ve == 0 &&
+           p->ldo % (cpl < ve ? cpl : ve) == 0;
+  for (const void *x : {p->q, (const void *)p->o, (const void *)c->k, (const void *)c->v}) v = v && kv_on(x, 16);
+  hipStream_t s = bnh_stream(stream);
+  if (c->f16) return v ? rows_d<h16, true>(d, a, r, work, s) : rows_d<h16, false>(d, a, r, work, s);
+  return v ? rows_d<float, true>(d, a, r, work, s) : rows_d<float, false>(d, a, r, work, s);
+}
+
+}  // extern "C"

@@ -523,6 +523,76 @@ size_t bnh_linattn_work_bytes(const bnh_la *p, int T, int B);
 int bnh_linattn(const bnh_la *p, int T, int B, int rows, const int32_t *start, const int32_t *len, void *work,
                 size_t work_bytes, void *stream);
 
+/* A cache of keys and values in pages, of which sequences (stations) hold as many as they need. Page x of the pool holds
+ * `page` tokens (a power of two, 16 to 1024) of Hk heads: keys [Hk][page][dk] at k + x k_ps, values [Hk][page][dv] at
+ * v + x v_ps (elements). table [B][ldt] has the pages of each sequence of a call in order: its token j is token j % page of
+ * page table[i][j / page]; an entry outside [0, pages), or none (j / page >= ldt), is a page that is not there. past [B]: the
+ * tokens of each sequence ahead of this call's rows (below 0 counts as 0). dk, dv <= 256, ldt page < 2^31. lo, hi
+ * [pages][Hk][dk] (both or neither): the smallest and the largest of a page's keys by value of dk, kept by bnh_kv_append for
+ * bnh_kv_select. Of the three entries that take it, each has B sequences of at most T rows among `rows` rows, as
+ * bnh_linattn has: row t of sequence i is row start[i] + t of the buffers and token past[i] + t of its cache. All of it is
+ * device memory. */
+typedef struct {
+  void *k, *v;
+  long long k_ps, v_ps;
+  int f16;            /* type of keys, values, bounds and of the rows that go with them: 0 fp32, 1 fp16 */
+  int pages, page, Hk, dk, dv;
+  void *lo, *hi;
+  const int32_t *table;
+  int ldt;
+  const int32_t *past;
+} bnh_kvcache;
+/* The rotation of a row by its position: the first rd (even, <= dk) values of each head are pairs (x, y), values e and
+ * e + rd/2 of the head (pairs 0) or 2e and 2e + 1 (pairs 1), e < rd/2, and become (x cos a - y sin a, x sin a + y cos a) with
+ * a = position freq[e]; freq fp32 [rd/2]. pos int32 [rows]: the positions; NULL: past[i] + t. The angle is taken in 64 bits:
+ * a position of 2^31 is as exact as one of 0. */
+typedef struct {
+  int rd, pairs;
+  const float *freq;
+  const int32_t *pos;
+} bnh_rotary;
+/* New rows into the cache: k's rows of Hk heads of dk at r ldk, rotated, and v's of dv at r ldv into their pages (a token whose
+ * page is not there is not stored), the bounds of the pages that they touch brought up to date (a NaN stays), and q's rows of H
+ * heads of dk at r ldq, rotated, to qr at r ldr (q NULL: none; qr may be q with ldr = ldq). r NULL: no rotation. No two
+ * sequences of a call put tokens into one page. Tokens of a page go in in order: those behind a call's last are taken as
+ * not there yet. H: a multiple of Hk. */
+int bnh_kv_append(const bnh_kvcache *c, const bnh_rotary *r, const void *k, int ldk, const void *v, int ldv, const void *q,
+                  int ldq, void *qr, int ldr, int H, int T, int B, int rows, const int32_t *start, const int32_t *len,
+                  void *stream);
+/* Attention of new rows over the cache, theirs included (append them first). Head h < H of row t of sequence i, with keys and
+ * values of head h Hk / H: over the tokens j <= past[i] + t, j > past[i] + t - window (window 0: all) whose pages are there,
+ *   s_j = scale q . k_j,  o = sum_j e^{s_j} v_j / sum_j e^{s_j},
+ * and 0 where there are none (or all s_j are -inf). sel int32 [rows][Hk][nsel] (NULL: all pages): of those tokens the ones in
+ * the pages i that the row's selection for the head lists in ascending order; an entry that is not above the one before it,
+ * or outside [0, ldt), is passed over. What the cache holds in other places reaches no output, infinities and NaNs neither.
+ * Scores, sums and outputs are fp32, rounded once at the end; fp16: the e^{s_j} are factors of 11 bits, or 22 where a call
+ * has few rows (or widths past 128) and reading the cache is what counts.
+ * work: device scratch of at least bnh_kv_attn_work_bytes bytes, 16-byte aligned (0 bytes for some shapes: NULL is allowed
+ * then); its size depends on c's and p's sizes, T, B and rows. */
+typedef struct {
+  const void *q;
+  int ldq;
+  void *o;
+  int ldo, H;         /* H: a multiple of Hk; o's rows hold H heads of dv */
+  float scale;
+  int window;
+  int32_t *sel;
+  int nsel;
+} bnh_kvattn;
+size_t bnh_kv_attn_work_bytes(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows);
+int bnh_kv_attn(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows, const int32_t *start, const int32_t *len,
+                void *work, size_t work_bytes, void *stream);
+/* The pages that each row looks at, into p->sel (p's q, ldq, H, window, sel and nsel; c's bounds): of the pages with a token that
+ * the row may see, the first `first` of the sequence and the row's last `last` (its own among them) always, then those of the
+ * largest
+ *   sum over the heads h of Hk's head and over d of q_hd (q_hd >= 0 ? hi_d : lo_d),
+ * no smaller than the sum of q . k_j over the heads for any token j of the page, up to nsel pages in all (>= first + last); of equal
+ * ones the lower pages, NaN counts as -inf. Ascending, -1 behind. The sums are in 64 bits. Rows of no sequence are left as they
+ * are. work as above, bnh_kv_select_work_bytes of it. */
+size_t bnh_kv_select_work_bytes(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows);
+int bnh_kv_select(const bnh_kvcache *c, const bnh_kvattn *p, int first, int last, int T, int B, int rows,
+                  const int32_t *start, const int32_t *len, void *work, size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
