@@ -37,6 +37,7 @@ SOURCES = [
     "kern_linattn.hip",
     "kern_kv.hip",
     "kern_kvattn.hip",
+    "kern_kvtile.hip",
     "pkg_file.cpp",
     "rt_contract.cpp",
     "rt_pkg.cpp",

@@ -13,11 +13,18 @@ struct KvDev {
   int pages, sh, Hk, dk, dv, ldt, T, rows;  // sh: log2 of the tokens to a page
 };
 
-// sequence b's first row, its rows (cut to T and to the buffers' rows) and the tokens ahead of them
+// An int that all lanes have, through the scalar cache whatever the kernel has stored before: for what nothing stores to while it
+// is read
+__device__ __forceinline__ int kv_int(const int32_t *p, long long i) {
+  typedef __attribute__((address_space(4))) const int32_t *P;
+  return __builtin_amdgcn_readfirstlane(((P)(uintptr_t)p)[i]);
+}
+// sequence b's (the same in all lanes) first row, its rows (cut to T and to the buffers' rows) and the tokens ahead of them
 __device__ __forceinline__ int kv_rows(const KvDev &c, int b, int *first, int *past) {
-  const long long s = c.start ? c.start[b] : (long long)b * c.T;
-  long long n = c.len ? c.len[b] : c.T;
-  const int m = c.past[b];
+  b = __builtin_amdgcn_readfirstlane(b);
+  const long long s = c.start ? kv_int(c.start, b) : (long long)b * c.T;
+  long long n = c.len ? kv_int(c.len, b) : c.T;
+  const int m = kv_int(c.past, b);
   *past = m > 0 ? m : 0;
   n = n < c.T ? n : c.T;
   if (s < 0 || s >= c.rows) n = 0;
@@ -32,7 +39,6 @@ __device__ __forceinline__ int kv_page(const KvDev &c, int b, int i) {
   const int p = c.table[(long long)b * c.ldt + i];
   return (unsigned)p < (unsigned)c.pages ? p : -1;
 }
-
 // N values of a row from its value c, zeros from value n on. V: N divides c and n and the row is aligned to the N values
 // or to 16 bytes
 template <typename T, int N>

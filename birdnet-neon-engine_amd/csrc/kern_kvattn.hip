@@ -4,22 +4,10 @@
 // in one pass over the keys with the running m and sum, both in fp32 and base 2.
 #include <math.h>
 
-#include "bnh_kv.h"
+#include "bnh_kvattn.h"
 
 namespace {
 
-struct AttnDev {
-  const void *q;
-  void *o;
-  const int32_t *sel;
-  int ldq, ldo, G, window, nsel;  // G: query heads that share one of keys
-  float sc;                       // scale log2(e)
-};
-
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef h16 v8h __attribute__((ext_vector_type(8)));
-template <typename T>
-using vec8 = T __attribute__((ext_vector_type(8)));
 // 32 steps of a product: 8 of row (or column) lane & 15 in a lane, the same 8 of both operands
 __device__ __forceinline__ v4f mma(kv_vec<h16, 8> a, kv_vec<h16, 8> b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -29,26 +17,6 @@ __device__ __forceinline__ v4f mma(kv_vec<float, 8> a, kv_vec<float, 8> b, v4f c
   for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
   return c;
 }
-template <typename T>
-__device__ __forceinline__ bool finite(T x) { return x - x == (T)0; }
-
-// A tile of rows: MR rows and query heads of one sequence and head of keys, heads innermost; with a selection, heads of one row
-struct Tile {
-  int t0, t1;  // its first and last row
-};
-__device__ __forceinline__ void tile_row(const AttnDev &p, int tile, int m, int MR, int *t, int *h) {
-  if (p.sel) {
-    const int ht = (p.G + MR - 1) / MR;
-    *t = tile / ht;
-    *h = tile % ht * MR + m;
-    if (*h >= p.G) *t = 0x7fffffff;  // nobody's
-  } else {
-    const long long x = (long long)tile * MR + m;
-    *t = (int)(x / p.G);
-    *h = (int)(x % p.G);
-  }
-}
-
 // The streaming form, for few rows, for fp32 and for widths that the tiled form does not take: bound by reading keys and values
 // where rows are few. Four waves of a block take tiles of 32 tokens in turn, straight from memory into the matrix
 // instructions' registers: the scores' product has keys as its rows in such an order that a lane ends with the scores of 8 tokens
@@ -57,7 +25,7 @@ __device__ __forceinline__ void tile_row(const AttnDev &p, int tile, int m, int 
 // the end over waves, and over the blocks of a split by k_kva_join. fp16: e^{s - m} goes into the product in two parts, 22 bits,
 // in units of 2^-12 so that the second part of small ones is no subnormal: the matrix cores wait for memory here.
 template <typename T, int D, int MT, bool V>
-__global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int nsp, long long blk0, float *part, float2 *pml) {
+__global__ __launch_bounds__(256) void k_kva(KvDev c, KvaDev p, int nrt, int nsp, long long blk0, float *part, float2 *pml) {
   constexpr bool F16 = sizeof(T) == 2;
   constexpr int DKT = D / 32, CPL = D / 16, MR = 16 * MT;
   constexpr float OFF = F16 ? 12.f : 0.f;
@@ -70,10 +38,10 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int first, past, t0, t1, hx;
   const int n = kv_rows(c, b, &first, &past);
-  tile_row(p, tile, 0, MR, &t0, &hx);
+  kva_row(p, tile, 0, MR, &t0, &hx);
   if (t0 >= n) return;
   if (p.sel) t1 = t0;
-  else tile_row(p, tile, MR - 1, MR, &t1, &hx);
+  else kva_row(p, tile, MR - 1, MR, &t1, &hx);
   t1 = t1 < n ? t1 : n - 1;
   // queries
   FV qf[MT][DKT];
@@ -81,13 +49,16 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
 #pragma unroll
   for (int m = 0; m < MT; m++) {
     int t, h;
-    tile_row(p, tile, 16 * m + lr, MR, &t, &h);
+    kva_row(p, tile, 16 * m + lr, MR, &t, &h);
     const bool in = t < n;
     at[m] = in ? past + t : -1;
     since[m] = p.window && at[m] >= p.window ? at[m] - p.window + 1 : 0;
     const T *q = (const T *)p.q + ((long long)first + (in ? t : t0)) * p.ldq + ((long long)g * p.G + (in ? h : 0)) * c.dk;
 #pragma unroll
-    for (int d = 0; d < DKT; d++) qf[m][d] = kv_ld<T, 8, V>(q, 32 * d + 8 * q4, in ? c.dk : 0);
+    for (int d = 0; d < DKT; d++) {
+      qf[m][d] = kv_ld<T, 8, V>(q, 32 * d + 8 * q4, in ? c.dk : 0);
+      if (p.neg) qf[m][d] = -qf[m][d];
+    }
   }
   // tokens
   const int all0 = p.window && past + t1 >= p.window ? past + t1 - p.window + 1 : 0;  // from here and ..
@@ -131,7 +102,7 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
       pg[s] = kv_page(c, b, pi);
     }
   };
-  int jn[2], pn[2];
+  int jn[2], pn[2], bad0 = 0x7fffffff, bad1 = -1;  // tiles with values that are not finite: left out, and added at the end
   look(kt0 + wave, jn, pn);
   for (int kt = kt0 + wave; kt < kt1; kt += 4) {
     int j[2] = {jn[0], jn[1]}, pg[2] = {pn[0], pn[1]};
@@ -166,50 +137,32 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
       for (int m = 0; m < MT; m++) s[m][0] = mma(kf[0][d], qf[m][d], s[m][0]), s[m][1] = mma(kf[1][d], qf[m][d], s[m][1]);
     const int jl = (q4 & 2 ? j[1] : j[0]) + 8 * (q4 & 1);  // the lane's 8 tokens
     const bool there = (q4 & 2 ? pg[1] : pg[0]) >= 0;
-    // a value is not finite, in a tile that not every query sees all of, or one whose factors are in two parts (an infinity times
-    // a second part of 0 or of the other sign)
-    bool odd = false;
-    if constexpr (F16) {
-      typedef unsigned short u2 __attribute__((ext_vector_type(2)));
-      u2 most = {0, 0};
+    kv_vec<T, 2> mk = {(T)0, (T)0};
+#pragma unroll
+    for (int e = 0; e < 8; e++) kv_mark<T, CPL>(vr[e], mk);
+    if (__builtin_amdgcn_ballot_w64(mk[0] != mk[0] || mk[1] != mk[1])) {
+      bad0 = bad0 < kt ? bad0 : kt, bad1 = kt;
 #pragma unroll
       for (int e = 0; e < 8; e++)
 #pragma unroll
-        for (int i = 0; i < CPL; i += 2)
-          most = __builtin_elementwise_max(most, (u2){hbits(vr[e][i]), hbits(vr[e][i + 1])} & (u2){0x7fff, 0x7fff});
-      odd = most[0] >= 0x7c00 || most[1] >= 0x7c00;
-    } else if (!full) {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-#pragma unroll
-        for (int i = 0; i < CPL; i++) odd = odd || !finite(vr[e][i]);
+        for (int i = 0; i < CPL; i++) vr[e][i] = kv_finite(vr[e][i]) ? vr[e][i] : (T)0;
     }
-    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-    if (odd)
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-#pragma unroll
-        for (int i = 0; i < CPL; i++) vr[e][i] = finite(vr[e][i]) ? vr[e][i] : (T)0;
     if (!full) {
 #pragma unroll
       for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const bool in = there && jl + e <= at[m] && jl + e >= since[m];
-          s[m][e / 4][e % 4] = in ? s[m][e / 4][e % 4] * p.sc : -INFINITY;
+          s[m][e / 4][e % 4] = in ? s[m][e / 4][e % 4] : -INFINITY;
         }
-    } else {
-#pragma unroll
-      for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) s[m][e / 4][e % 4] *= p.sc;
     }
     FV ph[MT], pl[F16 ? MT : 1];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-      float top = mx[m];
+      float top = s[m][0][0];
 #pragma unroll
-      for (int e = 0; e < 8; e++) top = fmaxf(top, s[m][e / 4][e % 4]);
+      for (int e = 1; e < 8; e++) top = fmaxf(top, s[m][e / 4][e % 4]);
+      top = fmaxf(mx[m], top * p.sc);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float to = (top == -INFINITY ? 0.f : top) - OFF;
@@ -222,7 +175,7 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
       mx[m] = top;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float x = __builtin_amdgcn_exp2f(s[m][e / 4][e % 4] - to);
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][e / 4][e % 4], p.sc, -to));
         l[m] += x;
         ph[m][e] = (T)x;
         if (F16) pl[m][e] = (T)(x - (float)ph[m][e]);
@@ -239,30 +192,42 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
         o[m][i] = mma(a, ph[m], o[m][i]);
       }
     }
-    if (odd) {  // what is not finite reaches the queries that see it one by one, not as 0 times it the others
-      float *w = s_o[wave];
+  }
+  // Values that are not finite, for the queries that see them: within the products, 0 times them would reach the others, and
+  // an infinity times a second part of 0 be none
+  for (int kt = bad0; kt <= bad1; kt += 4) {
+    int j[2], pg[2];
+    look(kt, j, pg);
+#pragma unroll 1
+    for (int k = 0; k < 32; k++) {
+      const int x = k >> 4, tk = (x ? j[1] : j[0]) + (k & 15), page = x ? pg[1] : pg[0];
+      if (page < 0) continue;
+      const long long in = ((long long)g << c.sh) + (tk & ((1 << c.sh) - 1));
+      const T *v = (const T *)c.v + page * c.v_ps + in * c.dv, *kr = (const T *)c.k + page * c.k_ps + in * c.dk;
+      bool bad = false;
+      for (int col = lane; col < c.dv; col += 64) bad = bad || !kv_finite(v[col]);
+      if (!__builtin_amdgcn_ballot_w64(bad)) continue;
 #pragma unroll
       for (int m = 0; m < MT; m++) {
+        float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[lr * 32 + 8 * q4 + e] = (float)ph[m][e];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-        for (int k = 0; k < 32; k++) {
-          const int x = k >> 4, tk = j[x] + (k & 15);
-          if (pg[x] < 0) continue;
-          const float y = w[lr * 32 + k];
-          const bool in = tk <= at[m] && tk >= since[m];
-          const T *v = vb[x] + (k & 15) * c.dv;
+        for (int d = 0; d < DKT; d++) {
+          const FV y = kv_ld<T, 8, V>(kr, 32 * d + 8 * q4, c.dk);
 #pragma unroll
-          for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int i = 0; i < CPL; i++) {
-              const int col = CPL * (4 * q4 + r) + i;
-              const float z = col < c.dv ? (float)v[col] : 0.f;
-              if (in && !finite(z)) o[m][i][r] += y * z;
-            }
+          for (int e = 0; e < 8; e++) s = __builtin_fmaf((float)y[e], (float)qf[m][d][e], s);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        if (tk > at[m] || tk < since[m] || s == -INFINITY) continue;
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.sc, OFF - mx[m]));
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int i = 0; i < CPL; i++) {
+            const int col = CPL * (4 * q4 + r) + i;
+            const float z = col < c.dv ? (float)v[col] : 0.f;
+            if (!kv_finite(z)) o[m][i][r] += y * z;
+          }
       }
     }
   }
@@ -300,7 +265,7 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
     }
     if (nsp == 1) {
       int t, h;
-      tile_row(p, tile, row, MR, &t, &h);
+      kva_row(p, tile, row, MR, &t, &h);
       if (t >= n) continue;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       T *out = (T *)p.o + ((long long)first + t) * p.ldo + ((long long)g * p.G + h) * c.dv;
@@ -326,7 +291,7 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, AttnDev p, int nrt, int ns
 
 // The blocks of a split: each row's sums over them, in order
 template <typename T, int D>
-__global__ __launch_bounds__(256) void k_kva_join(KvDev c, AttnDev p, int nrt, int nsp, int MR, long long unit0, const float *part,
+__global__ __launch_bounds__(256) void k_kva_join(KvDev c, KvaDev p, int nrt, int nsp, int MR, long long unit0, const float *part,
                                                   const float2 *pml) {
   constexpr int L = D / 4, R = 256 / L;  // threads to a row, rows at a time
   const int rg = MR / R > 0 ? MR / R : 1;
@@ -336,7 +301,7 @@ __global__ __launch_bounds__(256) void k_kva_join(KvDev c, AttnDev p, int nrt, i
   int first, past, t, h;
   const int n = kv_rows(c, b, &first, &past);
   if (m >= MR) return;
-  tile_row(p, tile, m, MR, &t, &h);
+  kva_row(p, tile, m, MR, &t, &h);
   if (t >= n) return;
   const long long at = unit * nsp * MR + m;
   float top = -INFINITY, sum = 0.f;
@@ -360,64 +325,77 @@ __global__ __launch_bounds__(256) void k_kva_join(KvDev c, AttnDev p, int nrt, i
     if (c0 + i < c.dv) out[i] = (T)z[i];
 }
 
-// How a call is cut
-struct Plan {
-  int D, MT, nrt, nsp;
-  long long units;
-};
-Plan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
-  Plan r;
+KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
+  KvaPlan r;
   const int d = c->dk > c->dv ? c->dk : c->dv, G = p->H / c->Hk;
-  r.D = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
   const long long m = p->nsel ? G : (long long)T * G;
-  const int big = c->f16 ? (r.D <= 128 ? 4 : 2) : r.D <= 64 ? 4 : r.D == 128 ? 2 : 1;
-  r.MT = m <= 16 ? 1 : big;
-  const int MR = 16 * r.MT;
-  r.nrt = (int)(p->nsel ? T * bnh_ceil_div(G, MR) : bnh_ceil_div(m, MR));
+  r.D = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  r.tiled = !p->nsel && m > 64;
+  if (r.tiled) {
+    r.DK = c->dk <= 64 && d <= 128 ? 64 : d <= 128 ? 128 : 256;
+    r.D = c->dv <= 64 && d <= 128 ? 64 : d <= 128 ? 128 : 256;
+    r.MR = 32 * kva_waves(r.DK);
+  } else {
+    const int big = c->f16 ? (r.D <= 128 ? 64 : 32) : r.D <= 64 ? 64 : r.D == 128 ? 32 : 16;
+    r.MR = m <= 16 ? 16 : big;
+  }
+  r.nrt = (int)(p->nsel ? T * bnh_ceil_div(G, r.MR) : bnh_ceil_div(m, r.MR));
   r.units = (long long)B * c->Hk * r.nrt;
   // tiles of 32 tokens that a row tile can see
   long long tok = (long long)c->ldt * c->page;
   if (p->nsel) tok = (long long)p->nsel * c->page;
-  else if (p->window && p->window + MR < tok) tok = p->window + MR;
+  else if (p->window && p->window + r.MR < tok) tok = p->window + r.MR;
   const long long tiles = bnh_ceil_div(tok, 32) + 1;
-  long long s = bnh_ceil_div(1024, r.units);
+  long long s = bnh_ceil_div(r.tiled ? 512 : 1024, r.units);
   if (s > tiles / 8) s = tiles / 8;
   r.nsp = (int)(s < 1 ? 1 : s > 128 ? 128 : s);
   return r;
 }
-size_t plan_bytes(const Plan &r) {
+size_t plan_bytes(const KvaPlan &r) {
   if (r.nsp == 1) return 0;
-  return (size_t)(r.units * r.nsp * 16 * r.MT * (4 * r.D + 8));
+  return (size_t)(r.units * r.nsp * r.MR * (4 * r.D + 8));
 }
 
+template <typename T, int D>
+int join_run(const KvDev &c, const KvaDev &p, const KvaPlan &r, const float *part, const float2 *pml, hipStream_t s) {
+  if (r.nsp == 1) return 0;
+  const long long most = bnh_most_blocks(256);
+  const int R = 256 / (D / 4), rg = r.MR / R > 0 ? r.MR / R : 1;
+  for (long long u0 = 0; u0 < r.units; u0 += most / rg) {
+    const long long u = r.units - u0 < most / rg ? r.units - u0 : most / rg;
+    hipLaunchKernelGGL((k_kva_join<T, D>), dim3((unsigned)(u * rg)), dim3(256), 0, s, c, p, r.nrt, r.nsp, r.MR, u0, part, pml);
+    BNH_HIP(hipGetLastError());
+  }
+  return 0;
+}
 template <typename T, int D, int MT, bool V>
-int rows_run(const KvDev &c, const AttnDev &p, const Plan &r, void *work, hipStream_t s) {
-  float2 *pml = (float2 *)work;
-  float *part = (float *)(pml + r.units * r.nsp * 16 * r.MT);
+int rows_run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
+  float2 *pml = kva_ml(r, work);
+  float *part = kva_part(r, work);
   const long long blocks = r.units * r.nsp, most = bnh_most_blocks(256);
   for (long long b0 = 0; b0 < blocks; b0 += most) {
     hipLaunchKernelGGL((k_kva<T, D, MT, V>), dim3((unsigned)(blocks - b0 < most ? blocks - b0 : most)), dim3(256), 0, s, c, p,
                        r.nrt, r.nsp, b0, part, pml);
     BNH_HIP(hipGetLastError());
   }
-  if (r.nsp == 1) return 0;
-  const int R = 256 / (D / 4), rg = 16 * MT / R > 0 ? 16 * MT / R : 1;
-  for (long long u0 = 0; u0 < r.units; u0 += most / rg) {
-    const long long u = r.units - u0 < most / rg ? r.units - u0 : most / rg;
-    hipLaunchKernelGGL((k_kva_join<T, D>), dim3((unsigned)(u * rg)), dim3(256), 0, s, c, p, r.nrt, r.nsp, 16 * MT, u0, part, pml);
-    BNH_HIP(hipGetLastError());
-  }
-  return 0;
+  return join_run<T, D>(c, p, r, part, pml, s);
 }
 template <typename T, int D, bool V>
-int rows_go(const KvDev &c, const AttnDev &p, const Plan &r, void *work, hipStream_t s) {
+int rows_go(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
   constexpr int big = sizeof(T) == 2 ? (D <= 128 ? 4 : 2) : D <= 64 ? 4 : D == 128 ? 2 : 1;
   if constexpr (big > 1)
-    if (r.MT > 1) return rows_run<T, D, big, V>(c, p, r, work, s);
+    if (r.MR > 16) return rows_run<T, D, big, V>(c, p, r, work, s);
   return rows_run<T, D, 1, V>(c, p, r, work, s);
 }
 template <typename T, bool V>
-int rows_d(const KvDev &c, const AttnDev &p, const Plan &r, void *work, hipStream_t s) {
+int run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
+  if (r.tiled) {
+    if (kva_tiles(c, p, r, sizeof(T) == 2, V, work, s)) return -1;
+    const float2 *pml = kva_ml(r, work);
+    const float *part = kva_part(r, work);
+    return r.D == 64 ? join_run<T, 64>(c, p, r, part, pml, s) : r.D == 128 ? join_run<T, 128>(c, p, r, part, pml, s)
+                                                                           : join_run<T, 256>(c, p, r, part, pml, s);
+  }
   if (r.D == 32) return rows_go<T, 32, V>(c, p, r, work, s);
   if (r.D == 64) return rows_go<T, 64, V>(c, p, r, work, s);
   if (r.D == 128) return rows_go<T, 128, V>(c, p, r, work, s);
@@ -447,18 +425,19 @@ int bnh_kv_attn(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int row
   BNH_REQ(p->q && p->o && p->ldq >= p->H * c->dk && p->ldo >= p->H * c->dv);
   const size_t es = c->f16 ? 2 : 4;
   BNH_REQ(kv_on(p->q, es) && kv_on(p->o, es) && kv_on(p->sel, 4));
-  const Plan r = plan(c, p, T, B);
+  const KvaPlan r = plan(c, p, T, B);
   const size_t need = plan_bytes(r);
   BNH_REQ(need == 0 || (work && kv_on(work, 16) && work_bytes >= need));
   const KvDev d = kv_dev(c, T, rows, start, len);
-  const AttnDev a = {p->q, p->o, p->sel, p->ldq, p->ldo, p->H / c->Hk, p->window, p->nsel, p->scale * 1.44269504f};
-  const int ve = 16 / (int)es, cpl = r.D / 16;
+  const float sc = fabsf(p->scale * 1.44269504f);  // a scale of 0 as one whose products round to 0
+  const KvaDev a = {p->q, p->o, p->sel, p->ldq, p->ldo, p->H / c->Hk, p->window, p->nsel, sc < 1e-37f ? 1e-37f : sc, p->scale < 0};
+  const int ve = 16 / (int)es, cpl = r.tiled ? 8 : r.D / 16;
   bool v = c->dk % 8 == 0 && c->dv % cpl == 0 && c->k_ps % ve == 0 && c->v_ps % ve == 0 && p->ldq % ve == 0 &&
            p->ldo % (cpl < ve ? cpl : ve) == 0;
   for (const void *x : {p->q, (const void *)p->o, (const void *)c->k, (const void *)c->v}) v = v && kv_on(x, 16);
   hipStream_t s = bnh_stream(stream);
-  if (c->f16) return v ? rows_d<h16, true>(d, a, r, work, s) : rows_d<h16, false>(d, a, r, work, s);
-  return v ? rows_d<float, true>(d, a, r, work, s) : rows_d<float, false>(d, a, r, work, s);
+  if (c->f16) return v ? run<h16, true>(d, a, r, work, s) : run<h16, false>(d, a, r, work, s);
+  return v ? run<float, true>(d, a, r, work, s) : run<float, false>(d, a, r, work, s);
 }
 
 }  // extern "C"
