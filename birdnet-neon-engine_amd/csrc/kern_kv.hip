@@ -46,11 +46,13 @@ __device__ __forceinline__ T high(T a, T b) { return a != a ? a : b != b ? b : a
 
 // A unit: VEC values at `a` and VEC more at `b` (pairs 0: the partners; pairs 1 and values past rd: the next ones)
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, int nu, long long blk0) {
+__global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, int nu, int b0, int pt0) {
   typedef T W __attribute__((ext_vector_type(VEC), aligned(sizeof(T) * VEC)));
   __shared__ T s_lo[512 * VEC], s_hi[512 * VEC];
-  const long long blk = blk0 + blockIdx.x;
-  const int g = (int)(blk % c.Hk), pt = (int)(blk / c.Hk % npt), b = (int)(blk / c.Hk / npt);
+  const unsigned sq = blockIdx.x / (unsigned)c.Hk;  // sequences and pages of a launch from (b0, pt0) on
+  const int g = (int)(blockIdx.x - sq * c.Hk);
+  const unsigned b1 = sq / (unsigned)npt, pt1 = sq - b1 * npt;
+  const int b = b0 + (int)b1, pt = pt0 + (int)pt1;
   int first, past;
   const int n = kv_rows(c, b, &first, &past);
   const int pi = (past >> c.sh) + pt;                   // the sequence's page
@@ -161,12 +163,15 @@ int append_run(const KvDev &c, const AppDev &p, int B, hipStream_t s) {
   const int npt = (int)(((long long)c.T + (1 << c.sh) - 2) >> c.sh) + 1;  // pages that T rows can touch
   const int half = p.rd / 2, nr = p.pairs ? 0 : (half + VEC - 1) / VEC, left = c.dk - (p.pairs ? 0 : p.rd);
   const int nu = nr + (left + 2 * VEC - 1) / (2 * VEC);
-  const long long blocks = (long long)B * npt * c.Hk, most = bnh_most_blocks(256);
-  for (long long b0 = 0; b0 < blocks; b0 += most) {
-    hipLaunchKernelGGL((k_kv_append<T, VEC>), dim3((unsigned)(blocks - b0 < most ? blocks - b0 : most)), dim3(256), 0, s, c, p,
-                       npt, nu, b0);
-    BNH_HIP(hipGetLastError());
-  }
+  const long long most = bnh_most_blocks(256);  // Hk <= 2^16
+  const int np = most / c.Hk < npt ? (int)(most / c.Hk) : npt, nb = most / c.Hk / np < B ? (int)(most / c.Hk / np) : B;
+  for (int b0 = 0; b0 < B; b0 += nb)
+    for (int p0 = 0; p0 < npt; p0 += np) {
+      const int n = npt - p0 < np ? npt - p0 : np;
+      hipLaunchKernelGGL((k_kv_append<T, VEC>), dim3((unsigned)((long long)(B - b0 < nb ? B - b0 : nb) * n * c.Hk)), dim3(256), 0, s,
+                         c, p, n, nu, b0, p0);
+      BNH_HIP(hipGetLastError());
+    }
   return 0;
 }
 
@@ -183,18 +188,19 @@ struct SelDev {
   int32_t *sel;
   int ldq, H, G, window, nsel, first, last;
 };
-// the row's place: its sequence's pages [lo, hi) have a token that it may see. Rows of a launch are numbered b T + t
-__device__ __forceinline__ bool sel_row(const KvDev &c, const SelDev &p, long long i, int *b, long long *row, int *lo, int *hi) {
-  *b = (int)(i / c.T);
-  const int t = (int)(i % c.T);
+// the row's place: its sequence's pages [lo, hi) have a token that it may see. Row i of a launch is row t0 + i of sequence b0, or
+// of those after it
+__device__ __forceinline__ bool sel_row(const KvDev &c, int window, int b0, int t0, unsigned i, int *b, long long *row, int *lo, int *hi) {
+  const unsigned x = (unsigned)t0 + i, q = x / (unsigned)c.T;
+  *b = b0 + (int)q;
+  const int t = (int)(x - q * (unsigned)c.T);
   int first, past;
   const int n = kv_rows(c, *b, &first, &past);
   if (t >= n) return false;
   *row = (long long)first + t;
   const int at = past + t;
-  *lo = p.window && at >= p.window ? (at - p.window + 1) >> c.sh : 0;
-  const int h = (at >> c.sh) + 1;
-  *hi = h;
+  *lo = window && at >= window ? (at - window + 1) >> c.sh : 0;
+  *hi = (at >> c.sh) + 1;
   return true;
 }
 
@@ -203,17 +209,17 @@ __device__ __forceinline__ bool sel_row(const KvDev &c, const SelDev &p, long lo
 // sums can make another choice.
 constexpr int PPB = 64;
 template <typename T, bool V>
-__global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, long long row0, u64 *key) {
+__global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, int b0, int t0, u64 *key) {
   __shared__ __attribute__((aligned(16))) float s_q[16 * 256];  // up to 16 query heads at a time
-  const int pb = (int)(blockIdx.x % npb), g = (int)(blockIdx.x / npb % c.Hk);
-  const long long i = blockIdx.x / ((long long)npb * c.Hk);
+  const unsigned x = blockIdx.x / (unsigned)npb, i = x / (unsigned)c.Hk;
+  const int pb = (int)(blockIdx.x - x * npb), g = (int)(x - i * c.Hk);
   int b, lo, hi;
   long long row;
-  if (!sel_row(c, p, row0 + i, &b, &row, &lo, &hi)) return;
+  if (!sel_row(c, p.window, b0, t0, i, &b, &row, &lo, &hi)) return;
   const int cur = hi - 1, end = hi < c.ldt ? hi : c.ldt;
   const int tid = threadIdx.x, l = tid & 15, team = tid >> 4;
   if (pb * PPB >= end) return;
-  u64 *out = key + (i * c.Hk + g) * c.ldt;
+  u64 *out = key + ((long long)i * c.Hk + g) * c.ldt;
   const int kd = (c.dk + 127) / 128 * 128;
   double acc[PPB / 16];
 #pragma unroll
@@ -221,9 +227,9 @@ __global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, lo
   for (int h0 = 0; h0 < p.G; h0 += 16) {
     const int nh = p.G - h0 < 16 ? p.G - h0 : 16;
     if (h0) __syncthreads();
-    for (int x = tid; x < nh * kd; x += 256) {
-      const int h = x / kd, d = x - h * kd;
-      s_q[x] = d < c.dk ? (float)((const T *)p.q)[row * p.ldq + (long long)(g * p.G + h0 + h) * c.dk + d] : 0.f;
+    for (int y = tid; y < nh * kd; y += 256) {
+      const int h = y / kd, d = y - h * kd;
+      s_q[y] = d < c.dk ? (float)((const T *)p.q)[row * p.ldq + (long long)(g * p.G + h0 + h) * c.dk + d] : 0.f;
     }
     __syncthreads();
 #pragma unroll
@@ -260,15 +266,15 @@ __global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, lo
 
 // The nsel largest of a row's keys by their digits of 8 bits from the top, the lower pages first where the last of them are
 // equal, in ascending order
-__global__ __launch_bounds__(256) void k_kv_pick(KvDev c, SelDev p, long long row0, const u64 *key) {
+__global__ __launch_bounds__(256) void k_kv_pick(KvDev c, SelDev p, int b0, int t0, const u64 *key) {
   __shared__ int s_n[256], s_w[4], s_t[4], s_b[3];
-  const int g = (int)(blockIdx.x % c.Hk);
-  const long long i = blockIdx.x / c.Hk;
+  const unsigned i = blockIdx.x / (unsigned)c.Hk;
+  const int g = (int)(blockIdx.x - i * c.Hk);
   int b, lo, hi;
   long long row;
-  if (!sel_row(c, p, row0 + i, &b, &row, &lo, &hi)) return;
+  if (!sel_row(c, p.window, b0, t0, i, &b, &row, &lo, &hi)) return;
   const int end = hi < c.ldt ? hi : c.ldt;
-  const u64 *k = key + (i * c.Hk + g) * c.ldt;
+  const u64 *k = key + ((long long)i * c.Hk + g) * c.ldt;
   int32_t *out = p.sel + (row * c.Hk + g) * p.nsel;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   u64 prefix = 0, mask = 0;
@@ -397,17 +403,18 @@ int bnh_kv_select(const bnh_kvcache *c, const bnh_kvattn *p, int first, int last
   hipStream_t s = bnh_stream(stream);
   for (long long r0 = 0; r0 < all; r0 += most) {
     const long long n = all - r0 < most ? all - r0 : most;
+    const int b0 = (int)(r0 / T), t0 = (int)(r0 % T);
     const dim3 grid((unsigned)(n * npb * c->Hk)), block(256);
     u64 *key = (u64 *)work;
     if (c->f16) {
-      if (v) hipLaunchKernelGGL((k_kv_score<h16, true>), grid, block, 0, s, d, e, npb, r0, key);
-      else hipLaunchKernelGGL((k_kv_score<h16, false>), grid, block, 0, s, d, e, npb, r0, key);
+      if (v) hipLaunchKernelGGL((k_kv_score<h16, true>), grid, block, 0, s, d, e, npb, b0, t0, key);
+      else hipLaunchKernelGGL((k_kv_score<h16, false>), grid, block, 0, s, d, e, npb, b0, t0, key);
     } else {
-      if (v) hipLaunchKernelGGL((k_kv_score<float, true>), grid, block, 0, s, d, e, npb, r0, key);
-      else hipLaunchKernelGGL((k_kv_score<float, false>), grid, block, 0, s, d, e, npb, r0, key);
+      if (v) hipLaunchKernelGGL((k_kv_score<float, true>), grid, block, 0, s, d, e, npb, b0, t0, key);
+      else hipLaunchKernelGGL((k_kv_score<float, false>), grid, block, 0, s, d, e, npb, b0, t0, key);
     }
     BNH_HIP(hipGetLastError());
-    hipLaunchKernelGGL(k_kv_pick, dim3((unsigned)(n * c->Hk)), block, 0, s, d, e, r0, key);
+    hipLaunchKernelGGL(k_kv_pick, dim3((unsigned)(n * c->Hk)), block, 0, s, d, e, b0, t0, key);
     BNH_HIP(hipGetLastError());
   }
   return 0;

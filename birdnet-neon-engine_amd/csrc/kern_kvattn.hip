@@ -25,24 +25,21 @@ __device__ __forceinline__ v4f mma(kv_vec<float, 8> a, kv_vec<float, 8> b, v4f c
 // the end over waves, and over the blocks of a split by k_kva_join. fp16: e^{s - m} goes into the product in two parts, 22 bits,
 // in units of 2^-12 so that the second part of small ones is no subnormal: the matrix cores wait for memory here.
 template <typename T, int D, int MT, bool V>
-__global__ __launch_bounds__(256) void k_kva(KvDev c, KvaDev p, int nrt, int nsp, long long blk0, float *part, float2 *pml) {
+__device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const KvaItem &it, int nrt, int2 *counts, float *part,
+                                         float2 *pml) {
   constexpr bool F16 = sizeof(T) == 2;
   constexpr int DKT = D / 32, CPL = D / 16, MR = 16 * MT;
   constexpr float OFF = F16 ? 12.f : 0.f;
   typedef kv_vec<T, 8> FV;
   __shared__ __attribute__((aligned(16))) float s_o[4][16 * (D + 4)];
   __shared__ float s_m[4][MR], s_l[4][MR];
-  const long long blk = blk0 + blockIdx.x, unit = blk / nsp;
-  const int sp = (int)(blk % nsp), tile = (int)(unit % nrt), g = (int)(unit / nrt % c.Hk), b = (int)(unit / nrt / c.Hk);
+  const int b = it.b, g = it.g, tile = it.tile;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int first, past, t0, t1, hx;
-  const int n = kv_rows(c, b, &first, &past);
-  kva_row(p, tile, 0, MR, &t0, &hx);
-  if (t0 >= n) return;
-  if (p.sel) t1 = t0;
-  else kva_row(p, tile, MR - 1, MR, &t1, &hx);
-  t1 = t1 < n ? t1 : n - 1;
+  const int first = it.first, past = it.past, n = it.n;
+  const KvaSpan span = kva_span(c, p, tile, MR, 32, n, past);
+  if (span.t0 >= n) return;
+  const int t0 = span.t0, t1 = span.t1, base = span.base;
   // queries
   FV qf[MT][DKT];
   int at[MT], since[MT];  // the last token that the lane's query sees, and the first
@@ -63,12 +60,8 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, KvaDev p, int nrt, int nsp
   // tokens
   const int all0 = p.window && past + t1 >= p.window ? past + t1 - p.window + 1 : 0;  // from here and ..
   const int all1 = past + t0;                                                         // .. up to here every query sees them
-  const long long cap = ((long long)c.ldt << c.sh) - 1;
-  const int j0 = p.window && past + t0 >= p.window ? past + t0 - p.window + 1 : 0, j1 = past + t1 < cap ? past + t1 : (int)cap;
-  const int base = j0 >> 5;
   const int *sel = p.sel ? p.sel + (((long long)first + t0) * c.Hk + g) * p.nsel : nullptr;
-  const int nt = p.sel ? (int)((((long long)p.nsel << (c.sh - 4)) + 1) >> 1) : j1 < j0 ? 0 : (j1 >> 5) - base + 1;
-  const int per = (nt + nsp - 1) / nsp, kt0 = sp * per, kt1 = kt0 + per < nt ? kt0 + per : nt;
+  const int kt0 = it.sp ? it.sp * it.per : 0, kt1 = it.per < span.nt - kt0 ? kt0 + it.per : span.nt;
 
   v4f o[MT][CPL];
   float mx[MT], l[MT];
@@ -231,6 +224,7 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, KvaDev p, int nrt, int nsp
       }
     }
   }
+  if (counts && tid == 0 && it.sp == 0) counts[((long long)b * c.Hk + g) * nrt + tile] = make_int2(it.item, it.parts);
   // the four waves' sums
 #pragma unroll
   for (int m = 0; m < MT; m++) {
@@ -263,7 +257,7 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, KvaDev p, int nrt, int nsp
 #pragma unroll
       for (int w = 0; w < 4; w++) y[i] = __builtin_fmaf(f[w], s_o[w][x * (D + 4) + c0 + i], y[i]);
     }
-    if (nsp == 1) {
+    if (it.parts == 1) {
       int t, h;
       kva_row(p, tile, row, MR, &t, &h);
       if (t >= n) continue;
@@ -280,7 +274,7 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, KvaDev p, int nrt, int nsp
           if (c0 + i < c.dv) out[c0 + i] = (T)(y[i] * inv);
       }
     } else {
-      const long long at = blk * MR + row;
+      const long long at = (long long)it.item * MR + row;
       if ((tid & 15) == 0) pml[at] = make_float2(top, sum);
       if (sum != 0.f)
 #pragma unroll
@@ -289,52 +283,138 @@ __global__ __launch_bounds__(256) void k_kva(KvDev c, KvaDev p, int nrt, int nsp
   }
 }
 
-// The blocks of a split: each row's sums over them, in order
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_kva_join(KvDev c, KvaDev p, int nrt, int nsp, int MR, long long unit0, const float *part,
-                                                  const float2 *pml) {
-  constexpr int L = D / 4, R = 256 / L;  // threads to a row, rows at a time
-  const int rg = MR / R > 0 ? MR / R : 1;
-  const long long unit = unit0 + blockIdx.x / rg;
-  const int tile = (int)(unit % nrt), g = (int)(unit / nrt % c.Hk), b = (int)(unit / nrt / c.Hk);
-  const int m = (int)(blockIdx.x % rg) * R + threadIdx.x / L, c0 = threadIdx.x % L * 4;
-  int first, past, t, h;
-  const int n = kv_rows(c, b, &first, &past);
-  if (m >= MR) return;
-  kva_row(p, tile, m, MR, &t, &h);
-  if (t >= n) return;
-  const long long at = unit * nsp * MR + m;
-  float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < nsp; s++) top = fmaxf(top, pml[at + (long long)s * MR].x);
-  const float to = top == -INFINITY ? 0.f : top;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < nsp; s++) {
-    const float2 z = pml[at + (long long)s * MR];
-    if (z.y == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(z.x - to);
-    const float4 x = *(const float4 *)(part + (at + (long long)s * MR) * D + c0);
-    sum = __builtin_fmaf(f, z.y, sum);
-    y.x = __builtin_fmaf(f, x.x, y.x), y.y = __builtin_fmaf(f, x.y, y.y);
-    y.z = __builtin_fmaf(f, x.z, y.z), y.w = __builtin_fmaf(f, x.w, y.w);
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T *out = (T *)p.o + ((long long)first + t) * p.ldo + ((long long)g * p.G + h) * c.dv + c0;
-  const float z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (c0 + i < c.dv) out[i] = (T)z[i];
+template <typename T, int D, int MT, bool V>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 128 && MT == 1 ? 3 : 1) void k_kva(KvDev c, KvaDev p, int B, int nrt, unsigned blk0, int2 *counts, float *part,
+                                             float2 *pml) {
+  KvaItem it;
+  if (kva_item(c, p, B, nrt, counts, 16 * MT, 32, blk0 + blockIdx.x, &it)) kva_tile<T, D, MT, V>(c, p, it, nrt, counts, part, pml);
 }
 
+// The parts of a split: each row's sums over them, in order. D / 4 lanes to a row, which read up to 8 of its parts at once, for
+// tiles of many rows
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_kva_join8(KvDev c, KvaDev p, int nrt, int MR, unsigned unit0, const int2 *counts,
+                                                   const float *part, const float2 *pml) {
+  constexpr int L = D / 4, R = 256 / L;  // lanes to a row; rows at a time
+  const unsigned unit = unit0 + blockIdx.x, sq = unit / (unsigned)nrt, b = sq / (unsigned)c.Hk;
+  const int tile = (int)(unit - sq * nrt), g = (int)(sq - b * c.Hk);
+  const int col = threadIdx.x % L * 4;
+  int first, past, t, h;
+  const int n = kv_rows(c, b, &first, &past);
+  kva_row(p, tile, 0, MR, &t, &h);
+  if (t >= n) return;
+  const int parts = kv_int(&counts->y, 2 * (long long)unit), item = kv_int(&counts->x, 2 * (long long)unit);
+  if (parts == 1) return;
+  for (int m = blockIdx.y * R + threadIdx.x / L; m < MR; m += gridDim.y * R) {
+    kva_row(p, tile, m, MR, &t, &h);
+    if (t >= n || col >= c.dv) continue;
+    const long long at = (long long)item * MR + m;
+    float top = -INFINITY, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += 8) {
+      float2 z[8];
+      float4 v[8];
+#pragma unroll
+      for (int s = 0; s < 8; s++) {
+        z[s] = make_float2(-INFINITY, 0.f);
+        if (s0 + s < parts)
+          z[s] = pml[at + (long long)(s0 + s) * MR], v[s] = *(const float4 *)(part + (at + (long long)(s0 + s) * MR) * D + col);
+      }
+      float now = top;
+#pragma unroll
+      for (int s = 0; s < 8; s++) now = fmaxf(now, z[s].x);
+      const float to = now == -INFINITY ? 0.f : now, a = __builtin_amdgcn_exp2f(top - to);
+      sum *= a;
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] *= a;
+      top = now;
+#pragma unroll
+      for (int s = 0; s < 8; s++) {
+        if (z[s].y == 0.f) continue;  // a part without a weight has stored nothing
+        const float f = __builtin_amdgcn_exp2f(z[s].x - to);
+        sum = __builtin_fmaf(f, z[s].y, sum);
+        y[0] = __builtin_fmaf(f, v[s].x, y[0]), y[1] = __builtin_fmaf(f, v[s].y, y[1]);
+        y[2] = __builtin_fmaf(f, v[s].z, y[2]), y[3] = __builtin_fmaf(f, v[s].w, y[3]);
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T *out = (T *)p.o + ((long long)first + t) * p.ldo + ((long long)g * p.G + h) * c.dv + col;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (col + i < c.dv) out[i] = (T)(y[i] * inv);
+  }
+}
+// For few rows: a block to a row, whose four waves share its parts
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_kva_join(KvDev c, KvaDev p, int nrt, int MR, unsigned unit0, const int2 *counts,
+                                                  const float *part, const float2 *pml) {
+  constexpr int N = D >= 64 ? D / 64 : 1;  // columns to a lane
+  typedef float VN __attribute__((ext_vector_type(N)));
+  __shared__ float s_f[4][kMostParts];
+  __shared__ __attribute__((aligned(16))) float s_y[4][D < 64 ? 64 : D];
+  const unsigned unit = unit0 + blockIdx.x, sq = unit / (unsigned)nrt, b = sq / (unsigned)c.Hk;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m = blockIdx.y, tile = (int)(unit - sq * nrt), g = (int)(sq - b * c.Hk);
+  int first, past, t, h;
+  const int n = kv_rows(c, b, &first, &past);
+  kva_row(p, tile, m, MR, &t, &h);
+  if (t >= n) return;  // the tile's first row is the sequence's if any is
+  const int parts = kv_int(&counts->y, 2 * (long long)unit), item = kv_int(&counts->x, 2 * (long long)unit);
+  if (parts == 1) return;
+  const long long at = (long long)item * MR + m;
+  // the parts' weights, in every wave
+  float top = -INFINITY, sum = 0.f;
+  float2 z[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    z[i] = make_float2(-INFINITY, 0.f);
+    if (lane + 64 * i < parts) z[i] = pml[at + (long long)(lane + 64 * i) * MR];
+    top = fmaxf(top, z[i].x);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  const float to = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const float f = z[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(z[i].x - to);
+    s_f[wave][lane + 64 * i] = f;
+    sum = __builtin_fmaf(f, z[i].y, sum);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  const int col = lane * N;
+  VN y = (VN)0.f;
+  if (col < D)
+#pragma unroll 8
+    for (int s = wave; s < parts; s += 4) {
+      const float f = s_f[wave][s];
+      const VN v = *(const VN *)(part + (at + (long long)s * MR) * D + col);
+      if (f != 0.f) y += f * v;
+    }
+  *(VN *)(s_y[wave] + col) = y;
+  __syncthreads();
+  if (wave || col >= c.dv) return;
+#pragma unroll
+  for (int i = 1; i < 4; i++) y += *(const VN *)(s_y[i] + col);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T *out = (T *)p.o + ((long long)first + t) * p.ldo + ((long long)g * p.G + h) * c.dv + col;
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if (col + i < c.dv) out[i] = (T)(y[i] * inv);
+}
+
+// How a call is cut
 KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
   KvaPlan r;
   const int d = c->dk > c->dv ? c->dk : c->dv, G = p->H / c->Hk;
   const long long m = p->nsel ? G : (long long)T * G;
   r.D = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
   r.tiled = !p->nsel && m > 64;
+  r.TK = 32;
   if (r.tiled) {
     r.DK = c->dk <= 64 && d <= 128 ? 64 : d <= 128 ? 128 : 256;
     r.D = c->dv <= 64 && d <= 128 ? 64 : d <= 128 ? 128 : 256;
-    r.MR = 32 * kva_waves(r.DK);
+    r.MR = 32 * kva_waves(c->f16, r.DK);
+    r.TK = kva_tokens(c->f16, r.DK);
   } else {
     const int big = c->f16 ? (r.D <= 128 ? 64 : 32) : r.D <= 64 ? 64 : r.D == 128 ? 32 : 16;
     r.MR = m <= 16 ? 16 : big;
@@ -346,39 +426,43 @@ KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
   if (p->nsel) tok = (long long)p->nsel * c->page;
   else if (p->window && p->window + r.MR < tok) tok = p->window + r.MR;
   const long long tiles = bnh_ceil_div(tok, 32) + 1;
-  long long s = bnh_ceil_div(r.tiled ? 512 : 1024, r.units);
-  if (s > tiles / 8) s = tiles / 8;
-  r.nsp = (int)(s < 1 ? 1 : s > 128 ? 128 : s);
+  // parts for the compute units (one block of the tiled form each, three of the other), where the tiles leave some without work
+  r.want = r.tiled ? 256 : 768;
+  r.least = r.tiled ? 256 / r.TK : 8;
+  r.split = r.units < 2 * r.want && tiles > (r.tiled ? 2 * r.least * r.TK / 32 : 2 * r.least);
+  r.items = r.split ? r.want + r.units + 1 : r.units;
   return r;
 }
-size_t plan_bytes(const KvaPlan &r) {
-  if (r.nsp == 1) return 0;
-  return (size_t)(r.units * r.nsp * r.MR * (4 * r.D + 8));
-}
-
 template <typename T, int D>
-int join_run(const KvDev &c, const KvaDev &p, const KvaPlan &r, const float *part, const float2 *pml, hipStream_t s) {
-  if (r.nsp == 1) return 0;
+int join_run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
+  if (!r.split) return 0;
   const long long most = bnh_most_blocks(256);
-  const int R = 256 / (D / 4), rg = r.MR / R > 0 ? r.MR / R : 1;
-  for (long long u0 = 0; u0 < r.units; u0 += most / rg) {
-    const long long u = r.units - u0 < most / rg ? r.units - u0 : most / rg;
-    hipLaunchKernelGGL((k_kva_join<T, D>), dim3((unsigned)(u * rg)), dim3(256), 0, s, c, p, r.nrt, r.nsp, r.MR, u0, part, pml);
+  // rows that a tile can have, as blocks, or as some passes of a few
+  const long long rows = p.nsel ? p.G : (long long)c.T * p.G;
+  const int R = 1024 / D, few = 16, y = r.tiled ? (r.MR / R < few ? r.MR / R : few) : (int)(rows < r.MR ? rows : r.MR);
+  for (long long u0 = 0; u0 < r.units; u0 += most) {
+    const dim3 grid((unsigned)(r.units - u0 < most ? r.units - u0 : most), y), block(256);
+    if (r.tiled)
+      hipLaunchKernelGGL((k_kva_join8<T, D>), grid, block, 0, s, c, p, r.nrt, r.MR, (unsigned)u0, kva_counts(r, work),
+                         kva_part(r, work), kva_ml(r, work));
+    else
+      hipLaunchKernelGGL((k_kva_join<T, D>), grid, block, 0, s, c, p, r.nrt, r.MR, (unsigned)u0, kva_counts(r, work),
+                         kva_part(r, work), kva_ml(r, work));
     BNH_HIP(hipGetLastError());
   }
   return 0;
 }
 template <typename T, int D, int MT, bool V>
 int rows_run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
-  float2 *pml = kva_ml(r, work);
-  float *part = kva_part(r, work);
-  const long long blocks = r.units * r.nsp, most = bnh_most_blocks(256);
-  for (long long b0 = 0; b0 < blocks; b0 += most) {
-    hipLaunchKernelGGL((k_kva<T, D, MT, V>), dim3((unsigned)(blocks - b0 < most ? blocks - b0 : most)), dim3(256), 0, s, c, p,
-                       r.nrt, r.nsp, b0, part, pml);
+  const long long most = bnh_most_blocks(256);
+  const int B = (int)(r.units / r.nrt / c.Hk);
+  for (long long b0 = 0; b0 < r.items; b0 += most) {
+    const long long n = r.items - b0 < most ? r.items - b0 : most;
+    hipLaunchKernelGGL((k_kva<T, D, MT, V>), dim3((unsigned)n), dim3(256), 0, s, c, p, B, r.nrt, (unsigned)b0, kva_counts(r, work),
+                       kva_part(r, work), kva_ml(r, work));
     BNH_HIP(hipGetLastError());
   }
-  return join_run<T, D>(c, p, r, part, pml, s);
+  return join_run<T, D>(c, p, r, work, s);
 }
 template <typename T, int D, bool V>
 int rows_go(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
@@ -391,10 +475,9 @@ template <typename T, bool V>
 int run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
   if (r.tiled) {
     if (kva_tiles(c, p, r, sizeof(T) == 2, V, work, s)) return -1;
-    const float2 *pml = kva_ml(r, work);
-    const float *part = kva_part(r, work);
-    return r.D == 64 ? join_run<T, 64>(c, p, r, part, pml, s) : r.D == 128 ? join_run<T, 128>(c, p, r, part, pml, s)
-                                                                           : join_run<T, 256>(c, p, r, part, pml, s);
+    return r.D == 64    ? join_run<T, 64>(c, p, r, work, s)
+           : r.D == 128 ? join_run<T, 128>(c, p, r, work, s)
+                        : join_run<T, 256>(c, p, r, work, s);
   }
   if (r.D == 32) return rows_go<T, 32, V>(c, p, r, work, s);
   if (r.D == 64) return rows_go<T, 64, V>(c, p, r, work, s);
@@ -415,7 +498,7 @@ extern "C" {
 
 size_t bnh_kv_attn_work_bytes(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows) {
   if (attn_check(c, p, T, B, rows)) return 0;
-  return plan_bytes(plan(c, p, T, B));
+  return kva_bytes(plan(c, p, T, B));
 }
 
 int bnh_kv_attn(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows, const int32_t *start, const int32_t *len,
@@ -426,11 +509,12 @@ int bnh_kv_attn(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int row
   const size_t es = c->f16 ? 2 : 4;
   BNH_REQ(kv_on(p->q, es) && kv_on(p->o, es) && kv_on(p->sel, 4));
   const KvaPlan r = plan(c, p, T, B);
-  const size_t need = plan_bytes(r);
+  const size_t need = kva_bytes(r);
+  BNH_REQ(r.items < (1LL << 31));
   BNH_REQ(need == 0 || (work && kv_on(work, 16) && work_bytes >= need));
   const KvDev d = kv_dev(c, T, rows, start, len);
   const float sc = fabsf(p->scale * 1.44269504f);  // a scale of 0 as one whose products round to 0
-  const KvaDev a = {p->q, p->o, p->sel, p->ldq, p->ldo, p->H / c->Hk, p->window, p->nsel, sc < 1e-37f ? 1e-37f : sc, p->scale < 0};
+  const KvaDev a = {p->q, p->o, p->sel, p->ldq, p->ldo, p->H / c->Hk, p->window, p->nsel, r.want, r.least, sc < 1e-37f ? 1e-37f : sc, p->scale < 0};
   const int ve = 16 / (int)es, cpl = r.tiled ? 8 : r.D / 16;
   bool v = c->dk % 8 == 0 && c->dv % cpl == 0 && c->k_ps % ve == 0 && c->v_ps % ve == 0 && p->ldq % ve == 0 &&
            p->ldo % (cpl < ve ? cpl : ve) == 0;

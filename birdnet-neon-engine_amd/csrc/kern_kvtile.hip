@@ -41,18 +41,15 @@ __device__ __forceinline__ float both(float x) {
   const u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// tokens to a tile
-constexpr int kvt_tokens(bool f16, int DK) { return f16 && DK < 256 ? 64 : 32; }
-
 // fp16: the waves of a block are two groups, one wave of each on every SIMD, half a tile apart: while one multiplies (its
 // last tile's values and the next one's scores), the other takes exponentials. Waves in step would all want the matrix cores
 // and then all want the exponentials: 17,280 rows of 12 heads of 128 took 1,292 us so. fp32 products take ten times as
 // long as the exponentials, and the groups go in step.
 template <typename T, int DK, int DV, int NW, int NG, bool V>
-__global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int B, int nrt, int nsp, long long blk0, float *part,
-                                                         float2 *pml) {
+__device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const KvaItem &it, int nrt, int2 *counts, float *part,
+                                         float2 *pml) {
   constexpr bool F16 = sizeof(T) == 2, PP = F16 && NW == 8;
-  constexpr int VE = 16 / sizeof(T), TK = kvt_tokens(F16, DK), ST = TK / 32, NT = 64 * NW, MR = 32 * NW;
+  constexpr int VE = 16 / sizeof(T), TK = kva_tokens(F16, DK), ST = TK / 32, NT = 64 * NW, MR = 32 * NW;
   constexpr int KC = DK / VE, VC = DV / VE;                    // pieces of a row
   constexpr int KP = NT / KC, VP = NT / VC;                    // tokens that one load of all threads covers
   constexpr int NK = TK / KP, NV = TK / VP, GT = TK / NG;
@@ -63,23 +60,21 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
   constexpr int KB = TK * KC * 16, VB = TK * VC * 16;          // bytes of a tile
   __shared__ PV s_kb[NB][TK * KC], s_vb[NB][TK * VC];
   __shared__ int s_bad[3];  // the first and last tile with values that are not finite; whether the outputs show any
-  const long long blk = blk0 + blockIdx.x, unit = blk / nsp;
-  // the last rows, which see most, of all heads and sequences first
-  const int sp = (int)(blk % nsp), g = (int)(unit % c.Hk), b = (int)(unit / c.Hk % B), tile = nrt - 1 - (int)(unit / c.Hk / B);
+  const int b = it.b, g = it.g, tile = it.tile;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int first, past, t0, t1, tx, hx;
-  const int n = kv_rows(c, b, &first, &past);
-  kva_row(p, tile, 0, MR, &t0, &hx);
-  if (t0 >= n) return;
-  kva_row(p, tile, MR - 1, MR, &t1, &hx);
-  t1 = t1 < n ? t1 : n - 1;
+  const int first = it.first, past = it.past, n = it.n;
+  int tx, hx;
+  const KvaSpan span = kva_span(c, p, tile, MR, TK, n, past);
+  if (span.t0 >= n) return;
+  const int j1 = span.j1, end = span.base + span.nt;
+  const int kt0 = it.sp ? span.base + it.sp * it.per : span.base, kt1 = it.per < end - kt0 ? kt0 + it.per : end;
   kva_row(p, tile, 32 * wave + lr, MR, &tx, &hx);
   const bool mine = tx < n;
   const int at = mine ? past + tx : -1, since = p.window && at >= p.window ? at - p.window + 1 : 0;
   FV qf[DK / 16];
   {
-    const T *q = (const T *)p.q + ((long long)first + (mine ? tx : t0)) * p.ldq + ((long long)g * p.G + (mine ? hx : 0)) * c.dk;
+    const T *q = (const T *)p.q + ((long long)first + (mine ? tx : span.t0)) * p.ldq + ((long long)g * p.G + (mine ? hx : 0)) * c.dk;
 #pragma unroll
     for (int d = 0; d < DK / 16; d++) {
       qf[d] = kv_ld<T, 8, V>(q, 16 * d + 8 * hi, mine ? c.dk : 0);
@@ -94,10 +89,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
   const bool idle = w0 >= n;
   const int all0 = p.window && past + w1 >= p.window ? past + w1 - p.window + 1 : 0, all1 = past + w0;
   const int see0 = p.window && past + w0 >= p.window ? past + w0 - p.window + 1 : 0, see1 = past + w1;
-  const long long cap = ((long long)c.ldt << c.sh) - 1;
-  const int j0 = p.window && past + t0 >= p.window ? past + t0 - p.window + 1 : 0, j1 = past + t1 < cap ? past + t1 : (int)cap;
-  const int base = j0 / TK, nt = j1 < j0 ? 0 : j1 / TK - base + 1;
-  const int per = (nt + nsp - 1) / nsp, kt0 = base + sp * per, kt1 = sp * per + per < nt ? kt0 + per : base + nt;
 
   v16f o[DV / 32];
   float mx, l;
@@ -333,9 +324,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
           for (int e = 0; e < 8; e++) ph[i][e] = (T)0;
         // tile kt0 - 1's values, which have no page and are zeros, lie in the last place
         issue(kt0, 0, 2);
-        RQ_WAIT_VM(0);
-        clean(kt0 - 1, 0, 2, pk, pv);
         issue(kt0 + 1, 1, 0);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK + NV) : "memory");
+        clean(kt0 - 1, 0, 2, pv, pw);
         prepare(kt0 + 2);
         __syncthreads();
         if (late) __syncthreads();
@@ -410,12 +401,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
         }
       }
     }
-    bool odd = false;
+    float odd = 0.f;
 #pragma unroll
     for (int i = 0; i < DV / 32; i++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) odd = odd || !kv_finite(o[i][r]);
-    if (odd) s_bad[2] = 1;
+      for (int r = 0; r < 16; r++) odd = __builtin_fmaf(o[i][r], 0.f, odd);
+    if (odd != 0.f) s_bad[2] = 1;
     __syncthreads();
     careful = s_bad[2] != 0;
   }
@@ -423,10 +414,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
     // Tile by tile through registers, where what is not finite is taken out of the values, and pieces need no alignment
     clear();
     const int kk = tid / KC, kx = tid % KC, vk = tid / VC, vx = tid % VC;
-    for (int kt = kt0; kt < kt1; kt++) {
-#pragma unroll
-      for (int i = 0; i < NG; i++) pc[i] = page_of(kt * TK + GT * i);
-      PV kn[NK], vn[NV];
+    PV kn[NK], vn[NV];
+    auto load = [&](int kt) {
 #pragma unroll
       for (int i = 0; i < NK; i++) {
         const int j = kt * TK + i * KP + kk, pg = kv_page(c, b, j >> c.sh);
@@ -437,6 +426,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
         const int j = kt * TK + i * VP + vk, pg = kv_page(c, b, j >> c.sh);
         vn[i] = kv_ld<T, VE, V>(vh + (pg < 0 ? 0 : pg) * c.v_ps + (j & inpage) * c.dv, vx * VE, pg < 0 ? 0 : c.dv);
       }
+    };
+    if (kt0 < kt1) load(kt0);
+    for (int kt = kt0; kt < kt1; kt++) {
+#pragma unroll
+      for (int i = 0; i < NG; i++) pc[i] = page_of(kt * TK + GT * i);
       kv_vec<T, 2> mk = {(T)0, (T)0};
 #pragma unroll
       for (int i = 0; i < NV; i++) kv_mark<T, VE>(vn[i], mk);
@@ -452,6 +446,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
       for (int i = 0; i < NK; i++) s_kb[q][piece<KC>(i * KP + kk, kx)] = kn[i];
 #pragma unroll
       for (int i = 0; i < NV; i++) s_vb[q][piece<VC>(i * VP + vk, vx)] = vn[i];
+      if (kt + 1 < kt1) load(kt + 1);
       __syncthreads();
       if (!seen(kt)) continue;
       scores(q);
@@ -494,8 +489,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
     }
   }
   l += __shfl_xor(l, 32);
+  if (counts && tid == 0 && it.sp == 0) counts[((long long)b * c.Hk + g) * nrt + tile] = make_int2(it.item, it.parts);
   if (!mine) return;
-  if (nsp == 1) {
+  if (it.parts == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *out = (T *)p.o + ((long long)first + tx) * p.ldo + ((long long)g * p.G + hx) * c.dv;
 #pragma unroll
@@ -515,7 +511,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
         }
       }
   } else {
-    const long long x = ((((long long)b * c.Hk + g) * nrt + tile) * nsp + sp) * MR + 32 * wave + lr;
+    const long long x = (long long)it.item * MR + 32 * wave + lr;
     if (hi == 0) pml[x] = make_float2(mx, l);
     if (l != 0.f)
 #pragma unroll
@@ -528,27 +524,37 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int 
 }
 
 template <typename T, int DK, int DV, int NW, int NG, bool V>
+__global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int B, int nrt, unsigned blk0, int2 *counts,
+                                                         float *part, float2 *pml) {
+  KvaItem it;
+  if (kva_item(c, p, B, nrt, counts, 32 * NW, kva_tokens(sizeof(T) == 2, DK), blk0 + blockIdx.x, &it))
+    kvt_item<T, DK, DV, NW, NG, V>(c, p, it, nrt, counts, part, pml);
+}
+
+template <typename T, int DK, int DV, int NG, bool V>
 int run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
-  const long long blocks = r.units * r.nsp, most = bnh_most_blocks(64 * NW);
+  constexpr int NW = kva_waves(sizeof(T) == 2, DK);
+  const long long most = bnh_most_blocks(64 * NW);
   const int B = (int)(r.units / r.nrt / c.Hk);
-  for (long long b0 = 0; b0 < blocks; b0 += most) {
-    hipLaunchKernelGGL((k_kvt<T, DK, DV, NW, NG, V>), dim3((unsigned)(blocks - b0 < most ? blocks - b0 : most)), dim3(64 * NW),
-                       0, s, c, p, B, r.nrt, r.nsp, b0, kva_part(r, work), kva_ml(r, work));
+  for (long long b0 = 0; b0 < r.items; b0 += most) {
+    const long long n = r.items - b0 < most ? r.items - b0 : most;
+    hipLaunchKernelGGL((k_kvt<T, DK, DV, NW, NG, V>), dim3((unsigned)n), dim3(64 * NW), 0, s, c, p, B, r.nrt, (unsigned)b0,
+                       kva_counts(r, work), kva_part(r, work), kva_ml(r, work));
     BNH_HIP(hipGetLastError());
   }
   return 0;
 }
 template <typename T, bool ONE, bool V>
 int widths(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
-  constexpr int NG = ONE ? 1 : kvt_tokens(sizeof(T) == 2, 128) / 16;
-  if (r.DK == 256) return run<T, 256, 256, 4, ONE ? 1 : 2, V>(c, p, r, work, s);
-  if (r.DK == 64) return r.D == 64 ? run<T, 64, 64, 8, NG, V>(c, p, r, work, s) : run<T, 64, 128, 8, NG, V>(c, p, r, work, s);
-  return r.D == 64 ? run<T, 128, 64, 8, NG, V>(c, p, r, work, s) : run<T, 128, 128, 8, NG, V>(c, p, r, work, s);
+  constexpr int NG = ONE ? 1 : kva_tokens(sizeof(T) == 2, 128) / 16;
+  if (r.DK == 256) return run<T, 256, 256, ONE ? 1 : 2, V>(c, p, r, work, s);
+  if (r.DK == 64) return r.D == 64 ? run<T, 64, 64, NG, V>(c, p, r, work, s) : run<T, 64, 128, NG, V>(c, p, r, work, s);
+  return r.D == 64 ? run<T, 128, 64, NG, V>(c, p, r, work, s) : run<T, 128, 128, NG, V>(c, p, r, work, s);
 }
 template <typename T>
 int go(const KvDev &c, const KvaDev &p, const KvaPlan &r, bool v, void *work, hipStream_t s) {
   if (!v) return widths<T, false, false>(c, p, r, work, s);
-  return 1 << c.sh >= kvt_tokens(sizeof(T) == 2, r.DK) ? widths<T, true, true>(c, p, r, work, s) : widths<T, false, true>(c, p, r, work, s);
+  return 1 << c.sh >= kva_tokens(sizeof(T) == 2, r.DK) ? widths<T, true, true>(c, p, r, work, s) : widths<T, false, true>(c, p, r, work, s);
 }
 
 }  // namespace
