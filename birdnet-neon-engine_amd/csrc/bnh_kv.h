@@ -43,20 +43,51 @@ __device__ __forceinline__ int kv_page(const KvDev &c, int b, int i) {
 // or to 16 bytes
 template <typename T, int N>
 using kv_vec = T __attribute__((ext_vector_type(N), aligned(sizeof(T) * N < 16 ? sizeof(T) * N : 16)));
-template <typename T, int N, bool V>
-__device__ __forceinline__ kv_vec<T, N> kv_ld(const T *p, int c, int n) {
+// Where they are not: N values from a place in the row, the last ones for a c near its end, so that every load is one; and what
+// kv_ld gives of them, once they are there (a row of fewer than N values is read value by value)
+template <typename T, int N>
+__device__ __forceinline__ kv_vec<T, N> kv_raw(const T *p, int c, int n) {
   kv_vec<T, N> r;
-  if (V) {
-#pragma unroll
-    for (int i = 0; i < N; i++) r[i] = (T)0;
-    if (c < n) r = *(const kv_vec<T, N> *)(p + c);
-  } else if (c + N <= n) {
-    __builtin_memcpy(&r, p + c, N * sizeof(T));
+  if (n >= N) {
+    __builtin_memcpy(&r, p + (c <= n - N ? c : c < n ? n - N : 0), N * sizeof(T));
   } else {
 #pragma unroll
     for (int i = 0; i < N; i++) r[i] = c + i < n ? p[c + i] : (T)0;
   }
   return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ kv_vec<T, N> kv_fix(kv_vec<T, N> r, int c, int n) {
+  constexpr int W = N * sizeof(T) / 4;
+  static_assert(W >= 1 && W * 4 == (int)(N * sizeof(T)), "whole words");
+  typedef uint32_t Words __attribute__((ext_vector_type(W)));
+  Words w = __builtin_bit_cast(Words, r);
+  if (n >= N && n % N) {  // the same for all lanes
+    const int s = c > n - N && c < n ? (c - (n - N)) * (int)sizeof(T) : 0;  // bytes too early
+    if (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < W; i++) w[i] = s & 2 ? __builtin_amdgcn_alignbit(i + 1 < W ? w[i + 1] : 0, w[i], 16) : w[i];
+    }
+#pragma unroll
+    for (int d = 1; d < W; d *= 2)
+#pragma unroll
+      for (int i = 0; i < W; i++) w[i] = s & 4 * d ? (i + d < W ? w[i + d] : 0) : w[i];
+  }
+#pragma unroll
+  for (int i = 0; i < W; i++) w[i] = c < n ? w[i] : 0;
+  return __builtin_bit_cast(kv_vec<T, N>, w);
+}
+template <typename T, int N, bool V>
+__device__ __forceinline__ kv_vec<T, N> kv_ld(const T *p, int c, int n) {
+  if constexpr (V) {
+    kv_vec<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; i++) r[i] = (T)0;
+    if (c < n) r = *(const kv_vec<T, N> *)(p + c);
+    return r;
+  } else {
+    return kv_fix<T, N>(kv_raw<T, N>(p, c, n), c, n);
+  }
 }
 
 // the host's checks that every entry makes, and the device's descriptor

@@ -426,9 +426,12 @@ KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
   if (p->nsel) tok = (long long)p->nsel * c->page;
   else if (p->window && p->window + r.MR < tok) tok = p->window + r.MR;
   const long long tiles = bnh_ceil_div(tok, 32) + 1;
-  // parts for the compute units (one block of the tiled form each, three of the other), where the tiles leave some without work
-  r.want = r.tiled ? 256 : 768;
-  r.least = r.tiled ? 256 / r.TK : 8;
+  // parts for the compute units where tiles leave some without work: one block each of the tiled form, with room for the last
+  // parts of tiles (24 chunks of up to 120 rows: 37 + 13 us, 44 + 15 with 256), four of the other (64 rows over up to a day: 223 +
+  // 6 us, 229 + 6 with 768, 241 + 5 with 512), of 512 tokens at least, or what is joined costs more (one row over a day: 24 + 7 us
+  // in 406 parts, 23 + 9 in 732)
+  r.want = r.tiled ? 192 : 1024;
+  r.least = r.tiled ? 256 / r.TK : p->nsel ? 8 : 16;
   r.split = r.units < 2 * r.want && tiles > (r.tiled ? 2 * r.least * r.TK / 32 : 2 * r.least);
   r.items = r.split ? r.want + r.units + 1 : r.units;
   return r;

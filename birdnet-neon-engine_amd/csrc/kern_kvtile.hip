@@ -415,22 +415,29 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
     clear();
     const int kk = tid / KC, kx = tid % KC, vk = tid / VC, vx = tid % VC;
     PV kn[NK], vn[NV];
+    bool kin[NK], vin[NV];  // whether there is a page
     auto load = [&](int kt) {
 #pragma unroll
       for (int i = 0; i < NK; i++) {
         const int j = kt * TK + i * KP + kk, pg = kv_page(c, b, j >> c.sh);
-        kn[i] = kv_ld<T, VE, V>(kh + (pg < 0 ? 0 : pg) * c.k_ps + (j & inpage) * c.dk, kx * VE, pg < 0 ? 0 : c.dk);
+        kn[i] = kv_raw<T, VE>(kh + (pg < 0 ? 0 : pg) * c.k_ps + (j & inpage) * c.dk, kx * VE, c.dk);
+        kin[i] = pg >= 0;
       }
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         const int j = kt * TK + i * VP + vk, pg = kv_page(c, b, j >> c.sh);
-        vn[i] = kv_ld<T, VE, V>(vh + (pg < 0 ? 0 : pg) * c.v_ps + (j & inpage) * c.dv, vx * VE, pg < 0 ? 0 : c.dv);
+        vn[i] = kv_raw<T, VE>(vh + (pg < 0 ? 0 : pg) * c.v_ps + (j & inpage) * c.dv, vx * VE, c.dv);
+        vin[i] = pg >= 0;
       }
     };
     if (kt0 < kt1) load(kt0);
     for (int kt = kt0; kt < kt1; kt++) {
 #pragma unroll
       for (int i = 0; i < NG; i++) pc[i] = page_of(kt * TK + GT * i);
+#pragma unroll
+      for (int i = 0; i < NK; i++) kn[i] = kv_fix<T, VE>(kn[i], kin[i] ? kx * VE : c.dk, c.dk);
+#pragma unroll
+      for (int i = 0; i < NV; i++) vn[i] = kv_fix<T, VE>(vn[i], vin[i] ? vx * VE : c.dv, c.dv);
       kv_vec<T, 2> mk = {(T)0, (T)0};
 #pragma unroll
       for (int i = 0; i < NV; i++) kv_mark<T, VE>(vn[i], mk);
