@@ -38,17 +38,17 @@ __device__ __forceinline__ void turn(int pos, float freq, float *cs, float *sn) 
   *cs = k == 1 || k == 2 ? -a : a;
   *sn = k >= 2 ? -b : b;
 }
-// the smaller and the larger of two, NaN where one is
-template <typename T>
-__device__ __forceinline__ T low(T a, T b) { return a != a ? a : b != b ? b : a < b ? a : b; }
-template <typename T>
-__device__ __forceinline__ T high(T a, T b) { return a != a ? a : b != b ? b : a > b ? a : b; }
+// the smaller and the larger of two, value by value, NaN where one is
+template <typename W>
+__device__ __forceinline__ W low(W a, W b) { return __builtin_elementwise_minimum(a, b); }
+template <typename W>
+__device__ __forceinline__ W high(W a, W b) { return __builtin_elementwise_maximum(a, b); }
 
 // A unit: VEC values at `a` and VEC more at `b` (pairs 0: the partners; pairs 1 and values past rd: the next ones)
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, int nu, int b0, int pt0) {
   typedef T W __attribute__((ext_vector_type(VEC), aligned(sizeof(T) * VEC)));
-  __shared__ T s_lo[512 * VEC], s_hi[512 * VEC];
+  __shared__ __attribute__((aligned(16))) T s_lo[512 * VEC], s_hi[512 * VEC];
   const unsigned sq = blockIdx.x / (unsigned)c.Hk;  // sequences and pages of a launch from (b0, pt0) on
   const int g = (int)(blockIdx.x - sq * c.Hk);
   const unsigned b1 = sq / (unsigned)npt, pt1 = sq - b1 * npt;
@@ -120,9 +120,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, i
         }
         if (bound) {
 #pragma unroll
-          for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int i = 0; i < VEC; i++) lo[j][i] = low(lo[j][i], x[j][i]), hi[j][i] = high(hi[j][i], x[j][i]);
+          for (int j = 0; j < 2; j++) lo[j] = low(lo[j], x[j]), hi[j] = high(hi[j], x[j]);
         }
       };
       if (page >= 0) rotate((const T *)p.k + r * p.ldk + g * c.dk, kc + (long long)(off + t - t0) * c.dk, c.lo != nullptr);
@@ -132,12 +130,26 @@ __global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, i
     }
   }
   if (page < 0) return;
-  // values as they are
+  // values as they are, 16 bytes at a time, the last ones of a row wherever they begin
   T *vc = (T *)c.v + page * c.v_ps + (((long long)g << c.sh) + off) * c.dv;
-  const int nv = c.dv / VEC, items = (t1 - t0) * nv;
-  for (int i = tid; i < items; i += 256) {
-    const int t = i / nv, e = (i - t * nv) * VEC;
-    *(W *)(vc + (long long)t * c.dv + e) = *(const W *)((const T *)p.v + ((long long)first + t0 + t) * p.ldv + g * c.dv + e);
+  constexpr int VE = 16 / sizeof(T);
+  if (c.dv < VE) {
+    for (int i = tid; i < (t1 - t0) * c.dv; i += 256) {
+      const int t = i / c.dv, e = i - t * c.dv;
+      vc[(long long)t * c.dv + e] = ((const T *)p.v)[((long long)first + t0 + t) * p.ldv + g * c.dv + e];
+    }
+  } else {
+    const int nv = (c.dv + VE - 1) / VE, step = 256 / nv, e0 = tid % nv * VE, e = VEC > 1 || e0 + VE <= c.dv ? e0 : c.dv - VE;
+    for (int t = tid / nv; t < t1 - t0 && tid < step * nv; t += step) {
+      const T *x = (const T *)p.v + ((long long)first + t0 + t) * p.ldv + g * c.dv + e;
+      if constexpr (VEC > 1) {
+        *(W *)(vc + (long long)t * c.dv + e) = *(const W *)x;
+      } else {
+        uint4 y;
+        __builtin_memcpy(&y, x, 16);
+        __builtin_memcpy(vc + (long long)t * c.dv + e, &y, 16);
+      }
+    }
   }
   if (!c.lo) return;
   if (rl < RL) {
@@ -148,13 +160,25 @@ __global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, i
     }
   }
   __syncthreads();
-  if (tid < c.dk) {
-    const long long at = ((long long)page * c.Hk + g) * c.dk + tid;
-    T l = s_lo[tid], h = s_hi[tid];
-    const int used = RL < t1 - t0 ? RL : t1 - t0;
-    for (int i = 1; i < used; i++) l = low(l, s_lo[i * c.dk + tid]), h = high(h, s_hi[i * c.dk + tid]);
-    if (off) l = low(l, ((const T *)c.lo)[at]), h = high(h, ((const T *)c.hi)[at]);
-    ((T *)c.lo)[at] = l, ((T *)c.hi)[at] = h;
+  // columns (two of fp16 where rows of LDS allow it), over groups of the rows and then over the groups
+  constexpr int PK = VEC > 1 && sizeof(T) == 2 ? 2 : 1;
+  typedef T P __attribute__((ext_vector_type(PK)));
+  const int cols = c.dk / PK, groups = 256 / cols, col = tid % cols, grp = tid / cols;
+  const int used = RL < t1 - t0 ? RL : t1 - t0;
+  P *pl = (P *)s_lo + col, *ph = (P *)s_hi + col;
+  if (grp < groups && grp < used) {
+    P l = pl[grp * cols], h = ph[grp * cols];
+    for (int i = grp + groups; i < used; i += groups) l = low(l, pl[i * cols]), h = high(h, ph[i * cols]);
+    pl[grp * cols] = l, ph[grp * cols] = h;
+  }
+  __syncthreads();
+  if (grp == 0) {
+    const long long at = ((long long)page * c.Hk + g) * c.dk + PK * col;
+    P l = pl[0], h = ph[0];
+    for (int i = 1; i < groups && i < used; i++) l = low(l, pl[i * cols]), h = high(h, ph[i * cols]);
+    P *gl = (P *)((T *)c.lo + at), *gh = (P *)((T *)c.hi + at);
+    if (off) l = low(l, *gl), h = high(h, *gh);
+    *gl = l, *gh = h;
   }
 }
 
@@ -372,6 +396,7 @@ int bnh_kv_append(const bnh_kvcache *c, const bnh_rotary *r, const void *k, int 
   const int rd = r ? r->rd : 0, pairs = r ? r->pairs : 0, ve = 16 / (int)es;
   const AppDev p = {k, v, q, qr, r ? r->freq : nullptr, r ? r->pos : nullptr, ldk, ldv, ldq, ldr, q ? H / c->Hk : 0, rd, pairs};
   bool vec = c->dk % (2 * ve) == 0 && c->dv % ve == 0 && rd % (2 * ve) == 0 && c->k_ps % ve == 0 && c->v_ps % ve == 0;
+  vec = vec && kv_on(c->lo, 4) && kv_on(c->hi, 4);
   for (const void *x : {(const void *)c->k, (const void *)c->v, k, v, q, (const void *)qr}) vec = vec && kv_on(x, 16);
   vec = vec && ldk % ve == 0 && ldv % ve == 0 && (!q || (ldq % ve == 0 && ldr % ve == 0));
   hipStream_t s = bnh_stream(stream);
