@@ -153,6 +153,6 @@ static inline size_t kva_bytes(const KvaPlan &r) {
 // tokens to a tile of the tiled form, and waves to a block of it (32 rows each)
 constexpr int kva_tokens(bool f16, int DK) { return f16 && DK < 256 ? 64 : 32; }
 constexpr int kva_waves(bool f16, int DK) { return f16 && DK < 256 ? 8 : 4; }
-// the tiled form's launch (kern_kvtile.hip); v: everything is aligned to 16 bytes, widths too
-int kva_tiles(const KvDev &c, const KvaDev &p, const KvaPlan &r, bool f16, bool v, void *work, hipStream_t s);
+// the tiled form's launch (kern_kvtile.hip); w: what everything is aligned to, widths too, in bytes: 16, 4 or 2
+int kva_tiles(const KvDev &c, const KvaDev &p, const KvaPlan &r, bool f16, int w, void *work, hipStream_t s);
 #endif

@@ -474,14 +474,15 @@ int rows_go(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipSt
     if (r.MR > 16) return rows_run<T, D, big, V>(c, p, r, work, s);
   return rows_run<T, D, 1, V>(c, p, r, work, s);
 }
+template <typename T>
+int tiles_run(const KvDev &c, const KvaDev &p, const KvaPlan &r, int w, void *work, hipStream_t s) {
+  if (kva_tiles(c, p, r, sizeof(T) == 2, w, work, s)) return -1;
+  return r.D == 64    ? join_run<T, 64>(c, p, r, work, s)
+         : r.D == 128 ? join_run<T, 128>(c, p, r, work, s)
+                      : join_run<T, 256>(c, p, r, work, s);
+}
 template <typename T, bool V>
 int run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
-  if (r.tiled) {
-    if (kva_tiles(c, p, r, sizeof(T) == 2, V, work, s)) return -1;
-    return r.D == 64    ? join_run<T, 64>(c, p, r, work, s)
-           : r.D == 128 ? join_run<T, 128>(c, p, r, work, s)
-                        : join_run<T, 256>(c, p, r, work, s);
-  }
   if (r.D == 32) return rows_go<T, 32, V>(c, p, r, work, s);
   if (r.D == 64) return rows_go<T, 64, V>(c, p, r, work, s);
   if (r.D == 128) return rows_go<T, 128, V>(c, p, r, work, s);
@@ -523,6 +524,12 @@ int bnh_kv_attn(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int row
            p->ldo % (cpl < ve ? cpl : ve) == 0;
   for (const void *x : {p->q, (const void *)p->o, (const void *)c->k, (const void *)c->v}) v = v && kv_on(x, 16);
   hipStream_t s = bnh_stream(stream);
+  if (r.tiled) {
+    bool four = !c->f16 || (c->dk % 2 == 0 && c->dv % 2 == 0 && c->k_ps % 2 == 0 && c->v_ps % 2 == 0);
+    for (const void *x : {(const void *)c->k, (const void *)c->v}) four = four && kv_on(x, 4);
+    const int w = v ? 16 : four ? 4 : 2;
+    return c->f16 ? tiles_run<h16>(d, a, r, w, work, s) : tiles_run<float>(d, a, r, w, work, s);
+  }
   if (c->f16) return v ? run<h16, true>(d, a, r, work, s) : run<h16, false>(d, a, r, work, s);
   return v ? run<float, true>(d, a, r, work, s) : run<float, false>(d, a, r, work, s);
 }

@@ -45,10 +45,13 @@ __device__ __forceinline__ float both(float x) {
 // last tile's values and the next one's scores), the other takes exponentials. Waves in step would all want the matrix cores
 // and then all want the exponentials: 17,280 rows of 12 heads of 128 took 1,292 us so. fp32 products take ten times as
 // long as the exponentials, and the groups go in step.
-template <typename T, int DK, int DV, int NW, int NG, bool V>
+// W: bytes of a lane's load, which everything is aligned to: 16, 4, or 2 (odd widths of fp16), where all goes through registers.
+// 8,000 rows of 12 heads of 128 and 126: 268 us by fours, 512 us through registers; fp32, 16 heads of 64 and 97, 256 tokens seen:
+// 53 us and 68
+template <typename T, int DK, int DV, int NW, int NG, int W>
 __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const KvaItem &it, int nrt, int2 *counts, float *part,
                                          float2 *pml) {
-  constexpr bool F16 = sizeof(T) == 2, PP = F16 && NW == 8;
+  constexpr bool F16 = sizeof(T) == 2, PP = F16 && NW == 8, V = W == 16;
   constexpr int VE = 16 / sizeof(T), TK = kva_tokens(F16, DK), ST = TK / 32, NT = 64 * NW, MR = 32 * NW;
   constexpr int KC = DK / VE, VC = DV / VE;                    // pieces of a row
   constexpr int KP = NT / KC, VP = NT / VC;                    // tokens that one load of all threads covers
@@ -224,8 +227,8 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
   clear();
   if (tid == 0) s_bad[0] = 0x7fffffff, s_bad[1] = -1, s_bad[2] = 0;
   __syncthreads();
-  bool careful = !V;
-  if constexpr (V) {
+  bool careful = W == 2;
+  if constexpr (W > 2) {
     // Tiles go from memory into LDS by themselves. Unit u is the keys of tile u and the values of tile u - LAG, LAG 1 where the
     // second product is a tile behind the first. A load of all threads covers KP (VP) tokens; a lane's piece of it lands in the
     // order of the lanes, so the lane asks for the piece that belongs there. Columns past a row's end are its first piece once
@@ -233,11 +236,15 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
     // no row sees are zeros once their place has been filled from somewhere, by the lanes that did. Keys and values that are not
     // finite show in the outputs: the rows are done again then
     constexpr int LAG = PP ? 1 : 0;
+    constexpr int E = W / (int)sizeof(T), PE = VE / E;           // elements of a load, loads of a piece
+    constexpr int KL = KC * PE, VL = VC * PE;                    // loads of a row
+    constexpr int KP = NT / KL, VP = NT / VL, NK = TK / KP, NV = TK / VP;
+    constexpr int KF = NG == 1 ? 1 : KP < 16 ? NG : NK, VF = NG == 1 ? 1 : VP < 16 ? NG : NV;  // loads that begin in groups of their own
     int pk[NG], pv[NG], pw[NG];  // the pages of unit u's keys, and of the two before
 #pragma unroll
     for (int i = 0; i < NG; i++) pk[i] = pv[i] = pw[i] = -1;
-    const int kk = tid / KC, vk = tid / VC;
-    const int kg = wave * 64 / KC / 16, vg = wave * 64 / VC / 16;  // a wave's part of a load lies in one group of 16 tokens
+    const int vk = tid / VL;
+    const int kg = wave * 64 / KL / 16, vg = wave * 64 / VL / 16;  // a wave's part of a load lies in one group of 16 tokens
     auto page = [&](const int (&pg)[NG], int i, int P, int w) {
       if (NG == 1) return pg[0];
       int r = pg[i * P / 16];
@@ -245,21 +252,21 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
       for (int x = 1; x < P / 16; x++) r = w == x ? pg[(i * P / 16 + x) % NG] : r;
       return r;
     };
-    // the lane's piece of load i: its token within the tile is i P + tid / CH
+    // the lane's part of load i: its token within the tile is i P + tid / L
     uint32_t ko[NK], vo[NV];
 #pragma unroll
     for (int i = 0; i < NK; i++) {
-      const int k = i * KP + kk, x = (piece<KC>(k, tid % KC) - k * KC) * VE;
+      const int k = i * KP + tid / KL, x = (piece<KC>(k, tid % KL / PE) - k * KC) * VE + tid % PE * E;
       ko[i] = (uint32_t)(((NG == 1 ? k : k & 15) * c.dk + (x < c.dk ? x : 0)) * sizeof(T));
     }
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int k = i * VP + vk, x = (piece<VC>(k, tid % VC) - k * VC) * VE;
+      const int k = i * VP + vk, x = (piece<VC>(k, tid % VL / PE) - k * VC) * VE + tid % PE * E;
       vo[i] = (uint32_t)(((NG == 1 ? k : k & 15) * c.dv + (x < c.dv ? x : 0)) * sizeof(T));
     }
     // the next unit's pages and where its loads begin; then load i of it (of a tile before the first or past the last from some
     // page; clean() has zeros for it)
-    const void *kfrom[NG == 1 ? 1 : NK], *vfrom[NG == 1 ? 1 : NV];
+    const void *kfrom[KF], *vfrom[VF];
     auto prepare = [&](int u) {
 #pragma unroll
       for (int i = 0; i < NG; i++) {
@@ -267,24 +274,24 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
         pk[i] = u < kt1 ? page_of(u * TK + GT * i) : -1;
       }
 #pragma unroll
-      for (int i = 0; i < (NG == 1 ? 1 : NK); i++) {
-        const int pg = page(pk, i, KP, kg), in = (u * TK + (NG == 1 ? 0 : i * KP / 16 + kg) * GT) & inpage;
-        kfrom[i] = one(kh + (pg < 0 ? 0 : pg) * c.k_ps + in * c.dk);
+      for (int f = 0; f < KF; f++) {
+        const int i = f * (NK / KF), pg = page(pk, i, KP, kg), in = (u * TK + (NG == 1 ? 0 : i * KP / 16 + kg) * GT) & inpage;
+        kfrom[f] = one(kh + (pg < 0 ? 0 : pg) * c.k_ps + in * c.dk);
       }
 #pragma unroll
-      for (int i = 0; i < (NG == 1 ? 1 : NV); i++) {
-        const int pg = LAG ? page(pv, i, VP, vg) : page(pk, i, VP, vg);
+      for (int f = 0; f < VF; f++) {
+        const int i = f * (NV / VF), pg = LAG ? page(pv, i, VP, vg) : page(pk, i, VP, vg);
         const int in = ((u - LAG) * TK + (NG == 1 ? 0 : i * VP / 16 + vg) * GT) & inpage;
-        vfrom[i] = one(vh + (pg < 0 ? 0 : pg) * c.v_ps + in * c.dv);
+        vfrom[f] = one(vh + (pg < 0 ? 0 : pg) * c.v_ps + in * c.dv);
       }
     };
     auto fire = [&](int i, int kbuf, int vbuf) {
-      if (i < NK)
-        rq_dma16s(kfrom[NG == 1 ? 0 : i], ko[i < NK ? i : 0],
-                  (const lds_i8 *)(Lds)&s_kb[0][0] + kbuf * KB + (i * NT + wave * 64) * 16);
-      else
-        rq_dma16s(vfrom[NG == 1 ? 0 : i - NK], vo[i < NK ? 0 : i - NK],
-                  (const lds_i8 *)(Lds)&s_vb[0][0] + vbuf * VB + ((i - NK) * NT + wave * 64) * 16);
+      const int j = i < NK ? i : i - NK;
+      const void *from = i < NK ? kfrom[j / (NK / KF) % KF] : vfrom[j / (NV / VF) % VF];
+      const uint32_t off = i < NK ? ko[j % NK] : vo[j % NV];
+      const lds_i8 *to = (const lds_i8 *)(i < NK ? (Lds)&s_kb[0][0] + kbuf * KB : (Lds)&s_vb[0][0] + vbuf * VB) + (j * NT + wave * 64) * W;
+      if constexpr (V) rq_dma16s(from, off, to);
+      else rq_dma4s(from, off, to);
     };
     auto issue = [&](int u, int kbuf, int vbuf) {
       prepare(u);
@@ -293,19 +300,21 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
     };
     // A unit has landed, keys of pages pku and values of tile kt, of pages pvu: what of it has no page, or is no row's
     auto clean = [&](int kt, int kbuf, int vbuf, const int (&pku)[NG], const int (&pvu)[NG]) {
-      const PV zero = (PV)(T)0;
+      typedef kv_vec<T, E> Part;
+      const Part zero = (Part)(T)0;
+      Part *kz = (Part *)&s_kb[kbuf][0] + tid, *vz = (Part *)&s_vb[vbuf][0] + tid;
       bool whole = true, seen = kt * TK + TK - 1 <= j1;
 #pragma unroll
       for (int i = 0; i < NG; i++) whole = whole && pku[i] >= 0, seen = seen && pvu[i] >= 0;
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < NK; i++)
-          if (page(pku, i, KP, kg) < 0) s_kb[kbuf][i * NT + tid] = zero;
+          if (page(pku, i, KP, kg) < 0) kz[i * NT] = zero;
       }
       if (!seen) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
-          if (page(pvu, i, VP, vg) < 0 || kt * TK + i * VP + vk > j1) s_vb[vbuf][i * NT + tid] = zero;
+          if (page(pvu, i, VP, vg) < 0 || kt * TK + i * VP + vk > j1) vz[i * NT] = zero;
       }
     };
     if (kt0 < kt1) {
@@ -530,42 +539,43 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
   }
 }
 
-template <typename T, int DK, int DV, int NW, int NG, bool V>
+template <typename T, int DK, int DV, int NW, int NG, int W>
 __global__ __launch_bounds__(64 * NW, NW / 4) void k_kvt(KvDev c, KvaDev p, int B, int nrt, unsigned blk0, int2 *counts,
                                                          float *part, float2 *pml) {
   KvaItem it;
   if (kva_item(c, p, B, nrt, counts, 32 * NW, kva_tokens(sizeof(T) == 2, DK), blk0 + blockIdx.x, &it))
-    kvt_item<T, DK, DV, NW, NG, V>(c, p, it, nrt, counts, part, pml);
+    kvt_item<T, DK, DV, NW, NG, W>(c, p, it, nrt, counts, part, pml);
 }
 
-template <typename T, int DK, int DV, int NG, bool V>
+template <typename T, int DK, int DV, int NG, int W>
 int run(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
   constexpr int NW = kva_waves(sizeof(T) == 2, DK);
   const long long most = bnh_most_blocks(64 * NW);
   const int B = (int)(r.units / r.nrt / c.Hk);
   for (long long b0 = 0; b0 < r.items; b0 += most) {
     const long long n = r.items - b0 < most ? r.items - b0 : most;
-    hipLaunchKernelGGL((k_kvt<T, DK, DV, NW, NG, V>), dim3((unsigned)n), dim3(64 * NW), 0, s, c, p, B, r.nrt, (unsigned)b0,
+    hipLaunchKernelGGL((k_kvt<T, DK, DV, NW, NG, W>), dim3((unsigned)n), dim3(64 * NW), 0, s, c, p, B, r.nrt, (unsigned)b0,
                        kva_counts(r, work), kva_part(r, work), kva_ml(r, work));
     BNH_HIP(hipGetLastError());
   }
   return 0;
 }
-template <typename T, bool ONE, bool V>
+template <typename T, bool ONE, int W>
 int widths(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
   constexpr int NG = ONE ? 1 : kva_tokens(sizeof(T) == 2, 128) / 16;
-  if (r.DK == 256) return run<T, 256, 256, ONE ? 1 : 2, V>(c, p, r, work, s);
-  if (r.DK == 64) return r.D == 64 ? run<T, 64, 64, NG, V>(c, p, r, work, s) : run<T, 64, 128, NG, V>(c, p, r, work, s);
-  return r.D == 64 ? run<T, 128, 64, NG, V>(c, p, r, work, s) : run<T, 128, 128, NG, V>(c, p, r, work, s);
+  if (r.DK == 256) return run<T, 256, 256, ONE ? 1 : 2, W>(c, p, r, work, s);
+  if (r.DK == 64) return r.D == 64 ? run<T, 64, 64, NG, W>(c, p, r, work, s) : run<T, 64, 128, NG, W>(c, p, r, work, s);
+  return r.D == 64 ? run<T, 128, 64, NG, W>(c, p, r, work, s) : run<T, 128, 128, NG, W>(c, p, r, work, s);
 }
-template <typename T>
-int go(const KvDev &c, const KvaDev &p, const KvaPlan &r, bool v, void *work, hipStream_t s) {
-  if (!v) return widths<T, false, false>(c, p, r, work, s);
-  return 1 << c.sh >= kva_tokens(sizeof(T) == 2, r.DK) ? widths<T, true, true>(c, p, r, work, s) : widths<T, false, true>(c, p, r, work, s);
+template <typename T, int W>
+int pages(const KvDev &c, const KvaDev &p, const KvaPlan &r, void *work, hipStream_t s) {
+  return 1 << c.sh >= kva_tokens(sizeof(T) == 2, r.DK) ? widths<T, true, W>(c, p, r, work, s) : widths<T, false, W>(c, p, r, work, s);
 }
 
 }  // namespace
 
-int kva_tiles(const KvDev &c, const KvaDev &p, const KvaPlan &r, bool f16, bool v, void *work, hipStream_t s) {
-  return f16 ? go<h16>(c, p, r, v, work, s) : go<float>(c, p, r, v, work, s);
+int kva_tiles(const KvDev &c, const KvaDev &p, const KvaPlan &r, bool f16, int w, void *work, hipStream_t s) {
+  if (!f16) return w == 16 ? pages<float, 16>(c, p, r, work, s) : pages<float, 4>(c, p, r, work, s);
+  if (w == 2) return widths<h16, false, 2>(c, p, r, work, s);
+  return w == 16 ? pages<h16, 16>(c, p, r, work, s) : pages<h16, 4>(c, p, r, work, s);
 }
