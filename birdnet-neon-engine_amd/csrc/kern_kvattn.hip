@@ -408,7 +408,11 @@ KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
   const int d = c->dk > c->dv ? c->dk : c->dv, G = p->H / c->Hk;
   const long long m = p->nsel ? G : (long long)T * G;
   r.D = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
-  r.tiled = !p->nsel && m > 64;
+  // The tiled form's waves have 32 rows each, and 128 or 256 to a block; the other one's time goes up at 17 rows and at 65. fp16,
+  // 24 stations' caches of up to 5,000 tokens and 4 heads of 128: 16 rows 22.4 us tiled and 19.8, 24 rows 22.7 and 31.0; one of a
+  // day and 12 heads: 34.1 and 29.9, 34.2 and 58.1. Heads of 256: 24 rows 37.2 and 35.6, 48 rows 40.7 and 53.6. fp32, whose
+  // products take as long as rows that are nobody's: 48 rows 63.3 and 63.2, 165 and 152; 96 rows 66.9 and 80.4
+  r.tiled = !p->nsel && m > (!c->f16 ? 64 : d <= 128 ? 16 : 32);
   r.TK = 32;
   if (r.tiled) {
     r.DK = c->dk <= 64 && d <= 128 ? 64 : d <= 128 ? 128 : 256;
