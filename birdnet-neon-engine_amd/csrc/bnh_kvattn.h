@@ -81,7 +81,9 @@ __device__ __forceinline__ bool kva_item(const KvDev &c, const KvaDev &p, int B,
   }
   const int lane = threadIdx.x & 63;
   const unsigned ht = (unsigned)(p.G + MR - 1) / (unsigned)MR;
-  // a lane's sequence: its tiles of rows, and of tokens for the last of them
+  // a lane's sequence: its tiles of rows, and the most tiles of tokens that one of them looks at: the last does, but in a window,
+  // where it has fewer rows than others
+  const unsigned most = ((unsigned)p.window + (unsigned)(MR - 1) / (unsigned)p.G) / (unsigned)TK + 2;
   int first, past, n, tiles, nt;
   auto size = [&](int b) {
     const int i = b < B ? b : B - 1;
@@ -96,6 +98,11 @@ __device__ __forceinline__ bool kva_item(const KvDev &c, const KvaDev &p, int B,
     first = (int)s;
     tiles = p.sel ? (int)((unsigned)n * ht) : (int)(((unsigned)n * (unsigned)p.G + MR - 1) / (unsigned)MR);
     nt = n ? kva_span(c, p, tiles - 1, MR, TK, n, past).nt : 0;
+    if (n && p.window && !p.sel) {
+      const long long cap = (long long)c.ldt << c.sh;
+      const unsigned all = ((unsigned)(cap < past + n ? cap : past + n) + TK - 1) / (unsigned)TK;
+      nt = (int)(all < most ? all : most);
+    }
   };
   float work = 0.f;
   for (int b0 = 0; b0 < B; b0 += 64) {
@@ -108,7 +115,7 @@ __device__ __forceinline__ bool kva_item(const KvDev &c, const KvaDev &p, int B,
   unsigned before = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
     if (B > 64) size(b0 + lane);
-    const unsigned most = (unsigned)(nt + kMostParts - 1) / kMostParts, per = most > (unsigned)floor ? most : floor;
+    const unsigned few = (unsigned)(nt + kMostParts - 1) / kMostParts, per = few > (unsigned)floor ? few : floor;
     const unsigned parts = (unsigned)nt > per ? ((unsigned)nt + per - 1) / per : 1, mine = (unsigned)(c.Hk * tiles) * parts;
     unsigned sum = mine;
     for (int d = 1; d < 64 && d < B; d *= 2) {

@@ -40,6 +40,16 @@ def test_rows_about_the_forms(hip, f16, heads, hk, n, d):
     a.check("rows")
 
 
+@pytest.mark.parametrize("f16,d,heads,n", [(1, 64, 3, 605), (1, 128, 2, 257), (0, 64, 3, 300), (0, 256, 2, 25), (0, 128, 1, 33), (1, 256, 1, 17)])
+@pytest.mark.parametrize("window", [300, 664, 1500, 2 ** 31 - 1])
+def test_windows_in_parts(hip, f16, d, heads, n, window):
+    """A window whose tokens are cut into parts: the last tile of rows has few of them, and looks at fewer tokens than the others."""
+    say(f"window {window} rows {n} d {d} f16 {f16}")
+    a = Attn(hip, [2000, 40, 1777], [n, n - 1, n // 2], heads, 1, d, d, 64, f16, window=window, seed=n)
+    a.run()
+    a.check("window")
+
+
 @pytest.mark.parametrize("f16", [0, 1])
 @pytest.mark.parametrize("n", [1, 40])
 def test_many_sequences_in_parts(hip, f16, n):
