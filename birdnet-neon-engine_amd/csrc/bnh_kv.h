@@ -44,7 +44,9 @@ __device__ __forceinline__ int kv_page(const KvDev &c, int b, int i) {
 template <typename T, int N>
 using kv_vec = T __attribute__((ext_vector_type(N), aligned(sizeof(T) * N < 16 ? sizeof(T) * N : 16)));
 // Where they are not: N values from a place in the row, the last ones for a c near its end, so that every load is one; and what
-// kv_ld gives of them, once they are there (a row of fewer than N values is read value by value)
+// kv_ld gives of them, once they are there. A row of fewer than N values is read value by value: fp16, what is there; fp32, some
+// value for the others, or the tests for them cost the rows that are not so few (64 rows over up to 4,000 tokens, 12 heads of
+// 127: 225 us, 313 with tests; fp16, up to 17,279 tokens: 451 us, 359 with tests)
 template <typename T, int N>
 __device__ __forceinline__ kv_vec<T, N> kv_raw(const T *p, int c, int n) {
   kv_vec<T, N> r;
@@ -52,7 +54,10 @@ __device__ __forceinline__ kv_vec<T, N> kv_raw(const T *p, int c, int n) {
     __builtin_memcpy(&r, p + (c <= n - N ? c : c < n ? n - N : 0), N * sizeof(T));
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) r[i] = c + i < n ? p[c + i] : (T)0;
+    for (int i = 0; i < N; i++) {
+      if (sizeof(T) == 2) r[i] = c + i < n ? p[c + i] : (T)0;
+      else r[i] = p[c + i < n ? c + i : 0];
+    }
   }
   return r;
 }
@@ -61,6 +66,10 @@ __device__ __forceinline__ kv_vec<T, N> kv_fix(kv_vec<T, N> r, int c, int n) {
   constexpr int W = N * sizeof(T) / 4;
   static_assert(W >= 1 && W * 4 == (int)(N * sizeof(T)), "whole words");
   typedef uint32_t Words __attribute__((ext_vector_type(W)));
+  if (sizeof(T) == 4 && n < N) {
+#pragma unroll
+    for (int i = 0; i < N; i++) r[i] = c + i < n ? r[i] : (T)0;
+  }
   Words w = __builtin_bit_cast(Words, r);
   if (n >= N && n % N) {  // the same for all lanes
     const int s = c > n - N && c < n ? (c - (n - N)) * (int)sizeof(T) : 0;  // bytes too early

@@ -95,6 +95,9 @@ __device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const 
       pg[s] = kv_page(c, b, pi);
     }
   };
+  // piece x of a row of values: CPL columns from here, the last ones for one that the row's end cuts (those that are the piece's
+  // before as well are the same twice; pieces past the end are nobody's)
+  auto vcol = [&](int x) { return V || CPL * x + CPL <= c.dv || c.dv < CPL ? CPL * x : c.dv - CPL; };
   int jn[2], pn[2], bad0 = 0x7fffffff, bad1 = -1;  // tiles with values that are not finite: left out, and added at the end
   look(kt0 + wave, jn, pn);
   for (int kt = kt0 + wave; kt < kt1; kt += 4) {
@@ -114,13 +117,31 @@ __device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const 
     const T *vp = (q4 & 2 ? vb[1] : vb[0]) + 8 * (q4 & 1) * c.dv;
     FV kf[2][DKT];
     kv_vec<T, CPL> vr[8];
+    if constexpr (V) {
 #pragma unroll
-    for (int d = 0; d < DKT; d++) {
-      kf[0][d] = kv_ld<T, 8, V>(kp, 32 * d + 8 * q4, c.dk);
-      kf[1][d] = kv_ld<T, 8, V>(kp + 4 * c.dk, 32 * d + 8 * q4, c.dk);
+      for (int d = 0; d < DKT; d++) {
+        kf[0][d] = kv_ld<T, 8, V>(kp, 32 * d + 8 * q4, c.dk);
+        kf[1][d] = kv_ld<T, 8, V>(kp + 4 * c.dk, 32 * d + 8 * q4, c.dk);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) vr[e] = kv_ld<T, CPL, V>(vp + e * c.dv, CPL * lr, c.dv);
+    } else {
+      int kc = 8 * q4, vc = vcol(lr);  // what follows from them is found anew for each tile: there is no room to keep it
+      asm volatile("" : "+v"(kc), "+v"(vc));
+#pragma unroll
+      for (int d = 0; d < DKT; d++) {
+        kf[0][d] = kv_raw<T, 8>(kp, 32 * d + kc, c.dk);
+        kf[1][d] = kv_raw<T, 8>(kp + 4 * c.dk, 32 * d + kc, c.dk);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) vr[e] = kv_raw<T, CPL>(vp + e * c.dv, vc, c.dv);
+#pragma unroll
+      for (int d = 0; d < DKT; d++)
+        if (32 * d + 32 > c.dk) {
+          kf[0][d] = kv_fix<T, 8>(kf[0][d], 32 * d + kc, c.dk);
+          kf[1][d] = kv_fix<T, 8>(kf[1][d], 32 * d + kc, c.dk);
+        }
     }
-#pragma unroll
-    for (int e = 0; e < 8; e++) vr[e] = kv_ld<T, CPL, V>(vp + e * c.dv, CPL * lr, c.dv);
     v4f s[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; m++) s[m][0] = s[m][1] = (v4f){0.f, 0.f, 0.f, 0.f};
@@ -217,7 +238,7 @@ __device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const 
         for (int r = 0; r < 4; r++)
 #pragma unroll
           for (int i = 0; i < CPL; i++) {
-            const int col = CPL * (4 * q4 + r) + i;
+            const int col = vcol(4 * q4 + r) + i;
             const float z = col < c.dv ? (float)v[col] : 0.f;
             if (!kv_finite(z)) o[m][i][r] += y * z;
           }
@@ -238,7 +259,8 @@ __device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const 
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
-      for (int i = 0; i < CPL; i++) s_o[wave][lr * (D + 4) + CPL * (4 * q4 + r) + i] = o[m][i][r];
+      for (int i = 0; i < CPL; i++)
+        if (V || CPL * (4 * q4 + r) < c.dv) s_o[wave][lr * (D + 4) + vcol(4 * q4 + r) + i] = o[m][i][r];
     __syncthreads();
     const int x = tid >> 4, c0 = (tid & 15) * CPL, row = 16 * m + x;
     float top = s_m[0][row], f[4], sum = 0.f;
