@@ -129,15 +129,16 @@ __device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const 
       int kc = 8 * q4, vc = vcol(lr);  // what follows from them is found anew for each tile: there is no room to keep it
       asm volatile("" : "+v"(kc), "+v"(vc));
 #pragma unroll
-      for (int d = 0; d < DKT; d++) {
-        kf[0][d] = kv_raw<T, 8>(kp, 32 * d + kc, c.dk);
-        kf[1][d] = kv_raw<T, 8>(kp + 4 * c.dk, 32 * d + kc, c.dk);
-      }
+      for (int d = 0; d < DKT; d++)
+        if (F16 || 32 * d < c.dk) {  // fp32: 64 rows over up to 4,000 tokens, 12 heads of 63 and 62, 90 us, 107 with those past the row read as well
+          kf[0][d] = kv_raw<T, 8>(kp, 32 * d + kc, c.dk);
+          kf[1][d] = kv_raw<T, 8>(kp + 4 * c.dk, 32 * d + kc, c.dk);
+        }
 #pragma unroll
       for (int e = 0; e < 8; e++) vr[e] = kv_raw<T, CPL>(vp + e * c.dv, vc, c.dv);
 #pragma unroll
       for (int d = 0; d < DKT; d++)
-        if (32 * d + 32 > c.dk) {
+        if (32 * d + 32 > c.dk && (F16 || 32 * d < c.dk)) {
           kf[0][d] = kv_fix<T, 8>(kf[0][d], 32 * d + kc, c.dk);
           kf[1][d] = kv_fix<T, 8>(kf[1][d], 32 * d + kc, c.dk);
         }
@@ -148,7 +149,7 @@ __device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const 
 #pragma unroll
     for (int d = 0; d < DKT; d++)
 #pragma unroll
-      for (int m = 0; m < MT; m++) s[m][0] = mma(kf[0][d], qf[m][d], s[m][0]), s[m][1] = mma(kf[1][d], qf[m][d], s[m][1]);
+      for (int m = 0; m < MT && (V || F16 || 32 * d < c.dk); m++) s[m][0] = mma(kf[0][d], qf[m][d], s[m][0]), s[m][1] = mma(kf[1][d], qf[m][d], s[m][1]);
     const int jl = (q4 & 2 ? j[1] : j[0]) + 8 * (q4 & 1);  // the lane's 8 tokens
     const bool there = (q4 & 2 ? pg[1] : pg[0]) >= 0;
     kv_vec<T, 2> mk = {(T)0, (T)0};
