@@ -9,7 +9,9 @@ namespace {
 // ---------------------------------------------------------------------------------------------- append
 // Bound by HBM: q, k and v are read once and written once. A block owns the new rows of one page for one head of keys, with the
 // query heads that read it, so that the page's bounds need no atomics: its threads are `nu` units of a head (VEC values,
-// with their partners VEC more) side by side, times as many rows as fit 256.
+// with their partners VEC more) side by side, times as many rows as fit 256. 24 archives of 720 rows, 12 heads of 128, 162 MB: 36 us,
+// 4.5 TB/s, of which the angles are 6; 8 of up to 500 rows of odd widths in fp32, value by value: 21 us, 2.5 TB/s; live rows 6 to 7,
+// a launch and two loads that wait for each other.
 struct AppDev {
   const void *k, *v, *q;
   void *qr;
@@ -230,7 +232,8 @@ __device__ __forceinline__ bool sel_row(const KvDev &c, int window, int b0, int 
 
 // The scores of PPB pages for one row and head of keys: 16 lanes a page, 8 values each a step. Bound by reading the bounds
 // (4 dk bytes a page and head in fp16); the products are exact in 64 bits and their sums good to 2^-50, so that no order of
-// sums can make another choice.
+// sums can make another choice. One row over 1,890 pages of 4 heads of 128: 8.2 us; 16 rows over up to 810: 13.4; 144 rows of 2
+// heads of 72 over up to 188, fp32: 10.7.
 constexpr int PPB = 64;
 template <typename T, bool V>
 __global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, int b0, int t0, u64 *key) {

@@ -17,8 +17,9 @@ __device__ __forceinline__ v4f mma(kv_vec<float, 8> a, kv_vec<float, 8> b, v4f c
   for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
   return c;
 }
-// The streaming form, for few rows, for fp32 and for widths that the tiled form does not take: bound by reading keys and values
-// where rows are few. Four waves of a block take tiles of 32 tokens in turn, straight from memory into the matrix
+// The streaming form, for few rows and for rows with a selection: bound by reading keys and values (64 rows over up to a day,
+// 1.15 GB: 223 us, 5.2 TB/s; a copy 5.1), and by the latency of its steps where there is little to read (12 heads of one row over a
+// day, 106 MB: 22 us and 7 for the join; 32 pages of a week 10 and 4). Four waves of a block take tiles of 32 tokens in turn, straight from memory into the matrix
 // instructions' registers: the scores' product has keys as its rows in such an order that a lane ends with the scores of 8 tokens
 // in a row, 8 q4 .. 8 q4 + 7 (q4 = lane / 16), for query lane & 15, which is what the second product's operand holds; values are
 // loaded as 8 tokens by CPL columns a lane and change places within the lane. Each wave has its own maximum and sums, joined at
