@@ -141,10 +141,10 @@ __global__ __launch_bounds__(256) void k_kv_append(KvDev c, AppDev p, int npt, i
       vc[(long long)t * c.dv + e] = ((const T *)p.v)[((long long)first + t0 + t) * p.ldv + g * c.dv + e];
     }
   } else {
-    const int nv = (c.dv + VE - 1) / VE, step = 256 / nv, e0 = tid % nv * VE, e = VEC > 1 || e0 + VE <= c.dv ? e0 : c.dv - VE;
+    const int nv = (c.dv + VE - 1) / VE, step = 256 / nv, e0 = tid % nv * VE, e = VEC == VE || e0 + VE <= c.dv ? e0 : c.dv - VE;
     for (int t = tid / nv; t < t1 - t0 && tid < step * nv; t += step) {
       const T *x = (const T *)p.v + ((long long)first + t0 + t) * p.ldv + g * c.dv + e;
-      if constexpr (VEC > 1) {
+      if constexpr (VEC == VE) {
         *(W *)(vc + (long long)t * c.dv + e) = *(const W *)x;
       } else {
         uint4 y;
@@ -493,13 +493,21 @@ int bnh_kv_append(const bnh_kvcache *c, const bnh_rotary *r, const void *k, int 
   const KvDev d = kv_dev(c, T, rows, start, len);
   const int rd = r ? r->rd : 0, pairs = r ? r->pairs : 0, ve = 16 / (int)es;
   const AppDev p = {k, v, q, qr, r ? r->freq : nullptr, r ? r->pos : nullptr, ldk, ldv, ldq, ldr, q ? H / c->Hk : 0, rd, pairs};
-  bool vec = c->dk % (2 * ve) == 0 && c->dv % ve == 0 && rd % (2 * ve) == 0 && c->k_ps % ve == 0 && c->v_ps % ve == 0;
-  vec = vec && kv_on(c->lo, 4) && kv_on(c->hi, 4);
-  for (const void *x : {(const void *)c->k, (const void *)c->v, k, v, q, (const void *)qr}) vec = vec && kv_on(x, 16);
-  vec = vec && ldk % ve == 0 && ldv % ve == 0 && (!q || (ldq % ve == 0 && ldr % ve == 0));
+  // values of q and k at a time: as many as widths, strides and addresses allow (24 archives of 720 rows, 12 heads, fp16, us: 128
+  // by eights 35; 120 by fours 39, one by one 56; 108 by twos 39 and 57; fp32, 108 by twos 73 and 119)
+  auto fits = [&](int n) {
+    bool x = c->dk % (2 * n) == 0 && rd % (2 * n) == 0 && c->k_ps % n == 0 && ldk % n == 0;
+    x = x && (!q || (ldq % n == 0 && ldr % n == 0)) && kv_on(c->lo, 4) && kv_on(c->hi, 4);
+    for (const void *y : {(const void *)c->k, k, q, (const void *)qr}) x = x && kv_on(y, n * es);
+    return x;
+  };
+  const bool vec = fits(ve) && c->dv % ve == 0 && c->v_ps % ve == 0 && ldv % ve == 0 && kv_on(c->v, 16) && kv_on(v, 16);
   hipStream_t s = bnh_stream(stream);
-  if (c->f16) return vec ? append_run<h16, 8>(d, p, B, s) : append_run<h16, 1>(d, p, B, s);
-  return vec ? append_run<float, 4>(d, p, B, s) : append_run<float, 1>(d, p, B, s);
+  if (c->f16) {
+    if (vec) return append_run<h16, 8>(d, p, B, s);
+    return fits(4) ? append_run<h16, 4>(d, p, B, s) : fits(2) ? append_run<h16, 2>(d, p, B, s) : append_run<h16, 1>(d, p, B, s);
+  }
+  return vec ? append_run<float, 4>(d, p, B, s) : fits(2) ? append_run<float, 2>(d, p, B, s) : append_run<float, 1>(d, p, B, s);
 }
 
 size_t bnh_kv_select_work_bytes(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int rows) {

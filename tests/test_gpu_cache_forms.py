@@ -172,6 +172,18 @@ def test_two_streams(hip, n):
 
 
 @pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("dk,dv,rd,pairs", [(108, 211, 108, 0), (40, 33, 24, 1), (44, 70, 20, 0), (24, 25, 8, 1), (24, 24, 8, 0), (200, 3, 40, 0),
+                                            (12, 9, 0, 0), (64, 63, 64, 0), (64, 63, 32, 1), (4, 16, 4, 0)])
+@pytest.mark.parametrize("pad,at,extra", [(0, 0, 0), (4, 4, 4), (2, 2, 2), (8, 1, 8), (1, 0, 8)])
+def test_append_some_at_a_time(hip, f16, dk, dv, rd, pairs, pad, at, extra):
+    """Widths, strides and places that allow 8, 4, 2 values of a row at a time, or one."""
+    say(f"append {dk} {dv} rd {rd} pairs {pairs} pad {pad} at {at} f16 {f16}")
+    a = Append(hip, [0, 40, 31, 7], [70, 1, 33, 0], 6, 2, dk, dv, rd, pairs, 32, f16, seed=dk + rd, pad=pad, at=at, extra=extra)
+    a.run()
+    a.check("some")
+
+
+@pytest.mark.parametrize("f16", [0, 1])
 def test_append_again(hip, f16):
     """The same rows once more at the same place change nothing, bounds neither: a call that failed half-way is made again."""
     say(f"append again f16 {f16}")
