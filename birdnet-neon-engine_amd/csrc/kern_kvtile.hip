@@ -61,8 +61,9 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
   constexpr int KP = NT / KC, VP = NT / VC;                    // tokens that one load of all threads covers
   constexpr int NK = TK / KP, NV = TK / VP, GT = TK / NG;
   constexpr int NB = DK == 256 && !F16 ? 2 : 3;                // tiles in LDS
-  // Weights are in units of 2^-12, so that fp16 holds those down to 2^-26 of the largest with all bits; the running maximum may be
-  // short by GROW in the exponent before the sums are scaled anew (2^15 at most: nothing overflows)
+  // Weights are in units of 2^-12, so that the second part of those down to 2^-15 of the largest is no subnormal, and nothing above
+  // 2^-37 of it is lost; the running maximum may be short by GROW in the exponent before the sums are scaled anew (2^15 at most:
+  // nothing overflows)
   constexpr float OFF = F16 ? 12.f : 0.f, GROW = 3.f;
   typedef kv_vec<T, 8> FV;
   typedef kv_vec<T, VE> PV;
@@ -117,7 +118,9 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
 
   // The work on a tile
   v16f s[ST];
-  FV ph[2 * ST];
+  // fp16: weights in two parts, 22 bits, and a product for each. In one part's 11 bits outputs whose terms cancel are off by several
+  // times their own rounding (17,280 rows of 12 heads of 128: 966 us so, 1,300 with both; 24 chunks of up to 120 rows 48 and 53)
+  FV ph[2 * ST], pl[F16 ? 2 * ST : 1];
   // A tile is NG groups of GT tokens that have a page each: one for pages of TK tokens or more, else groups of 16
   int pc[NG];
   auto seen = [&](int kt) {  // whether the wave has rows that see a token of the tile
@@ -192,7 +195,9 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
       for (int r = 0; r < 16; r++) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], p.sc, -to));
         sum[r & 3] += x;
-        ph[2 * i + r / 8][r % 8] = (T)x;
+        const T y = (T)x;
+        ph[2 * i + r / 8][r % 8] = y;
+        if (F16) pl[2 * i + r / 8][r % 8] = (T)(x - (float)y);
       }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   };
@@ -218,6 +223,7 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
           for (int e = 0; e < 8; e++)
             a[e] = *(L)((Lds)&s_vb[0][0] + (x ^ 16 * (8 * v ^ ((e & 3) << 2 | e >> 2))) + (16 * k + e) * VC * 16);
         }
+        if (F16) o[v] = mma(a, pl[k], o[v]);
         o[v] = mma(a, ph[k], o[v]);
         if (v == DV / 32 - 1) between(k);
       }
@@ -336,7 +342,7 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
 #pragma unroll
         for (int i = 0; i < 2 * ST; i++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) ph[i][e] = (T)0;
+          for (int e = 0; e < 8; e++) ph[i][e] = pl[i][e] = (T)0;
         // tile kt0 - 1's values, which have no page and are zeros, lie in the last place
         issue(kt0, 0, 2);
         issue(kt0 + 1, 1, 0);
@@ -361,7 +367,7 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
             __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
             for (int i = 0; i < 2 * ST * (DV / 32); i++) {
-              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
               __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
             }
 #pragma unroll
@@ -386,7 +392,7 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
 #pragma unroll
             for (int i = 0; i < 2 * ST; i++)
 #pragma unroll
-              for (int e = 0; e < 8; e++) ph[i][e] = (T)0;
+              for (int e = 0; e < 8; e++) ph[i][e] = pl[i][e] = (T)0;
           }
           was = on;
           __syncthreads();

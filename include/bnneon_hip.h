@@ -565,8 +565,7 @@ int bnh_kv_append(const bnh_kvcache *c, const bnh_rotary *r, const void *k, int 
  * and 0 where there are none (or all s_j are -inf). sel int32 [rows][Hk][nsel] (NULL: all pages): of those tokens the ones in
  * the pages i that the row's selection for the head lists in ascending order; an entry that is not above the one before it,
  * or outside [0, ldt), is passed over. What the cache holds in other places reaches no output, infinities and NaNs neither.
- * Scores, sums and outputs are fp32, rounded once at the end; fp16: the e^{s_j} are factors of 22 bits where reading the cache
- * is what counts (a selection; T H/Hk up to 16, or 32 at widths past 128), and of 11 bits where there are more rows.
+ * Scores, sums and outputs are fp32, rounded once at the end; fp16: the e^{s_j} are factors of 22 bits, however many rows there are.
  * work: device scratch of at least bnh_kv_attn_work_bytes bytes, 16-byte aligned (0 bytes for some shapes: NULL is allowed
  * then); its size depends on c's and p's sizes, T, B and rows. */
 typedef struct {

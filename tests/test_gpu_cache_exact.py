@@ -1,0 +1,37 @@
+"""Cached attention where its precision shows: weights as factors of 22 bits in every form."""
+import numpy as np
+import pytest
+
+from test_gpu_cache import TWO, Attn
+from test_gpu_context import say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dk,dv", [(16, 16), (64, 64), (64, 128), (128, 64), (128, 128), (256, 256), (200, 72), (127, 127), (126, 98)])
+@pytest.mark.parametrize("heads,hk,n", [(1, 1, 16), (1, 1, 17), (2, 1, 20), (3, 3, 40)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_weights_of_many_rows(hip, dk, dv, heads, hk, n, page):
+    """A row's weights are as exact beside many rows as alone. Few tokens and small scores, so that 32-bit sums leave less than
+    11 bits would."""
+    say(f"weights {dk} {dv} heads {heads} {hk} rows {n} page {page}")
+    a = Attn(hip, [0, 9, 30], [n, n, n - 1], heads, hk, dk, dv, page, 1, seed=dk + n, qstd=2.0 / dk ** 0.5)
+    a.run()
+    a.check("weights", TWO)
+
+
+@pytest.mark.parametrize("n", [1, 16, 40])
+@pytest.mark.parametrize("d", [64, 256])
+def test_mean_of_the_largest(hip, d, n):
+    """A mean of equal values is that value, also of fp16's largest: 22 bits of a weight are 2^-22 off, half a step is 2^-12."""
+    say(f"largest rows {n} d {d}")
+
+    def edit(c):
+        for i in range(c.B):
+            c.V[i][:] = 65504
+
+    a = Attn(hip, [0, 300], [n, n], 2, 1, d, d, 32, 1, seed=n, edit=edit)
+    a.run()
+    got = a.do.get()[0].reshape(a.c.rows, -1)
+    for s in a.c.start:
+        assert (got[s:s + n].astype(np.float32) == 65504).all()
