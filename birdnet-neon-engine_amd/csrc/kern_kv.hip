@@ -202,8 +202,10 @@ int append_run(const KvDev &c, const AppDev &p, int B, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------------- select
-// A score's order as a whole number: larger for larger scores, 0 for a page that is not to be had
+// A score's order as a whole number: larger for larger scores, 0 for a page that is not to be had, above that of +infinity for one
+// that is always taken
 typedef unsigned long long u64;
+constexpr u64 ALWAYS = ~0ull;
 __device__ __forceinline__ u64 order_of(double x) {
   if (x != x) x = -INFINITY;
   const u64 b = (u64)__double_as_longlong(x == 0 ? 0.0 : x);  // -0 is 0
@@ -287,17 +289,16 @@ __global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, in
 #pragma unroll
     for (int m = 1; m < 16; m *= 2) x += __shfl_xor(x, m);
     const bool there = pi >= lo && kv_page(c, b, pi) >= 0;
-    if (l == 0) out[pi] = !there ? 0 : order_of(pi < p.first || pi > cur - p.last ? (double)INFINITY : x);
+    if (l == 0) out[pi] = !there ? 0 : pi < p.first || pi > cur - p.last ? ALWAYS : order_of(x);
   }
 }
 
 // The nsel largest of a row's keys, the lower pages first where the last of them are equal, in ascending order. The bits that all
 // keys agree on are passed over, then digits of 8 bits are counted until the last one needed is known; pages that are always
-// taken (the largest key of all) stand aside, or they would stretch the range to all 64 bits. 512 threads hold 8 keys each, in
+// taken (no more than nsel) stand aside, or they would stretch the range to all 64 bits. 512 threads hold 8 keys each, in
 // order; more than 4,096 are read again for each digit. Bound by the steps, of which each waits for the one before: 1,890
 // pages of a row 7.3 us, 14.8 with digits from the top (the first are the same for all) and keys read again for each.
 constexpr int KEYS = 8, NTP = 512;
-constexpr u64 ALWAYS = 0xfff0000000000000ull;  // order_of(+infinity)
 __global__ __launch_bounds__(NTP) void k_kv_pick(KvDev c, SelDev p, int b0, int t0, const u64 *key) {
   __shared__ int s_n[256], s_w[NTP / 64], s_t[NTP / 64], s_b[2];
   __shared__ unsigned s_lo[NTP / 64], s_hi[NTP / 64];
@@ -390,13 +391,12 @@ __global__ __launch_bounds__(NTP) void k_kv_pick(KvDev c, SelDev p, int b0, int 
     always += s_w[w], any += s_t[w];
   }
   any -= always;
-  // taken: above `cut` in the bits of `mask`, and the first `need` that agree with it there
-  u64 cut = 0, mask = 0;
+  // taken: those that always are, those above `cut` in the bits of `mask`, and the first `need` that agree with it there
+  u64 cut = 0, mask = ~0ull;
   int need = p.nsel - always;
-  if (need <= 0 || any <= need) {
-    // of those that are always taken the first, or all there are
-    cut = need <= 0 ? ALWAYS : 0, mask = ~0ull, need = need <= 0 ? p.nsel : 0;
-  } else {
+  if (need <= 0) {
+    cut = ALWAYS - 1;  // none of the others
+  } else if (any > need) {
     int bits = least == most ? 32 : 64 - __builtin_clz(least ^ most);  // that are not the same for all
     mask = bits < 64 ? ~0ull << bits : 0;
     cut = (u64)most << 32 & mask;
@@ -439,19 +439,21 @@ __global__ __launch_bounds__(NTP) void k_kv_pick(KvDev c, SelDev p, int b0, int 
       __syncthreads();
     }
   }
+  auto above = [&](u64 x) { return x == ALWAYS || (x & mask) > cut; };
+  auto agrees = [&](u64 x) { return x && x != ALWAYS && (x & mask) == cut; };
   int done = 0, ties = 0;
   for (int x0 = lo; x0 < end; x0 += KEYS * NTP) {
     if (!once) fetch(x0);
     int n = 0, total;  // those above, and 2^16 times those that agree
 #pragma unroll
     for (int e = 0; e < KEYS; e++)
-      n += y[e] ? ((y[e] & mask) > cut) + (((y[e] & mask) == cut) << 16) : 0;
+      n += above(y[e]) + (agrees(y[e]) << 16);
     const int in = before(n, &total, s_n);
     int rank = ties + (in >> 16), at = done + (in & 0xffff) + ((rank < need ? rank : need) - (ties < need ? ties : need));
 #pragma unroll
     for (int e = 0; e < KEYS; e++) {
-      const bool tie = y[e] && (y[e] & mask) == cut;
-      if (y[e] && ((y[e] & mask) > cut || (tie && rank < need))) out[at++] = x0 + tid * each + e;
+      const bool tie = agrees(y[e]);
+      if (above(y[e]) || (tie && rank < need)) out[at++] = x0 + tid * each + e;
       rank += tie;
     }
     const int now = ties + (total >> 16);

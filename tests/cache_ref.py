@@ -69,10 +69,10 @@ def select(q, lo, hi, there, at, page, window, first, last, n):
     s = scores(q, lo, hi)
     i = np.arange(len(there))
     s = np.where(np.isnan(s), -np.inf, s)
-    s[:, (i < first) | (i > at // page - last)] = np.inf
+    forced = (i < first) | (i > at // page - last)  # above any score, +infinity too
     can = there & (i * page <= at) & (((i + 1) * page > at - window + 1) if window else True)
     out = np.full((len(s), n), -1, np.int32)
     for g in range(len(s)):
-        mine = sorted(i[can], key=lambda x: (-s[g, x], x))[:n]
+        mine = sorted(i[can], key=lambda x: (not forced[x], -s[g, x], x))[:n]
         out[g, :len(mine)] = sorted(mine)
     return out

@@ -1,0 +1,59 @@
+"""The selection of pages where scores are not finite, and where its launches are cut."""
+import numpy as np
+import pytest
+
+import cache_ref as R
+from test_gpu_cache import TWO, Attn, Rows, check_pick, pick
+from test_gpu_context import near, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+@pytest.mark.parametrize("tokens", [300, 700, 3000, 70000])
+def test_forced_before_infinite(hip, f16, tokens):
+    """The first pages and the row's own are taken always, also where more pages than there is room for have bounds of +infinity:
+    few pages, a pass of them, and more than one pass."""
+    say(f"forced tokens {tokens} f16 {f16}")
+
+    def edit(c):  # an infinite key in every third page
+        c.K[0][5::48, :, 4] = np.inf
+
+    a = Attn(hip, [tokens - 4], [4], 4, 2, 24, 8, 16, f16, edit=edit, seed=tokens)
+    a.q[..., 4] = np.abs(a.q[..., 4]) + 1
+    a.dq = Rows(hip, 1, a.c.rows, 96, a.c.t, 96, 0, 0, a.q.reshape(a.c.rows, -1))
+    own = (tokens - 4 + np.arange(4)) // 16
+    some = (tokens + 15) // 16 // 3
+    for first, last, n in ((1, 2, 3), (1, 2, 4), (0, 1, 1), (0, 1, 2), (2, 1, 9), (0, 0, 5), (1, 1, some - 1), (1, 1, some + 7)):
+        got = pick(a, first, last, n)
+        for r in range(4):
+            for g in range(2):
+                s = got[r, g][got[r, g] >= 0]
+                assert (np.diff(s) > 0).all()
+                assert set(range(first)) | {own[r] - x for x in range(last)} <= set(s.tolist()), (first, last, n, r, g)
+        check_pick(a, got, first, last, n, f"forced {first} {last} {n}")
+
+
+@pytest.mark.parametrize("f16", [0, 1])
+def test_an_infinite_key_that_the_row_does_not_see(hip, f16):
+    """A window that begins within a page: an infinite key ahead of it makes the page's bound infinite, and does not cost the row its
+    own page."""
+    say(f"infinite key ahead of the window f16 {f16}")
+
+    def edit(c):
+        c.K[0][640:644, :, 4] = np.inf
+
+    a = Attn(hip, [999], [1], 2, 2, 32, 32, 16, f16, window=350, edit=edit, seed=3)  # tokens from 650 on: page 40's last six
+    a.q[..., 4] = np.abs(a.q[..., 4]) + 1
+    a.dq = Rows(hip, 1, a.c.rows, 64, a.c.t, 64, 0, 0, a.q.reshape(a.c.rows, -1))
+    sel = pick(a, 0, 1, 1)
+    assert (sel[0] == 62).all()
+    sel = pick(a, 0, 1, 2)
+    assert (sel[0] == [40, 62]).all()
+    b = Attn(hip, [999], [1], 2, 2, 32, 32, 16, f16, window=350, edit=edit, seed=3, sel=lambda c: sel)
+    b.q[:], b.dq = a.q, a.dq
+    b.run()
+    got = b.do.get()[0][:1].reshape(1, 2, 32)
+    o, err = R.attention(b.q[:1], np.nan_to_num(b.c.K[0], posinf=0), b.c.V[0], b.seen(0, 1), b.scale, TWO if f16 else 0)
+    assert np.isfinite(got).all()
+    near(got, o, err, "selected", f16)
