@@ -529,9 +529,10 @@ int bnh_kv_select(const bnh_kvcache *c, const bnh_kvattn *p, int first, int last
   const SelDev e = {p->q, p->sel, p->ldq, p->H, p->H / c->Hk, p->window, p->nsel, first, last};
   const bool v = c->dk % 8 == 0 && kv_on(c->lo, 16) && kv_on(c->hi, 16);
   const int npb = (int)bnh_ceil_div(c->ldt, PPB);
-  // rows of a launch also by its blocks
+  // rows of a launch also by its blocks, of the scores and of the choice
   long long most = bnh_most_blocks(256) / ((long long)npb * c->Hk);
   BNH_REQ(most > 0);
+  if (most > bnh_most_blocks(NTP) / c->Hk) most = bnh_most_blocks(NTP) / c->Hk;
   if (most > per) most = per;
   hipStream_t s = bnh_stream(stream);
   for (long long r0 = 0; r0 < all; r0 += most) {

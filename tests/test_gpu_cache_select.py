@@ -57,3 +57,22 @@ def test_an_infinite_key_that_the_row_does_not_see(hip, f16):
     o, err = R.attention(b.q[:1], np.nan_to_num(b.c.K[0], posinf=0), b.c.V[0], b.seen(0, 1), b.scale, TWO if f16 else 0)
     assert np.isfinite(got).all()
     near(got, o, err, "selected", f16)
+
+
+def test_more_rows_than_a_launch_has_threads_for(hip):
+    """Rows and heads whose choices, a block of 512 threads each, would be 2^32 threads and more in one launch."""
+    say("rows past a launch")
+    L, hk, rows = hip.lib(), 4, (1 << 21) + 3
+    z = hip.DeviceArray.zeros
+    q, sel, kv = z((rows, hk), np.float16), hip.DeviceArray((rows, hk, 2), np.int32), z((hk * 16,), np.float16)
+    sel.fill(0x7f)
+    table, past = z((1,), np.int32), z((1,), np.int32)
+    c = hip.KvCache(k=kv.ptr, v=kv.ptr, k_ps=hk * 16, v_ps=hk * 16, f16=1, pages=1, page=16, Hk=hk, dk=1, dv=1, lo=kv.ptr, hi=kv.ptr,
+                    table=table.ptr, ldt=1, past=past.ptr)
+    a = hip.KvAttn(q=q.ptr, ldq=hk, H=hk, scale=1, sel=sel.ptr, nsel=2)
+    wb = L.bnh_kv_select_work_bytes(c, a, rows, 1, rows)
+    ws = hip.DeviceArray((wb,), np.uint8)
+    hip.check(L.bnh_kv_select(c, a, 0, 1, rows, 1, rows, None, None, ws.ptr, wb, None))
+    hip.sync()
+    got = sel.numpy()
+    assert (got[..., 0] == 0).all() and (got[..., 1] == -1).all()
