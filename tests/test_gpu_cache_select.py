@@ -76,3 +76,28 @@ def test_more_rows_than_a_launch_has_threads_for(hip):
     hip.sync()
     got = sel.numpy()
     assert (got[..., 0] == 0).all() and (got[..., 1] == -1).all()
+
+
+def test_launches_that_begin_within_a_sequence(hip):
+    """A table wide enough for a few rows' scores to fill the workspace: launches begin in the middle of sequences, and use it
+    again."""
+    say("launches within a sequence")
+    a = Attn(hip, [200, 0, 33, 5], [23, 20, 0, 17], 12, 12, 8, 8, 16, 1, seed=1, more=70000)
+    c, L = a.c, hip.lib()
+    p = a.args()
+    p.nsel = 6
+    wb = L.bnh_kv_select_work_bytes(c.args(), p, *c.seqs()[:3])
+    per = wb // (8 * c.hk * c.ldt)
+    assert 1 < per < 20 and c.T % per
+    got = pick(a, 1, 2, 6)  # the workspace's end and rows of nobody are looked at by what follows and by pick
+    lo, hi = c.dlo.numpy(), c.dhi.numpy()
+    none = np.ones(c.rows, bool)
+    for i in range(c.B):
+        m = -(-c.total[i] // 16)
+        x = c.table[i, :m]
+        for r in range(c.lens[i]):
+            row = int(c.start[i]) + r
+            want = R.select(a.q[row], lo[x], hi[x], np.ones(m, bool), c.pasts[i] + r, 16, 0, 1, 2, 6)
+            assert np.array_equal(got[row], want), (i, r)
+            none[row] = False
+    assert (got[none] == -7).all()
