@@ -86,6 +86,8 @@ class ContextNet:
         self.past = np.zeros(self.stations, np.int32)
 
     def reset(self):
+        """As a new net: all states zero, all pages free. Waits for the device first, as forget() does."""
+        hip.device_sync()
         for s in self.state:
             if s is not None:
                 s.fill(0)
@@ -165,9 +167,12 @@ class ContextNet:
             self.past[s] = n
 
     def forget(self, station):
-        """The station's next window is its first: its states are zero, and its pages free."""
+        """The station's next window is its first: its states are zero, and its pages free. Waits for all that runs on the device:
+        a run on any stream may still store the station's states or read its pages, and what comes next on any stream finds
+        the states cleared."""
         if not 0 <= station < self.stations:
             raise ValueError(f"station {station} of {self.stations}")
+        hip.device_sync()
         for s in self.state:
             if s is not None:
                 n = s.nbytes // self.stations

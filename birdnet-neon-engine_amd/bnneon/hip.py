@@ -102,6 +102,7 @@ _SIGS = {
     "bnh_stream_new": (vp, []),
     "bnh_stream_free": (i32, [vp]),
     "bnh_stream_sync": (i32, [vp]),
+    "bnh_device_sync": (i32, []),
     "bnh_event_new": (vp, []),
     "bnh_event_free": (i32, [vp]),
     "bnh_event_record": (i32, [vp, vp]),
@@ -311,6 +312,11 @@ class DeviceArray:
 
 def sync(stream=None):
     check(lib().bnh_stream_sync(stream), "bnh_stream_sync")
+
+
+def device_sync():
+    """Waits for the work of all streams."""
+    check(lib().bnh_device_sync(), "bnh_device_sync")
 
 
 class S8Weights:

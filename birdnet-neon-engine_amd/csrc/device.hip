@@ -62,7 +62,8 @@ int bnh_memcpy_d2h(void *dst, const void *src, size_t bytes) {
   return 0;
 }
 int bnh_memset(void *dst, int value, size_t bytes) {
-  BNH_HIP(hipMemset(dst, value, bytes));
+  BNH_HIP(hipMemset(dst, value, bytes));  // device memory: may return before it is done, and streams of bnh_stream_new do not wait
+  BNH_HIP(hipStreamSynchronize(nullptr));
   return 0;
 }
 void *bnh_stream_new(void) {
@@ -77,6 +78,10 @@ int bnh_stream_free(void *s) {
 }
 int bnh_stream_sync(void *s) {
   BNH_HIP(hipStreamSynchronize(bnh_stream(s)));
+  return 0;
+}
+int bnh_device_sync(void) {
+  BNH_HIP(hipDeviceSynchronize());
   return 0;
 }
 void *bnh_event_new(void) {

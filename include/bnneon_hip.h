@@ -38,6 +38,7 @@ int bnh_memset(void *dst, int value, size_t bytes);               /* synchronous
 void *bnh_stream_new(void);
 int bnh_stream_free(void *stream);
 int bnh_stream_sync(void *stream);
+int bnh_device_sync(void);                                        /* waits for all streams, of any kind */
 void *bnh_event_new(void);
 int bnh_event_free(void *ev);
 int bnh_event_record(void *ev, void *stream);

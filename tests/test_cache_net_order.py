@@ -1,0 +1,52 @@
+"""What the temporal context net asks of the device, and in which order: against a library that only notes its calls."""
+import itertools
+
+import pytest
+
+from bnneon import contextnet, hip
+
+
+class Notes:
+    """Entry points that do nothing and succeed; `calls` has their names and arguments."""
+
+    def __init__(self):
+        self.calls, self.at, self.fail = [], itertools.count(1 << 20, 1 << 20), None
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            if name == "bnh_malloc":
+                return next(self.at)
+            if name == "bnh_last_error":
+                return b"refused"
+            return 1 if name == self.fail else 0
+        return call
+
+    def names(self):
+        return [n for n, _ in self.calls]
+
+
+@pytest.fixture
+def notes(monkeypatch):
+    n = Notes()
+    monkeypatch.setattr(hip, "lib", lambda: n)
+    return n
+
+
+def net(**kw):
+    return contextnet.ContextNet(**{**dict(dim=64, heads=2, layers=2, stations=3, rank=2, cached=[1], windows=100, page=16), **kw})
+
+
+@pytest.mark.parametrize("cached", [[], [0], [0, 1]])
+@pytest.mark.parametrize("what", ["forget", "reset"])
+def test_clearing_waits(notes, cached, what):
+    """Runs on any stream are over before a station's states are cleared (which returns once it is done) and its pages are free."""
+    x = net(cached=cached)
+    p = x.plan([20, 1], [0, 2])
+    x.run(p, stream=77)
+    notes.calls.clear()
+    x.forget(0) if what == "forget" else x.reset()
+    names = notes.names()
+    clears = [i for i, n in enumerate(names) if n == "bnh_memset"]
+    assert names[0] == "bnh_device_sync"
+    assert len(clears) == 2 - len(cached)
