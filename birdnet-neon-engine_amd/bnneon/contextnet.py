@@ -202,10 +202,20 @@ class ContextNet:
     def run(self, p, stream=None, advance=True):
         """The blocks over p["x"], which holds the embeddings (rows of one sequence in time order): x in place, and its last
         norm in p["n"], fp16. The states of p's stations move on, and their caches, for which advance() has been called before
-        where `advance` is not set."""
+        where `advance` is not set. A run that fails leaves the caches where they were; linear attention ahead of the call that
+        failed has moved its states on, so that the stations have to be forgotten if there is any."""
+        if not (advance and self.cached):
+            return self._blocks(p, stream)
+        before = self.past.copy()
+        self.advance(p, stream)
+        try:
+            self._blocks(p, stream)
+        except BaseException:
+            self.past[p["stations"]] = before[p["stations"]]
+            raise
+
+    def _blocks(self, p, stream):
         L, dim = hip.lib(), self.dim
-        if advance:
-            self.advance(p, stream)
 
         def norm(pre, f=None, b=None):
             a = hip.BlockNorm(f16=1, x=p["x"].ptr, ldx=dim, n=p["n"].ptr, ldn=dim, pre=hip.Norm(1, 1e-6, pre.ptr, None))

@@ -50,3 +50,23 @@ def test_clearing_waits(notes, cached, what):
     clears = [i for i, n in enumerate(names) if n == "bnh_memset"]
     assert names[0] == "bnh_device_sync"
     assert len(clears) == 2 - len(cached)
+
+
+@pytest.mark.parametrize("entry", ["bnh_block_norm", "bnh_pw_lora", "bnh_kv_append", "bnh_kv_select", "bnh_kv_attn"])
+def test_a_run_that_fails_does_not_move_the_caches(notes, entry):
+    """A call that is refused leaves each station's windows where they were, and its next run puts its rows there; pages that it has
+    been given stay its own."""
+    x = net(seen=3)
+    p, other = x.plan([20, 1], [0, 2]), x.plan([5], [1])
+    x.run(p)
+    x.run(other)
+    past, pages = list(x.past), len(x.free)
+    notes.fail = entry
+    with pytest.raises(hip.HipError):
+        x.run(p)
+    assert list(x.past) == past == [20, 5, 1]
+    assert len(x.free) == pages - 1  # the 33rd to 40th window's page
+    notes.fail = None
+    x.run(p)
+    assert list(x.past) == [40, 5, 2] and len(x.free) == pages - 1
+    assert sorted(x.free + [i for i in x.table.ravel() if i >= 0]) == list(range(x.pages))
