@@ -452,7 +452,7 @@ KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
   // tiles of 32 tokens that a row tile can see
   long long tok = (long long)c->ldt * c->page;
   if (p->nsel) tok = (long long)p->nsel * c->page;
-  else if (p->window && p->window + r.MR < tok) tok = p->window + r.MR;
+  else if (p->window && (long long)p->window + r.MR < tok) tok = (long long)p->window + r.MR;
   const long long tiles = bnh_ceil_div(tok, 32) + 1;
   // parts for the compute units where tiles leave some without work: one block each of the tiled form, with room for the last
   // parts of tiles (24 chunks of up to 120 rows: 37 + 13 us, 44 + 15 with 256), four of the other (64 rows over up to a day: 223 +

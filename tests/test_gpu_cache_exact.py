@@ -35,3 +35,17 @@ def test_mean_of_the_largest(hip, d, n):
     got = a.do.get()[0].reshape(a.c.rows, -1)
     for s in a.c.start:
         assert (got[s:s + n].astype(np.float32) == 65504).all()
+
+
+@pytest.mark.parametrize("f16,d,n", [(1, 64, 1), (1, 128, 200), (0, 64, 1), (0, 64, 100)])
+def test_a_window_wider_than_any_cache_in_parts(hip, f16, d, n):
+    """As no window: the same parts, the same output."""
+    say(f"widest window rows {n} d {d} f16 {f16}")
+    got = []
+    for window in (0, 2 ** 31 - 1):
+        a = Attn(hip, [2000, 40], [n, n], 3, 1, d, d, 64, f16, window=window, seed=n)
+        assert hip.lib().bnh_kv_attn_work_bytes(a.c.args(), a.args(), *a.c.seqs()[:3]) > 0
+        a.run()
+        a.check("window")
+        got.append(a.do.get()[0].copy())
+    assert np.array_equal(*got)
