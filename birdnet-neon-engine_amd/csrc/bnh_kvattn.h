@@ -10,8 +10,8 @@ struct KvaDev {
   const int32_t *sel;
   int ldq, ldo, G, window, nsel;  // G: query heads that share one of keys
   int want, least;                // parts of a split call in all, about, and tiles to one of them at least
-  float sc;                       // |scale| log2(e), above 0
-  bool neg;                       // scale < 0: queries are taken negative
+  float sc;                       // |scale| log2(e), above 0 (times it, -inf is -inf), and what queries are taken times: the
+  float sign;                     // scale's sign, 0 for a scale of 0
 };
 
 typedef float v4f __attribute__((ext_vector_type(4)));

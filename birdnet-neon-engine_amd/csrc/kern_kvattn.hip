@@ -55,7 +55,7 @@ __device__ __forceinline__ void kva_tile(const KvDev &c, const KvaDev &p, const 
 #pragma unroll
     for (int d = 0; d < DKT; d++) {
       qf[m][d] = kv_ld<T, 8, V>(q, 32 * d + 8 * q4, in ? c.dk : 0);
-      if (p.neg) qf[m][d] = -qf[m][d];
+      if (p.sign != 1.f) qf[m][d] *= (T)p.sign;
     }
   }
   // tokens
@@ -545,8 +545,8 @@ int bnh_kv_attn(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B, int row
   BNH_REQ(r.items < (1LL << 31));
   BNH_REQ(need == 0 || (work && kv_on(work, 16) && work_bytes >= need));
   const KvDev d = kv_dev(c, T, rows, start, len);
-  const float sc = fabsf(p->scale * 1.44269504f);  // a scale of 0 as one whose products round to 0
-  const KvaDev a = {p->q, p->o, p->sel, p->ldq, p->ldo, p->H / c->Hk, p->window, p->nsel, r.want, r.least, sc < 1e-37f ? 1e-37f : sc, p->scale < 0};
+  const float sc = p->scale == 0 ? 1.f : fabsf(p->scale * 1.44269504f), sign = p->scale == 0 ? 0.f : p->scale < 0 ? -1.f : 1.f;
+  const KvaDev a = {p->q, p->o, p->sel, p->ldq, p->ldo, p->H / c->Hk, p->window, p->nsel, r.want, r.least, sc, sign};
   const int ve = 16 / (int)es, cpl = r.tiled ? 8 : r.D / 16;
   bool v = c->dk % 8 == 0 && c->dv % cpl == 0 && c->k_ps % ve == 0 && c->v_ps % ve == 0 && p->ldq % ve == 0 &&
            p->ldo % (cpl < ve ? cpl : ve) == 0;

@@ -88,7 +88,7 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
 #pragma unroll
     for (int d = 0; d < DK / 16; d++) {
       qf[d] = kv_ld<T, 8, V>(q, 16 * d + 8 * hi, mine ? c.dk : 0);
-      if (p.neg) qf[d] = -qf[d];
+      if (p.sign != 1.f) qf[d] *= (T)p.sign;
     }
   }
   // this wave's rows see all of [all0, all1], and nothing outside [see0, see1]

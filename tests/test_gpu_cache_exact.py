@@ -49,3 +49,14 @@ def test_a_window_wider_than_any_cache_in_parts(hip, f16, d, n):
         a.check("window")
         got.append(a.do.get()[0].copy())
     assert np.array_equal(*got)
+
+
+@pytest.mark.parametrize("n", [1, 20, 100])
+@pytest.mark.parametrize("scale", [0.0, 5e-39, 2e-38, -6e-38, 2e-37])
+def test_small_scales_of_large_scores(hip, scale, n):
+    """fp32 products of 1e37 times a scale near fp32's smallest, or of 0: scores are what the two give."""
+    say(f"scale {scale} rows {n}")
+    scale = float(np.float32(scale))
+    a = Attn(hip, [90, 0], [n, n], 4, 2, 64, 64, 32, 0, seed=n, qstd=1e18, std=1e18, scale=scale)
+    a.run()
+    a.check(f"scale {scale}")
