@@ -20,12 +20,17 @@ struct AppDev {
   int ldk, ldv, ldq, ldr, G, rd, pairs;
 };
 
-// cos and sin of pos freq: the angle in turns in 64 bits, reduced to [-1/8, 1/8] of one about the nearest quarter, where the
-// series of sin and cos up to x^9 and x^10 are within 2e-9
+// cos and sin of pos freq: the angle in quarters of a turn, reduced to half a one about the nearest, where the series of sin and cos
+// up to x^9 and x^10 are within 2e-9. The angle (55 bits) and 2 / pi are in two parts each and whole turns go before the parts
+// are joined, so that a far position's angle is as exact as that of 0. In one part of 53 bits it is off by 2^-53 of itself at each of
+// three steps, five units of what 32 bits leave at position 2^31 (24 archives of 720 rows, 12 heads: 34.9 us so, 35.6 now)
 __device__ __forceinline__ void turn(int pos, float freq, float *cs, float *sn) {
-  const double t = (double)pos * (double)freq * 0.63661977236758134308;  // quarters: 2 / pi
-  const double n = __builtin_rint(t);
-  const float x = (float)((t - n) * 1.57079632679489661923), y = x * x;
+  constexpr double Q1 = 0x1.45f306dc9c883p-1, Q2 = -0x1.6b01ec5417056p-55;  // 2 / pi and what is left of it
+  const double a1 = (double)pos * (double)freq, a2 = __builtin_fma((double)pos, (double)freq, -a1);
+  const double t1 = a1 * Q1, t2 = __builtin_fma(a1, Q1, -t1) + __builtin_fma(a1, Q2, a2 * Q1);
+  const double t = __builtin_fma(-4.0, __builtin_rint(0.25 * t1), t1) + t2, n = __builtin_rint(t), r = t - n;
+  const int k = (int)n & 3;
+  const float x = (float)(r * 1.57079632679489661923), y = x * x;
   float s = __builtin_fmaf(y, 2.7557319e-6f, -1.9841270e-4f);
   s = __builtin_fmaf(y, s, 8.3333333e-3f);
   s = __builtin_fmaf(y, s, -1.6666667e-1f);
@@ -35,7 +40,6 @@ __device__ __forceinline__ void turn(int pos, float freq, float *cs, float *sn) 
   c = __builtin_fmaf(y, c, 4.1666667e-2f);
   c = __builtin_fmaf(y, c, -0.5f);
   c = __builtin_fmaf(y, c, 1.f);
-  const int k = (int)((long long)n & 3);
   const float a = k & 1 ? s : c, b = k & 1 ? c : s;
   *cs = k == 1 || k == 2 ? -a : a;
   *sn = k >= 2 ? -b : b;

@@ -545,8 +545,8 @@ typedef struct {
 } bnh_kvcache;
 /* The rotation of a row by its position: the first rd (even, <= dk) values of each head are pairs (x, y), values e and
  * e + rd/2 of the head (pairs 0) or 2e and 2e + 1 (pairs 1), e < rd/2, and become (x cos a - y sin a, x sin a + y cos a) with
- * a = position freq[e]; freq fp32 [rd/2]. pos int32 [rows]: the positions; NULL: past[i] + t. The angle is taken in 64 bits:
- * a position of 2^31 is as exact as one of 0. */
+ * a = position freq[e]; freq fp32 [rd/2]. pos int32 [rows]: the positions; NULL: past[i] + t. The angle is exact before it is
+ * reduced to a quarter of a turn, so that a position of 2^31 is as good as one of 0. */
 typedef struct {
   int rd, pairs;
   const float *freq;

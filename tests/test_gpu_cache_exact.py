@@ -1,9 +1,10 @@
-"""Cached attention where its precision shows: weights as factors of 22 bits in every form."""
+"""Cached attention where its precision shows: weights as factors of 22 bits in every form, scales near the smallest, far angles."""
 import numpy as np
 import pytest
 
-from test_gpu_cache import TWO, Attn
-from test_gpu_context import say
+import cache_ref as R
+from test_gpu_cache import TWO, Append, Attn
+from test_gpu_context import near, say
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +61,32 @@ def test_small_scales_of_large_scores(hip, scale, n):
     a = Attn(hip, [90, 0], [n, n], 4, 2, 64, 64, 32, 0, seed=n, qstd=1e18, std=1e18, scale=scale)
     a.run()
     a.check(f"scale {scale}")
+
+
+@pytest.mark.parametrize("pairs", [0, 1])
+@pytest.mark.parametrize("first", [1.0, 0.37, 3e4, 2e6])
+def test_far_angles(hip, first, pairs):
+    """An angle is as exact at positions of 2^31 as near 0: against cos and sin of products that 64 bits of mantissa hold whole
+    (31 + 24 bits), within the bound of 32-bit arithmetic on exact angles."""
+    say(f"far angles {first} pairs {pairs}")
+    assert np.finfo(np.longdouble).nmant >= 63
+
+    def pos(c):
+        p = np.random.default_rng(3).integers(-2 ** 31, 2 ** 31, c.rows)
+        p[:5] = 2 ** 31 - 1, -2 ** 31, 0, 1, 2 ** 30 + 1
+        return p
+
+    a = Append(hip, [3, 0], [400, 150], 1, 1, 256, 8, 256, pairs, 16, 0, pos=pos, seed=pairs)
+    a.freq = (first * np.geomspace(1, 1e-3, 128)).astype(np.float32)
+    a.dfreq.upload(a.freq)
+    a.run()
+    got = a.dqr.get()[0].reshape(a.c.rows, 256).astype(np.float64)
+    e = np.arange(128)
+    i, j = (2 * e, 2 * e + 1) if pairs else (e, e + 128)
+    for s, n in zip(a.c.start, a.c.lens):
+        t = a.pos[s:s + n].astype(np.longdouble)[:, None] * a.freq.astype(np.longdouble)
+        x, y = (a.q[s:s + n, 0][:, k].astype(np.float64) for k in (i, j))
+        cs, sn = np.cos(t).astype(np.float64), np.sin(t).astype(np.float64)
+        err = 6 * R.U * (np.abs(x) + np.abs(y))
+        near(got[s:s + n][:, i], x * cs - y * sn, err, "x")
+        near(got[s:s + n][:, j], x * sn + y * cs, err, "y")
