@@ -32,6 +32,8 @@ class ContextNet:
             raise ValueError(f"cached blocks {cached} of {layers}")
         if windows < 1 or not 16 <= page <= 1024 or page & (page - 1) or (pages is not None and pages < 1):
             raise ValueError(f"a cache of {pages} pages of {page}, up to {windows} windows a station")
+        if -(-windows // page) * page >= (1 << 31) - 1024:
+            raise ValueError(f"{windows} windows a station: below 2^31 - 1024 of them")
         if seen and not 3 <= seen <= 1 << 20:
             raise ValueError(f"{seen} pages seen: 3 at least, the first and the last two among them, or 0 for all")
         self.dim, self.heads, self.layers, self.stations, self.rank = dim, heads, layers, stations, rank

@@ -70,3 +70,16 @@ def test_a_run_that_fails_does_not_move_the_caches(notes, entry):
     x.run(p)
     assert list(x.past) == [40, 5, 2] and len(x.free) == pages - 1
     assert sorted(x.free + [i for i in x.table.ravel() if i >= 0]) == list(range(x.pages))
+
+
+@pytest.mark.parametrize("page", [16, 1024])
+def test_as_many_windows_as_a_table_can_have(notes, page):
+    """A station's tokens are numbered in 31 bits: what no call would take is refused when the net is made."""
+    most = ((1 << 31) - 1024 - 1) // page * page
+    for n in (most + 1, 1 << 31, 1 << 40):
+        with pytest.raises(ValueError, match="windows"):
+            net(windows=n, page=page, pages=8, cached=[0], stations=1)
+        assert not notes.calls
+    if page == 1024:
+        x = net(windows=most, page=page, pages=8, cached=[0], stations=1)
+        assert x.ldt * page < (1 << 31) - 1024
