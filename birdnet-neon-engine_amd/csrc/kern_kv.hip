@@ -9,9 +9,9 @@ namespace {
 // ---------------------------------------------------------------------------------------------- append
 // Bound by HBM: q, k and v are read once and written once. A block owns the new rows of one page for one head of keys, with the
 // query heads that read it, so that the page's bounds need no atomics: its threads are `nu` units of a head (VEC values,
-// with their partners VEC more) side by side, times as many rows as fit 256. 24 archives of 720 rows, 12 heads of 128, 162 MB: 36 us,
-// 4.5 TB/s, of which the angles are 6; 8 of up to 500 rows of odd widths in fp32, value by value: 21 us, 2.5 TB/s; live rows 6 to 7,
-// a launch and two loads that wait for each other.
+// with their partners VEC more) side by side, times as many rows as fit 256. 24 archives of 720 rows, 12 heads of 128, 162 MB: 50 us,
+// 3.2 TB/s, of which the angles are 6 (36 us for the same buffers again, which the last-level cache holds); 8 of up to 500 rows of odd
+// widths in fp32, value by value: 21 us, 2.5 TB/s; live rows 6 to 7, a launch and two loads that wait for each other.
 struct AppDev {
   const void *k, *v, *q;
   void *qr;
@@ -23,7 +23,7 @@ struct AppDev {
 // cos and sin of pos freq: the angle in quarters of a turn, reduced to half a one about the nearest, where the series of sin and cos
 // up to x^9 and x^10 are within 2e-9. The angle (55 bits) and 2 / pi are in two parts each and whole turns go before the parts
 // are joined, so that a far position's angle is as exact as that of 0. In one part of 53 bits it is off by 2^-53 of itself at each of
-// three steps, five units of what 32 bits leave at position 2^31 (24 archives of 720 rows, 12 heads: 34.9 us so, 35.6 now)
+// three steps, five units of what 32 bits leave at position 2^31 (24 archives of 720 rows, 12 heads: 49.4 us so, 50.3 now)
 __device__ __forceinline__ void turn(int pos, float freq, float *cs, float *sn) {
   constexpr double Q1 = 0x1.45f306dc9c883p-1, Q2 = -0x1.6b01ec5417056p-55;  // 2 / pi and what is left of it
   const double a1 = (double)pos * (double)freq, a2 = __builtin_fma((double)pos, (double)freq, -a1);
@@ -237,9 +237,9 @@ __device__ __forceinline__ bool sel_row(const KvDev &c, int window, int b0, int 
 }
 
 // The scores of PPB pages for one row and head of keys: 16 lanes a page, 8 values each a step. Bound by reading the bounds
-// (4 dk bytes a page and head in fp16); the products are exact in 64 bits and their sums good to 2^-50, so that no order of
-// sums can make another choice. One row over 1,890 pages of 4 heads of 128: 8.2 us; 16 rows over up to 810: 13.4; 144 rows of 2
-// heads of 72 over up to 188, fp32: 10.7.
+// (4 dk bytes a page and head in fp16). The products are exact in 64 bits; a sum of n of them is off by n 2^-53 of its terms' sizes
+// at most, and always in the same order, which decides between scores that are closer. One row over 1,890 pages of 4 heads of 128:
+// 9.4 us; 16 rows over up to 810: 14.2; 144 rows of 2 heads of 72 over up to 188, fp32: 11.4.
 constexpr int PPB = 64;
 template <typename T, bool V>
 __global__ __launch_bounds__(256) void k_kv_score(KvDev c, SelDev p, int npb, int b0, int t0, u64 *key) {
@@ -500,7 +500,7 @@ int bnh_kv_append(const bnh_kvcache *c, const bnh_rotary *r, const void *k, int 
   const int rd = r ? r->rd : 0, pairs = r ? r->pairs : 0, ve = 16 / (int)es;
   const AppDev p = {k, v, q, qr, r ? r->freq : nullptr, r ? r->pos : nullptr, ldk, ldv, ldq, ldr, q ? H / c->Hk : 0, rd, pairs};
   // values of q and k at a time: as many as widths, strides and addresses allow (24 archives of 720 rows, 12 heads, fp16, us: 128
-  // by eights 35; 120 by fours 39, one by one 56; 108 by twos 39 and 57; fp32, 108 by twos 73 and 119)
+  // by eights 50, one by one 86; 120 by fours 59 and 88; 108 by twos 57 and 86; fp32, 108 by twos 83 and 129)
   auto fits = [&](int n) {
     bool x = c->dk % (2 * n) == 0 && rd % (2 * n) == 0 && c->k_ps % n == 0 && ldk % n == 0;
     x = x && (!q || (ldq % n == 0 && ldr % n == 0)) && kv_on(c->lo, 4) && kv_on(c->hi, 4);

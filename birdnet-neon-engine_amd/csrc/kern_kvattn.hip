@@ -18,9 +18,9 @@ __device__ __forceinline__ v4f mma(kv_vec<float, 8> a, kv_vec<float, 8> b, v4f c
   return c;
 }
 // The streaming form, for few rows and for rows with a selection: bound by reading keys and values (64 rows over up to a day,
-// 1.15 GB: 223 us, 5.2 TB/s; a copy 5.1), and by the latency of its steps where there is little to read (12 heads of one row over a
-// day, 106 MB: 22 us and 7 for the join; 32 pages of a week 10 and 4). Four waves of a block take tiles of 32 tokens in turn, straight from memory into the matrix
-// instructions' registers: the scores' product has keys as its rows in such an order that a lane ends with the scores of 8 tokens
+// 1.15 GB: 224 us, 5.1 TB/s; a copy 5.1), and by the latency of its steps where there is little to read (12 heads of one row over a
+// day, 106 MB: 29 us and 7 for the join; 32 pages of a week 12 and 4). Four waves of a block take tiles of 32 tokens in turn,
+// straight from memory into the matrix instructions' registers: the scores' product has keys as its rows in such an order that a lane ends with the scores of 8 tokens
 // in a row, 8 q4 .. 8 q4 + 7 (q4 = lane / 16), for query lane & 15, which is what the second product's operand holds; values are
 // loaded as 8 tokens by CPL columns a lane and change places within the lane. Each wave has its own maximum and sums, joined at
 // the end over waves, and over the blocks of a split by k_kva_join. fp16: e^{s - m} goes into the product in two parts, 22 bits,
@@ -432,10 +432,12 @@ KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
   const int d = c->dk > c->dv ? c->dk : c->dv, G = p->H / c->Hk;
   const long long m = p->nsel ? G : (long long)T * G;
   r.D = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
-  // The tiled form's waves have 32 rows each, and 128 or 256 to a block; the other one's time goes up at 17 rows and at 65. fp16,
-  // 24 stations' caches of up to 5,000 tokens and 4 heads of 128: 16 rows 22.4 us tiled and 19.8, 24 rows 22.7 and 31.0; one of a
-  // day and 12 heads: 34.1 and 29.9, 34.2 and 58.1. Heads of 256: 24 rows 37.2 and 35.6, 48 rows 40.7 and 53.6. fp32, whose
-  // products take as long as rows that are nobody's: 48 rows 63.3 and 63.2, 165 and 152; 96 rows 66.9 and 80.4
+  // The tiled form's waves have 32 rows each, and 128 or 256 to a block; the other one's time goes up at 17 rows and at 65, past 128
+  // wide at 33. Tiled and the other, us, for 24 stations' caches of up to 5,000 tokens and 4 heads, and one of a day and 12 heads.
+  // fp16, 64 wide: 16 rows 20.8 and 16.5, 34.1 and 21.6; 17 rows 20.8 and 25.9, 34.3 and 43.4. 128: 25.4 and 20.7, 40.9 and 30.0; 25.3
+  // and 30.3, 40.8 and 57.7. 136: 32 rows 38.3 and 40.6, 86.3 and 73.6; 33 rows 39.3 and 43.8, 88.2 and 131.5. 192: 39.0 and 33.7, 87.0
+  // and 62.3; 39.7 and 38.1, 89.2 and 107.9. 256: 40.5 and 36.3, 89.6 and 67.4; 40.8 and 40.0, 91.5 and 119.5. fp32, whose products
+  // take as long for rows that are nobody's: 64 rows of 128 63.4 and 65.0, 167 and 150; 65 rows 63.8 and 72.5, 166 and 185
   r.tiled = !p->nsel && m > (!c->f16 ? 64 : d <= 128 ? 16 : 32);
   r.TK = 32;
   if (r.tiled) {
@@ -455,7 +457,7 @@ KvaPlan plan(const bnh_kvcache *c, const bnh_kvattn *p, int T, int B) {
   else if (p->window && (long long)p->window + r.MR < tok) tok = (long long)p->window + r.MR;
   const long long tiles = bnh_ceil_div(tok, 32) + 1;
   // parts for the compute units where tiles leave some without work: one block each of the tiled form, with room for the last
-  // parts of tiles (24 chunks of up to 120 rows: 37 + 13 us, 44 + 15 with 256), four of the other (64 rows over up to a day: 223 +
+  // parts of tiles (24 chunks of up to 120 rows: 54 us with the join, 63 with 256), four of the other (64 rows over up to a day: 223 +
   // 6 us, 229 + 6 with 768, 241 + 5 with 512), of 512 tokens at least, or what is joined costs more (one row over a day: 24 + 7 us
   // in 406 parts, 23 + 9 in 732)
   r.want = r.tiled ? 192 : 1024;

@@ -1,12 +1,12 @@
 // Attention of many rows over a paged cache (bnh_kv_attn): the tiled form.
 //
 // Bound by the matrix cores, the exponentials and what feeds both out of LDS, at the clock that the card's power leaves: 17,280
-// rows of 12 heads of 128 from an empty cache 915 to 970 us on different cards, 950 to 1,000 TFLOP/s (a library product of 8,192
-// cubed 1,164), the matrix cores busy for 47% of the cycles, no bank conflict. fp32 4,000 rows 561 us, 88 of 154 TFLOP/s. Short
-// calls are bound by what a block does before its first tile, about 14,000 cycles, and by the join of parts: 24 chunks of up to 120
-// rows over up to 5,000 tokens 35 + 13 us. The NW waves of a block own 32 rows each (query
-// heads that share keys are rows too) and share tiles of TK tokens in LDS, which pass through registers while the tile before is
-// multiplied. Scores are K q^T, so that a lane has tokens of one query (lane & 31): maxima and sums stay in the lane but for
+// rows of 12 heads of 128 from an empty cache 1,290 to 1,320 us, 700 TFLOP/s of the two products and 1,050 with the weights' second
+// part (a library product of 8,192 cubed 1,164), the matrix cores busy for 56% of the cycles, no bank conflict. fp32 4,000 rows 565 us,
+// 87 of 153 TFLOP/s. Short calls are bound by what a block does before its first tile, about 14,000 cycles, and by the join of parts:
+// 24 chunks of up to 120 rows over up to 5,000 tokens 41 + 13 us. The NW waves of a block own 32 rows each (query heads that share
+// keys are rows too) and share tiles of TK tokens in LDS, which loads bring there while the tile before is multiplied (by way of
+// registers for odd widths of fp16, and where values are not finite). Scores are K q^T, so that a lane has tokens of one query (lane & 31): maxima and sums stay in the lane but for
 // one exchange, and the exponentials are the second product's operand as they lie, given that row m of the first product is
 // token m with bits 2 and 3 exchanged. Rows of LDS are pieces of 16 bytes, exchanged by bits of the token such that neither the
 // reads of 16 tokens' pieces nor the transposing reads of 4 tokens meet in a bank.
@@ -47,10 +47,10 @@ __device__ __forceinline__ float both(float x) {
 }
 // fp16: the waves of a block are two groups, one wave of each on every SIMD, half a tile apart: while one multiplies (its
 // last tile's values and the next one's scores), the other takes exponentials. Waves in step would all want the matrix cores
-// and then all want the exponentials: 17,280 rows of 12 heads of 128 took 1,292 us so. fp32 products take ten times as
+// and then all want the exponentials: 17,280 rows of 12 heads of 128 take 1,438 us so, not 1,315. fp32 products take ten times as
 // long as the exponentials, and the groups go in step.
 // W: bytes of a lane's load, which everything is aligned to: 16, 4, or 2 (odd widths of fp16), where all goes through registers.
-// 8,000 rows of 12 heads of 128 and 126: 268 us by fours, 512 us through registers; fp32, 16 heads of 64 and 97, 256 tokens seen:
+// 8,000 rows of 12 heads of 128 and 126: 332 us by fours, 595 us through registers; fp32, 16 heads of 64 and 97, 256 tokens seen:
 // 53 us and 68
 template <typename T, int DK, int DV, int NW, int NG, int W>
 __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const KvaItem &it, int nrt, int2 *counts, float *part,
@@ -119,7 +119,7 @@ __device__ __forceinline__ void kvt_item(const KvDev &c, const KvaDev &p, const 
   // The work on a tile
   v16f s[ST];
   // fp16: weights in two parts, 22 bits, and a product for each. In one part's 11 bits outputs whose terms cancel are off by several
-  // times their own rounding (17,280 rows of 12 heads of 128: 966 us so, 1,300 with both; 24 chunks of up to 120 rows 48 and 53)
+  // times their own rounding (17,280 rows of 12 heads of 128: 976 us so, 1,315 with both; 24 chunks of up to 120 rows 48 and 54)
   FV ph[2 * ST], pl[F16 ? 2 * ST : 1];
   // A tile is NG groups of GT tokens that have a page each: one for pages of TK tokens or more, else groups of 16
   int pc[NG];
