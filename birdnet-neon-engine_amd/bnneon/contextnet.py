@@ -132,7 +132,9 @@ class ContextNet:
     def _plan_cached(self, p):
         """The descriptors of the cached blocks, and the workspace that they need."""
         L, d, n, H = hip.lib(), self.dim // self.heads, 0, self.heads
-        p["table"], p["past"] = hip.DeviceArray((p["B"], self.ldt), np.int32), hip.DeviceArray((p["B"],), np.int32)
+        # no pages until advance() writes them: a run ahead of it stores nothing
+        p["table"] = hip.DeviceArray.from_host(np.full((p["B"], self.ldt), -1, np.int32))
+        p["past"] = hip.DeviceArray.zeros((p["B"],), np.int32)
         p["sel"] = hip.DeviceArray((p["rows"], H, self.seen), np.int32) if self.seen else None
         p["kv"], q = {}, p["qkvg"].ptr
         for i, c in self.cache.items():

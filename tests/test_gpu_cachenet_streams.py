@@ -42,3 +42,24 @@ def test_a_station_starts_again_between_streams(hip, cached, seen):
     for a, b in zip(*results):
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
     assert np.isfinite(results[0][0][0]).all()
+
+
+def test_a_run_ahead_of_its_pages_stores_nothing(hip):
+    """A run without advance() whose plan has been given no pages yet: no station's cache changes."""
+    from bnneon import contextnet
+    say("ahead of its pages")
+    net = contextnet.ContextNet(dim=64, heads=2, layers=1, stations=3, rank=2, cached=[0], windows=100, page=16)
+    x = np.random.default_rng(1).standard_normal((90, 64)).astype(np.float32)
+    p = net.plan([30, 30, 30], range(3))
+    p["x"].upload(x)
+    net.run(p)
+    hip.sync()
+    before = [net.cache[0][k].numpy() for k in "kv"]
+    other = net.plan([40, 50], [2, 0])
+    other["x"].upload(x)
+    net.run(other, advance=False)
+    hip.sync()
+    assert (other["table"].numpy() == -1).all() and not other["past"].numpy().any()
+    for a, k in zip(before, "kv"):
+        assert np.array_equal(a, net.cache[0][k].numpy())
+    assert list(net.past) == [30, 30, 30]
